@@ -28,6 +28,10 @@ ACH_ENAN = -5
 
 LOGISTIC, RELU, LINEAR, LEAKY = 0, 1, 3, 7
 
+F32, BF16, F16 = 0, 1, 2  # element types of logits
+TOP_MAX = 128
+DISTILL_RENORM, DISTILL_TAIL = 0, 1
+
 AN_CONVOLUTIONAL, AN_MAXPOOL, AN_AVGPOOL, AN_DROPOUT, AN_SOFTMAX = 0, 1, 2, 3, 4
 
 # an_policy (the reference's LearningRatePolicy order)
@@ -40,6 +44,7 @@ _i = C.c_int
 _f = C.c_float
 _u64 = C.c_uint64
 _u32 = C.c_uint32
+_i64 = C.c_int64
 
 
 class ConvDesc(C.Structure):
@@ -77,6 +82,17 @@ class Augment(C.Structure):
 class FilterJob(C.Structure):
     """ach_filter_job"""
     _fields_ = [("desc", ConvDesc), ("w", _vp), ("wt", _vp), ("wft", _vp)]
+
+
+class LogitsDesc(C.Structure):
+    """ach_logits_desc; stride 0 (the default) means classes"""
+    _fields_ = [("rows", _i), ("classes", _i), ("type", _i), ("temperature", _f),
+                ("stride", _i64)]
+
+
+class DistillDesc(C.Structure):
+    """ach_distill_desc"""
+    _fields_ = [("k", _i), ("mode", _i), ("teacher_type", _i), ("soft", _f), ("hard", _f)]
 
 
 # name -> (restype, argtypes)
@@ -162,6 +178,14 @@ _OPS = {
     "ach_avgpool_bwd": (_i, [_vp, _i, _i, _i, _vp, _vp]),
     "ach_softmax_workspace": (_sz, [_i, _i]),
     "ach_softmax_xent": (_i, [_vp, _i, _i, _i, _f, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ach_logprobs_workspace": (_sz, [C.POINTER(LogitsDesc), _i]),
+    "ach_logprobs_fwd": (_i, [C.POINTER(LogitsDesc), _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp,
+                              _vp, _sz, _vp]),
+    "ach_logprobs_bwd": (_i, [C.POINTER(LogitsDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+                              _vp]),
+    "ach_distill_workspace": (_sz, [C.POINTER(LogitsDesc), C.POINTER(DistillDesc)]),
+    "ach_distill_xent": (_i, [C.POINTER(LogitsDesc), C.POINTER(DistillDesc), _vp, _vp, _vp, _vp,
+                              _vp, _vp, _vp, _i64, _vp, _vp, _sz, _vp]),
     "ach_dropout_uniform": (_f, [_u64, _u32, _u32, _u32]),
     "ach_dropout_fwd": (_i, [_vp, _sz, _f, _u64, _u32, _u32, _vp]),
     "ach_dropout_bwd": (_i, [_vp, _sz, _f, _u64, _u32, _u32, _vp]),

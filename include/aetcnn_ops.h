@@ -386,6 +386,96 @@ int ach_softmax_xent(const float *in, int batch, int inputs, int groups,
                      float *output, float *delta, float *error, float *cost,
                      void *ws, size_t ws_bytes, ach_stream_t stream);
 
+/* ---- operators on logits: log probabilities, distillation -----------------
+ * No counterpart in the reference, whose softmax layer (SoftMaxLayer.c:
+ * 47-119) knows one-hot truth and whose answers are probabilities and a top-k
+ * taken on the host (DnnUtils.c:463-477).
+ *
+ * `logits` holds `rows` rows of `classes` values of `type`, row r at element
+ * r*stride (stride 0: classes; else >= classes; what lies between the rows is
+ * neither read nor written).  Any element address will do; rows may be 0.
+ * z = x/temperature (positive, 1e-6 to 1e6).  Everything is computed in 32
+ * bits or more and rounded once, to nearest even, where an output has fewer;
+ * results do not depend on the run (no float atomics).
+ *  - a logit of -inf is a masked class: its probability is 0
+ *  - a row whose logits are all -inf has no distribution: log probabilities
+ *    are -inf, ranks 0, the entropy, losses and gradients 0
+ *  - a row with a NaN or a +inf gives NaN, and ranks and top ids of -1
+ *  - a class id outside [0, classes) stands for "none" (padding)           */
+#define ACH_F32 0
+#define ACH_BF16 1
+#define ACH_F16 2
+#define ACH_TOP_MAX 128 /* most alternatives, or teacher entries, of a row  */
+typedef struct {
+    int rows, classes;
+    int type;             /* ACH_F32, ACH_BF16 or ACH_F16                    */
+    float temperature;
+    int64_t stride;       /* elements from one row to the next; 0: classes   */
+} ach_logits_desc;
+/* Any of the outputs may be NULL (top_ids and top_logprobs only with k 0):
+ *   logprobs[r]   log softmax(z)[ids[r]]; 0 where ids[r] is none
+ *   ranks[r]      number of classes with a larger logit than ids[r]'s; -1
+ *                 where it is none
+ *   entropy[r]    -sum p log p
+ *   stats[r][2]   {max of x, log sum exp((x - max)/temperature)}, which
+ *                 ach_logprobs_bwd reads
+ *   top_ids[r][k], top_logprobs[r][k]
+ *                 the k (at most ACH_TOP_MAX and classes) largest logits,
+ *                 largest first, equal ones by ascending id
+ * ids may be NULL if logprobs and ranks are.                               */
+size_t ach_logprobs_workspace(const ach_logits_desc *d, int k);
+int ach_logprobs_fwd(const ach_logits_desc *d, const void *logits, const int32_t *ids, int k,
+                     float *logprobs, int32_t *ranks, float *entropy, float *stats,
+                     int32_t *top_ids, float *top_logprobs, void *ws, size_t ws_bytes,
+                     ach_stream_t stream);
+/* dlogits[r][j] = 1/temperature * (dlogprobs[r]*([j == ids[r]] - p_j)
+ *                                  - dentropy[r]*p_j*(log p_j + entropy[r]))
+ * from the stats and (with dentropy) the entropy of ach_logprobs_fwd.
+ * dlogprobs (with ids) or dentropy may be NULL, not both.  dlogits has the
+ * logits' type and rows dstride apart (0: classes); it may be `logits`
+ * itself with the same stride.  Rows whose ids[r] is none take no gradient
+ * from dlogprobs[r]; rows with no gradient to take (that and/or zeros) are
+ * set to 0 without reading their logits, whatever these hold.              */
+int ach_logprobs_bwd(const ach_logits_desc *d, const void *logits, const int32_t *ids,
+                     const float *stats, const float *entropy, const float *dlogprobs,
+                     const float *dentropy, void *dlogits, int64_t dstride, ach_stream_t stream);
+/* Distillation.  The teacher of row r is k entries (teacher_ids[r][k],
+ * teacher_values[r][k] of teacher_type); entries whose id is none or repeats
+ * an earlier one of the row are dropped.  With q = softmax(z):
+ *   ACH_DISTILL_RENORM  values are logits, or log probabilities at
+ *       temperature 1: p = softmax(values/temperature) over the row's
+ *       entries; KD = sum p_i (log p_i - log q_i), 0 where no entry is left
+ *   ACH_DISTILL_TAIL    values are log probabilities at this temperature
+ *       (top_logprobs of ach_logprobs_fwd): p = exp(values), and all other
+ *       classes form one more entry, of p_rest = max(0, 1 - sum p) against
+ *       q_rest = their sum of q; KD = sum p_i (log p_i - log q_i)
+ *       + p_rest (log p_rest - log q_rest), without the last term where q_rest
+ *       has no class of finite logit
+ *   loss[r] = row_weights[r] * (soft*temperature^2*KD
+ *                               - hard*log softmax(x)[labels[r]])
+ *   delta[r][j] = -d loss[r] / d x[r][j]   (the sign of ach_softmax_xent)
+ *   *cost = sum of loss[r] (in double, rounded once)
+ * Either term is left out where its factor is 0 (soft: the teacher may then
+ * be NULL and k 0; hard: labels may be NULL); a label that is none has no
+ * second term.  row_weights NULL: 1; rows of weight 0 are set to 0 without
+ * reading their logits.  delta (of the logits' type, rows delta_stride apart,
+ * 0: classes; it may be `logits` itself with the same stride), loss and cost
+ * may be NULL, not all three; cost and delta need no loss array.           */
+#define ACH_DISTILL_RENORM 0
+#define ACH_DISTILL_TAIL 1
+typedef struct {
+    int k;                /* teacher entries per row, up to ACH_TOP_MAX      */
+    int mode;
+    int teacher_type;     /* of teacher_values                               */
+    float soft, hard;
+} ach_distill_desc;
+size_t ach_distill_workspace(const ach_logits_desc *d, const ach_distill_desc *t);
+int ach_distill_xent(const ach_logits_desc *d, const ach_distill_desc *t, const void *logits,
+                     const int32_t *teacher_ids, const void *teacher_values,
+                     const int32_t *labels, const float *row_weights, float *loss, void *delta,
+                     int64_t delta_stride, float *cost, void *ws, size_t ws_bytes,
+                     ach_stream_t stream);
+
 /* ---- dropout (DropoutLayer.c:55-86) ---------------------------------------
  * r = u(seed, iter, layer, i) from a counter-based generator (SplitMix64
  * finaliser, top 24 bits); r < p -> 0 else x * 1/(1-p).  Same mask forward
