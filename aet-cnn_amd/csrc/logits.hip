@@ -16,6 +16,13 @@
 namespace ach {
 namespace {
 
+#ifndef UNROLL
+#define UNROLL 4
+#endif
+#ifndef T64
+#define T64 2048
+#define T256 16384
+#endif
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 // An element type: 16 bytes of it as one load from any element's address.
@@ -55,6 +62,7 @@ __device__ __forceinline__ uint64_t compound(float x, int j)
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Combines v over the wave; every lane gets the result.
 template <class V, class F> __device__ __forceinline__ V wave_all(V v, F f)
 {
 #pragma unroll
@@ -68,22 +76,52 @@ struct Add {
 struct Max {
     template <class V> __device__ V operator()(V a, V b) const { return a > b ? a : b; }
 };
-struct Min {
-    template <class V> __device__ V operator()(V a, V b) const { return a < b ? a : b; }
-};
 
-// Combines v over the workgroup in a fixed order; every thread gets the
-// result.  sh holds one V per wave and may be used again at once.
-template <int NT, class V, class F> __device__ __forceinline__ V block_all(V v, V *sh, F f)
+// The same for 32 bits without the LDS crossbar: within rows of 16 lanes by
+// shifts, then from row to row; lane 63 has seen all.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp(float old, float v)
 {
-    v = wave_all(v, f);
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL,
+                                                      ROWS, 0xf, false));
+}
+__device__ __forceinline__ float lane_value(float v, int lane)
+{
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+__device__ __forceinline__ float wave_total(float v)
+{
+    v += dpp<0x111, 0xf>(0.f, v);
+    v += dpp<0x112, 0xf>(0.f, v);
+    v += dpp<0x114, 0xf>(0.f, v);
+    v += dpp<0x118, 0xf>(0.f, v);
+    v += dpp<0x142, 0xa>(0.f, v);
+    v += dpp<0x143, 0xc>(0.f, v);
+    return lane_value(v, 63);
+}
+__device__ __forceinline__ float wave_most(float v)
+{
+    v = fmaxf(v, dpp<0x111, 0xf>(v, v));
+    v = fmaxf(v, dpp<0x112, 0xf>(v, v));
+    v = fmaxf(v, dpp<0x114, 0xf>(v, v));
+    v = fmaxf(v, dpp<0x118, 0xf>(v, v));
+    v = fmaxf(v, dpp<0x142, 0xa>(v, v));
+    v = fmaxf(v, dpp<0x143, 0xc>(v, v));
+    return lane_value(v, 63);
+}
+
+// Sum of v over the workgroup; every thread gets it.  sh holds one V per
+// wave and may be used again at once.
+template <int NT, class V> __device__ __forceinline__ V block_sum(V v, V *sh)
+{
+    v = wave_all(v, Add());
     if (NT == 64) return v;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
     __syncthreads();
     V r = sh[0];
 #pragma unroll
-    for (int i = 1; i < NT / 64; ++i) r = f(r, sh[i]);
+    for (int i = 1; i < NT / 64; ++i) r += sh[i];
     return r;
 }
 
@@ -102,7 +140,8 @@ template <int TYPE> struct Range {
 // A thread's running statistics of the logits it has seen: their maximum m
 // (-FLT_MAX before the first finite one, which a logit of -inf leaves there:
 // its exponential is 0 either way), s = sum exp2((x - m) c) and, for the
-// entropy, t = sum exp2((x - m) c) (x - m) c.  A NaN or +inf makes s a NaN.
+// entropy, t = sum exp2((x - m) c) (x - m) c; and its wave's count of logits
+// above the given one.  A NaN or +inf makes s a NaN.
 struct Stat {
     float m, s, t;
     int above;
@@ -119,50 +158,68 @@ __device__ __forceinline__ void raise(Stat &a, float m, float c)
     a.m = m;
 }
 
-template <int N> __device__ __forceinline__ void absorb(Stat &a, const float (&x)[N], float c,
-                                                        float x_id)
+// N logits of each lane, all lanes taking part.  Masked logits make the plain
+// sum for t a NaN, 0 * -inf: then it is formed again without them.
+template <bool ENTROPY, bool RANK, int N>
+__device__ __forceinline__ void absorb(Stat &a, const float (&x)[N], float c, float x_id)
 {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
     if (m > a.m) raise(a, m, c);
+    float t = a.t;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const float d = (x[i] - a.m) * c, e = exp2_fast(d);
         a.s += e;
-        a.t = fmaf(e, fmaxf(d, FAR), a.t);
-        a.above += x[i] > x_id;
+        if (ENTROPY) t = fmaf(e, d, t);
+        if (RANK) a.above += __popcll(__ballot(x[i] > x_id));
+    }
+    if (ENTROPY) {
+        if (t != t) {
+            t = a.t;
+            for (int i = 0; i < N; ++i) {
+                const float d = fmaxf((x[i] - a.m) * c, FAR);
+                t = fmaf(exp2_fast(d), d, t);
+            }
+        }
+        a.t = t;
     }
 }
 
-template <int TYPE, int NT>
+template <int TYPE, int NT, bool ENTROPY, bool RANK>
 __device__ __forceinline__ Stat stream(const Range<TYPE> &g, float c, float x_id)
 {
-    constexpr int V = Row<TYPE>::VEC, U = 4;
+    constexpr int V = Row<TYPE>::VEC, U = UNROLL;
+    typedef typename Row<TYPE>::Chunk Chunk;
     Stat a = {-FLT_MAX, 0.f, 0.f, 0};
-    const int n = g.chunks();
-    int q = threadIdx.x;
-    float x[U * V];
-    for (; q + (U - 1) * NT < n; q += U * NT) {
-        typename Row<TYPE>::Chunk v[U];
+    const int n = g.chunks(), lane = threadIdx.x & 63;
+    int q = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);  // the wave's first chunk
+    for (; q + (U - 1) * NT + 64 <= n; q += U * NT) {
+        Chunk v[U];
+        float x[U * V];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = Row<TYPE>::load(g.p + (size_t)(q + u * NT) * V);
+        for (int u = 0; u < U; ++u) v[u] = Row<TYPE>::load(g.p + (size_t)(q + u * NT + lane) * V);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < V; ++i) x[u * V + i] = (float)v[u][i];
-        absorb(a, x, c, x_id);
+        absorb<ENTROPY, RANK>(a, x, c, x_id);
     }
     for (; q < n; q += NT) {
-        float y[V];
-        const typename Row<TYPE>::Chunk v = Row<TYPE>::load(g.p + (size_t)q * V);
+        float x[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = (float)v[i];
-        absorb(a, y, c, x_id);
+        for (int i = 0; i < V; ++i) x[i] = -INFINITY;
+        if (q + lane < n) {
+            const Chunk v = Row<TYPE>::load(g.p + (size_t)(q + lane) * V);
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = (float)v[i];
+        }
+        absorb<ENTROPY, RANK>(a, x, c, x_id);
     }
-    if (threadIdx.x < g.rest()) {
-        const float y[1] = {(float)g.p[(size_t)n * V + threadIdx.x]};
-        absorb(a, y, c, x_id);
+    if (threadIdx.x < 64) {
+        const float x[1] = {lane < g.rest() ? (float)g.p[(size_t)n * V + lane] : -INFINITY};
+        absorb<ENTROPY, RANK>(a, x, c, x_id);
     }
     return a;
 }
@@ -175,50 +232,88 @@ struct Total {
     int above;
 };
 
+// A wave's statistics; `own` is the part of the sum of the first thread that
+// has seen the maximum, whose exponential, 1, it contains.
+struct WaveStat {
+    float m, own, others, t;
+    int above, owner;
+};
+
 template <int NT> struct StatLds {
-    float f[NT / 64];
-    int i[NT / 64];
-    float own;
+    WaveStat wave[NT / 64];
+    float rest;
 };
 
 // m is -inf where every logit is; rest is NaN where one is NaN or +inf.
 template <int TYPE, int NT>
-__device__ Total total_of(const Range<TYPE> &g, Stat a, float c, StatLds<NT> &sh)
+__device__ __forceinline__ Total total_of(const Range<TYPE> &g, Stat a, float c, StatLds<NT> &sh)
 {
-    const float mine = a.m;
-    const float m = block_all<NT>(a.m, sh.f, Max());
-    const int owner = block_all<NT>(mine == m ? (int)threadIdx.x : NT, sh.i, Min());
-    if (a.m != m) raise(a, m, c);
-    if ((int)threadIdx.x == owner) sh.own = a.s;
-    const float others = block_all<NT>((int)threadIdx.x == owner ? 0.f : a.s, sh.f, Add());
-    if (NT == 64) __syncthreads();
-    const float own = sh.own;
-    Total r;
+    constexpr int W = NT / 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    WaveStat w;
+    w.m = wave_most(a.m);
+    const int first = __ffsll((unsigned long long)__ballot(a.m == w.m)) - 1;
+    raise(a, w.m, c);
+    w.own = lane_value(a.s, first);
+    w.others = wave_total(lane == first ? 0.f : a.s);
+    w.t = wave_total(a.t);
+    w.above = a.above;
+    w.owner = wave * 64 + first;
+    int owner_wave = 0;
+    float m = w.m, others = w.others, own = w.own;
+    Total r = {m, 0.f, w.t, w.above};
+    if (W > 1) {
+        if (lane == 0) sh.wave[wave] = w;
+        __syncthreads();
+        m = sh.wave[0].m;
+#pragma unroll
+        for (int i = 1; i < W; ++i)
+            if (sh.wave[i].m > m) {
+                m = sh.wave[i].m;
+                owner_wave = i;
+            }
+        others = r.t = 0.f;
+        r.above = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const WaveStat &v = sh.wave[i];
+            const float d = fmaxf((v.m - m) * c, FAR), f = exp2_fast(d), s = v.own + v.others;
+            others += i == owner_wave ? v.others : f * s;
+            r.t += f * (v.t + s * d);
+            r.above += v.above;
+        }
+        own = sh.wave[owner_wave].own;
+        w.owner = sh.wave[owner_wave].owner;
+    }
     r.m = m;
-    r.t = block_all<NT>(a.t, sh.f, Add());
-    r.above = block_all<NT>(a.above, sh.i, Add());
     r.rest = others + (own - 1.f);
     if (others + own == 0.f) {
         r.m = -INFINITY;
         r.rest = 0.f;
     } else if (others + own < 1.5f) {
-        // own - 1 has lost what the owner's other logits add to its 1: sum them again without it
+        // own - 1 has lost what the owner's other logits add to its 1: the
+        // owner's wave sums them again without it
         constexpr int V = Row<TYPE>::VEC;
-        const int chunks = (g.chunks() - owner + NT - 1) / NT;
-        float s = 0.f;
-        int at_max = 0;
-        for (int i = threadIdx.x; i < chunks * V + 1; i += NT) {
-            size_t j = (size_t)(owner + i / V * NT) * V + i % V;
-            if (i == chunks * V) {  // its single element behind the chunks, if it has one
-                if (owner >= g.rest()) continue;
-                j = (size_t)g.chunks() * V + owner;
+        if (wave == owner_wave) {
+            const int n = g.chunks(), rounds = w.owner < n ? (n - w.owner + NT - 1) / NT : 0;
+            float s = 0.f, at_max = 0.f;
+            for (int i = lane; i < rounds * V + 1; i += 64) {
+                size_t j = (size_t)(w.owner + i / V * NT) * V + i % V;
+                if (i == rounds * V) {  // its single element behind the chunks, if it has one
+                    if (w.owner >= g.rest()) continue;
+                    j = (size_t)n * V + w.owner;
+                }
+                const float x = (float)g.p[j];
+                if (x == m) at_max += 1.f;
+                else s += exp2_fast((x - m) * c);
             }
-            const float x = (float)g.p[j];
-            if (x == m) ++at_max;
-            else s += exp2_fast((x - m) * c);
+            r.rest = others + (wave_total(s) + (wave_total(at_max) - 1.f));
+            if (W > 1 && lane == 0) sh.rest = r.rest;
         }
-        at_max = block_all<NT>(at_max, sh.i, Add());
-        r.rest = others + (block_all<NT>(s, sh.f, Add()) + (float)(at_max - 1));
+        if (W > 1) {
+            __syncthreads();
+            r.rest = sh.rest;
+        }
     }
     return r;
 }
@@ -305,7 +400,7 @@ __device__ int candidates(const Range<TYPE> &g, float mine, int k, TopLds<NT> &s
             const uint32_t up = kth | (1u << b);
             int count = 0;
             each_hot<TYPE, NT>(g, sh, [&](float x, int) { count += order_key(x) >= up; });
-            if (block_all<NT>(count, sh.sum, Add()) >= k) kth = up;
+            if (block_sum<NT>(count, sh.sum) >= k) kth = up;
         }
         low = key_value(kth);
         __syncthreads();
@@ -390,7 +485,7 @@ __device__ __forceinline__ void write_top(const LogprobsOut &o, size_t at, uint6
 
 // One workgroup per row, or per part of a row (parts > 1), `span` classes
 // each; the parts' totals and their k largest go to `part` and `lists`.
-template <int TYPE, int NT>
+template <int TYPE, int NT, bool ENTROPY, bool RANK>
 __global__ void __launch_bounds__(NT)
     k_logprobs(ach_logits_desc d, const typename Elem<TYPE>::T *__restrict__ logits,
                const int32_t *__restrict__ ids, int k, LogprobsOut o, int parts, int span,
@@ -406,7 +501,7 @@ __global__ void __launch_bounds__(NT)
         const int id = ids ? ids[r] : -1;
         const bool given = id >= 0 && id < d.classes;
         const float x_id = given ? (float)row[id] : INFINITY;
-        const Stat mine = stream<TYPE, NT>(g, c, x_id);
+        const Stat mine = stream<TYPE, NT, ENTROPY, RANK>(g, c, x_id);
         const Total a = total_of<TYPE, NT>(g, mine, c, st);
         const bool bad = !(a.rest < INFINITY);
         if (parts > 1) {
@@ -608,7 +703,7 @@ template <int NT> struct DistillLds {
     uint32_t bits[SEG / 32];
     Entry entry[ACH_TOP_MAX];
     int dropped[ACH_TOP_MAX];
-    float f[NT / 64];
+    Dense wave[NT / 64];
     // the row's constants, from one wave
     double ref, total, total1, P, mt, tail;
     float K, K1, loss;
@@ -618,7 +713,7 @@ template <int NT> struct DistillLds {
 template <int TYPE, int NT, bool TWO>
 __device__ Dense stream_dense(const Range<TYPE> &all, float c, int k, int y, DistillLds<NT> &sh)
 {
-    constexpr int V = Row<TYPE>::VEC, U = 4, SEG = DistillLds<NT>::SEG;
+    constexpr int V = Row<TYPE>::VEC, U = UNROLL, SEG = DistillLds<NT>::SEG;
     Dense a = {-FLT_MAX, 0.f, 0.f};
     for (int at = 0; at < all.len; at += SEG) {
         const Range<TYPE> g = {all.p + at, all.begin + at, min(SEG, all.len - at)};
@@ -663,10 +758,22 @@ __device__ Dense stream_dense(const Range<TYPE> &all, float c, int k, int y, Dis
             absorb_dense<TWO>(a, x, c);
         }
     }
-    const float m = block_all<NT>(a.m, sh.f, Max());
-    if (a.m != m) raise_dense<TWO>(a, m, c);
-    a.s = block_all<NT>(a.s, sh.f, Add());
-    if (TWO) a.s1 = block_all<NT>(a.s1, sh.f, Add());
+    raise_dense<TWO>(a, wave_most(a.m), c);
+    a.s = wave_total(a.s);
+    if (TWO) a.s1 = wave_total(a.s1);
+    if (NT == 64) return a;
+    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = sh.wave[0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) {
+        Dense b = sh.wave[i];
+        const float m = fmaxf(a.m, b.m);
+        raise_dense<TWO>(a, m, c);
+        raise_dense<TWO>(b, m, c);
+        a.s += b.s;
+        if (TWO) a.s1 += b.s1;
+    }
     return a;
 }
 
@@ -922,7 +1029,7 @@ __global__ void __launch_bounds__(256) k_sum_losses(const float *__restrict__ ro
     __shared__ double sh[4];
     double s = 0;
     for (int i = threadIdx.x; i < rows; i += 256) s += row_loss[i];
-    s = block_all<256>(s, sh, Add());
+    s = block_sum<256>(s, sh);
     if (threadIdx.x == 0) *cost = (float)s;
 }
 
@@ -970,8 +1077,8 @@ Split split_rows(int rows, int classes)
 // (the bound on the k-th largest is taken from the threads' maxima).
 int threads_for(int span, int k)
 {
-    if (span <= 2048 && k <= 32) return 64;
-    return span <= 16384 ? 256 : 1024;
+    if (span <= T64 && k <= 32) return 64;
+    return span <= T256 ? 256 : 1024;
 }
 
 unsigned grid_of(size_t n) { return (unsigned)(n < (1u << 20) ? n : 1u << 20); }
@@ -1023,9 +1130,16 @@ int ach_logprobs_fwd(const ach_logits_desc *desc, const void *logits, const int3
     uint64_t *lists = (uint64_t *)(part + (size_t)d.rows * sp.parts);
     const LogprobsOut o = {logprobs, ranks, entropy, stats, top_ids, top_logprobs};
     hipStream_t st = as_stream(s);
-#define GO(TYPE, NT)                                                                              \
-    hipLaunchKernelGGL((k_logprobs<TYPE, NT>), grid, dim3(NT), 0, st, d,                          \
+#define GO_(TYPE, NT, E, R)                                                                       \
+    hipLaunchKernelGGL((k_logprobs<TYPE, NT, E, R>), grid, dim3(NT), 0, st, d,                    \
                        (const Elem<TYPE>::T *)logits, ids, k, o, sp.parts, sp.span, part, lists)
+#define GO(TYPE, NT)                                                                              \
+    do {                                                                                          \
+        if (entropy && ranks) GO_(TYPE, NT, true, true);                                          \
+        else if (entropy) GO_(TYPE, NT, true, false);                                             \
+        else if (ranks) GO_(TYPE, NT, false, true);                                               \
+        else GO_(TYPE, NT, false, false);                                                         \
+    } while (0)
 #define CALL(TYPE)                                                                                \
     do {                                                                                          \
         if (nt == 64) GO(TYPE, 64);                                                               \
@@ -1035,6 +1149,7 @@ int ach_logprobs_fwd(const ach_logits_desc *desc, const void *logits, const int3
     FOR_TYPE(d.type, CALL);
 #undef CALL
 #undef GO
+#undef GO_
     const int rc = check_launch();
     if (rc || sp.parts == 1) return rc;
 #define CALL(TYPE)                                                                                \
