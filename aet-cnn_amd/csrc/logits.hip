@@ -16,12 +16,12 @@
 namespace ach {
 namespace {
 
-#ifndef UNROLL
-#define UNROLL 4
-#endif
 #ifndef T64
 #define T64 2048
 #define T256 16384
+#endif
+#ifndef D256
+#define D256 131072
 #endif
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
@@ -159,9 +159,10 @@ __device__ __forceinline__ void raise(Stat &a, float m, float c)
 }
 
 // N logits of each lane, all lanes taking part.  Masked logits make the plain
-// sum for t a NaN, 0 * -inf: then it is formed again without them.
-template <bool ENTROPY, bool RANK, int N>
-__device__ __forceinline__ void absorb(Stat &a, const float (&x)[N], float c, float x_id)
+// sum for t a NaN, 0 * -inf: then it is formed again without them.  Returns the
+// lane's maximum of them.
+template <bool FULL, int N>
+__device__ __forceinline__ float absorb(Stat &a, const float (&x)[N], float c, float x_id)
 {
     float m = x[0];
 #pragma unroll
@@ -172,10 +173,10 @@ __device__ __forceinline__ void absorb(Stat &a, const float (&x)[N], float c, fl
     for (int i = 0; i < N; ++i) {
         const float d = (x[i] - a.m) * c, e = exp2_fast(d);
         a.s += e;
-        if (ENTROPY) t = fmaf(e, d, t);
-        if (RANK) a.above += __popcll(__ballot(x[i] > x_id));
+        if (FULL) t = fmaf(e, d, t);
+        if (FULL) a.above += __popcll(__ballot(x[i] > x_id));
     }
-    if (ENTROPY) {
+    if (FULL) {
         if (t != t) {
             t = a.t;
             for (int i = 0; i < N; ++i) {
@@ -185,28 +186,69 @@ __device__ __forceinline__ void absorb(Stat &a, const float (&x)[N], float c, fl
         }
         a.t = t;
     }
+    return m;
 }
 
-template <int TYPE, int NT, bool ENTROPY, bool RANK>
-__device__ __forceinline__ Stat stream(const Range<TYPE> &g, float c, float x_id)
+// How a range's chunks are read: `full` times UNROLL chunks by every thread,
+// chunk q by thread q % NT, then what is left.  With alternatives to be found,
+// the maxima of what a thread reads in 2^shift turns, a group, and of what is
+// left are kept.
+constexpr int UNROLL = 4, GROUPS = 16;
+#ifndef UNROLL_D
+#define UNROLL_D 4
+#endif
+
+template <int TYPE, int NT> struct Turns {
+    int full, shift;
+    __device__ explicit Turns(const Range<TYPE> &g)
+        : full(g.chunks() / (UNROLL * NT)), shift(0)
+    {
+        while (full > GROUPS << shift) ++shift;
+    }
+    // chunk i of a thread's group, or -1
+    __device__ int chunk(const Range<TYPE> &g, int group, int thread, int i) const
+    {
+        const int turn = group == GROUPS ? full : (group << shift) + i / UNROLL;
+        if (group == GROUPS ? i >= UNROLL : turn >= full) return -1;
+        const int q = (turn * UNROLL + i % UNROLL) * NT + thread;
+        return q < g.chunks() ? q : -1;
+    }
+};
+
+template <int NT> struct GroupLds {
+    float most[GROUPS + 1][NT];
+};
+
+template <int TYPE, int NT, bool FULL, bool TOP>
+__device__ __forceinline__ Stat stream(const Range<TYPE> &g, const Turns<TYPE, NT> &turns, float c,
+                                       float x_id, GroupLds<NT> *groups)
 {
     constexpr int V = Row<TYPE>::VEC, U = UNROLL;
     typedef typename Row<TYPE>::Chunk Chunk;
     Stat a = {-FLT_MAX, 0.f, 0.f, 0};
     const int n = g.chunks(), lane = threadIdx.x & 63;
-    int q = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);  // the wave's first chunk
-    for (; q + (U - 1) * NT + 64 <= n; q += U * NT) {
+    const auto *p = g.p + (size_t)threadIdx.x * V;
+    float most = -INFINITY;
+    for (int turn = 0; turn < turns.full; ++turn, p += (size_t)U * NT * V) {
         Chunk v[U];
         float x[U * V];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = Row<TYPE>::load(g.p + (size_t)(q + u * NT + lane) * V);
+        for (int u = 0; u < U; ++u) v[u] = Row<TYPE>::load(p + (size_t)u * NT * V);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < V; ++i) x[u * V + i] = (float)v[u][i];
-        absorb<ENTROPY, RANK>(a, x, c, x_id);
+        const float m = absorb<FULL>(a, x, c, x_id);
+        if (TOP) {
+            most = fmaxf(most, m);
+            if (((turn + 1) & ((1 << turns.shift) - 1)) == 0 || turn + 1 == turns.full) {
+                groups->most[turn >> turns.shift][threadIdx.x] = most;
+                most = -INFINITY;
+            }
+        }
     }
-    for (; q < n; q += NT) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);
+    for (int q = turns.full * U * NT + wave; q < n; q += NT) {
         float x[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) x[i] = -INFINITY;
@@ -215,12 +257,13 @@ __device__ __forceinline__ Stat stream(const Range<TYPE> &g, float c, float x_id
 #pragma unroll
             for (int i = 0; i < V; ++i) x[i] = (float)v[i];
         }
-        absorb<ENTROPY, RANK>(a, x, c, x_id);
+        most = fmaxf(most, absorb<FULL>(a, x, c, x_id));
     }
-    if (threadIdx.x < 64) {
+    if (wave == 0) {
         const float x[1] = {lane < g.rest() ? (float)g.p[(size_t)n * V + lane] : -INFINITY};
-        absorb<ENTROPY, RANK>(a, x, c, x_id);
+        most = fmaxf(most, absorb<FULL>(a, x, c, x_id));
     }
+    if (TOP) groups->most[GROUPS][threadIdx.x] = most;
     return a;
 }
 
@@ -321,42 +364,59 @@ __device__ __forceinline__ Total total_of(const Range<TYPE> &g, Stat a, float c,
 // ---- the k largest ---------------------------------------------------------------
 // The threads' maxima bound the k-th largest logit from below: each wave's
 // ceil(k / waves)-th largest maximum has k logits at or above the least of
-// these.  Only the threads whose maximum reaches that bound have seen
-// candidates, so only their chunks are read again (from the caches), by all
-// threads together.  Of random logits some k log(waves) + k pass; they are put
-// in order by counting for each how many are before it.
+// these.  Only groups whose maximum reaches that bound hold candidates, so only
+// they are read again (from the caches), by all threads together.  Of random
+// logits some k log(waves) + k pass; they are put in order by counting for each
+// how many are before it.
 template <int NT> struct TopLds {
-    // logits above the bound, and at it
-    static constexpr int CAP = NT == 64 ? 256 : 1024, EQUAL = NT == 64 ? 128 : 512;
+    // logits above the bound, and at it; groups to be read again
+    static constexpr int CAP = NT == 64 ? 256 : 1024, EQUAL = NT == 64 ? 128 : 512, HOT = 512;
     uint64_t list[CAP + EQUAL];
     uint64_t equal[EQUAL];
+    GroupLds<NT> groups;
     uint32_t bound[NT / 64];
-    int hot[NT];
+    int hot[HOT];
     int sum[NT / 64];
     int nhot, nlist, nequal;
 };
 
-// f(x, class) for every logit that the hot threads have seen.
+// f(x, class) for every logit of the groups whose maximum reaches `low`,
+// which are listed unless they are too many.
 template <int TYPE, int NT, class F>
-__device__ __forceinline__ void each_hot(const Range<TYPE> &g, const TopLds<NT> &sh, F f)
+__device__ __forceinline__ void each_hot(const Range<TYPE> &g, const Turns<TYPE, NT> &turns,
+                                         const TopLds<NT> &sh, float low, F f)
 {
     constexpr int V = Row<TYPE>::VEC;
-    const int n = g.chunks(), hot = sh.nhot, rounds = (n + NT - 1) / NT;
-    for (int i = threadIdx.x; i < hot * rounds; i += NT) {
-        const int q = i / hot * NT + sh.hot[i % hot];
-        if (q >= n) continue;
+    const auto chunk = [&](int q) {
+        if (q < 0) return;
         const typename Row<TYPE>::Chunk v = Row<TYPE>::load(g.p + (size_t)q * V);
 #pragma unroll
         for (int e = 0; e < V; ++e) f((float)v[e], g.begin + q * V + e);
+    };
+    const int each = UNROLL << turns.shift;
+    if (sh.nhot <= TopLds<NT>::HOT) {
+        for (int i = threadIdx.x; i < sh.nhot * each; i += NT) {
+            const int h = sh.hot[i / UNROLL >> turns.shift];
+            chunk(turns.chunk(g, h / NT, h % NT, i & (each - 1)));
+        }
+    } else {
+        for (int group = 0; group <= GROUPS; ++group)
+            if (group == GROUPS || (group << turns.shift) < turns.full)
+                if (sh.groups.most[group][threadIdx.x] >= low)
+                    for (int i = 0; i < each; ++i)
+                        chunk(turns.chunk(g, group, threadIdx.x, i));
     }
-    if (threadIdx.x < g.rest())
-        f((float)g.p[(size_t)n * V + threadIdx.x], g.begin + n * V + (int)threadIdx.x);
+    if (threadIdx.x < g.rest()) {
+        const int j = g.chunks() * V + threadIdx.x;
+        f((float)g.p[j], g.begin + j);
+    }
 }
 
 // Leaves in sh.list a superset of the k largest of the range (k <= its
 // length, no NaN) and returns its size; `mine` is the thread's maximum.
 template <int TYPE, int NT>
-__device__ int candidates(const Range<TYPE> &g, float mine, int k, TopLds<NT> &sh)
+__device__ __forceinline__ int candidates(const Range<TYPE> &g, const Turns<TYPE, NT> &turns,
+                                          float mine, int k, TopLds<NT> &sh)
 {
     constexpr int CAP = TopLds<NT>::CAP, EQUAL = TopLds<NT>::EQUAL, W = NT / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -374,15 +434,18 @@ __device__ int candidates(const Range<TYPE> &g, float mine, int k, TopLds<NT> &s
     for (int i = 0; i < W; ++i) bound = min(bound, sh.bound[i]);
     // up to -FLT_MAX, where a thread that has seen -inf alone starts: anything
     float low = bound <= order_key(-FLT_MAX) ? -INFINITY : key_value(bound);
-    const bool is_hot = mine >= low;
-    const uint64_t ballot = __ballot(is_hot);
-    int at = 0;
-    if (lane == 0) at = atomicAdd(&sh.nhot, __popcll(ballot));
-    at = __shfl(at, 0, 64);
-    if (is_hot) sh.hot[at + __popcll(ballot & ((1ull << lane) - 1))] = threadIdx.x;
+    const float first_low = low;
+    if (mine >= low)
+        for (int group = 0; group <= GROUPS; ++group) {
+            if (group < GROUPS && (group << turns.shift) >= turns.full) continue;
+            if (sh.groups.most[group][threadIdx.x] >= low) {
+                const int i = atomicAdd(&sh.nhot, 1);
+                if (i < TopLds<NT>::HOT) sh.hot[i] = group * NT + threadIdx.x;
+            }
+        }
     __syncthreads();
-    for (int round = 0;; ++round) {
-        each_hot<TYPE, NT>(g, sh, [&](float x, int j) {
+    while (true) {
+        each_hot<TYPE, NT>(g, turns, sh, first_low, [&](float x, int j) {
             if (x > low) {
                 const int i = atomicAdd(&sh.nlist, 1);
                 if (i < CAP) sh.list[i] = compound(x, j);
@@ -399,7 +462,7 @@ __device__ int candidates(const Range<TYPE> &g, float mine, int k, TopLds<NT> &s
         for (int b = 31; b >= 0; --b) {
             const uint32_t up = kth | (1u << b);
             int count = 0;
-            each_hot<TYPE, NT>(g, sh, [&](float x, int) { count += order_key(x) >= up; });
+            each_hot<TYPE, NT>(g, turns, sh, first_low, [&](float x, int) { count += order_key(x) >= up; });
             if (block_sum<NT>(count, sh.sum) >= k) kth = up;
         }
         low = key_value(kth);
@@ -485,14 +548,22 @@ __device__ __forceinline__ void write_top(const LogprobsOut &o, size_t at, uint6
 
 // One workgroup per row, or per part of a row (parts > 1), `span` classes
 // each; the parts' totals and their k largest go to `part` and `lists`.
-template <int TYPE, int NT, bool ENTROPY, bool RANK>
+template <bool B, class X, class Y> struct Pick {
+    using T = X;
+};
+template <class X, class Y> struct Pick<false, X, Y> {
+    using T = Y;
+};
+
+template <int TYPE, int NT, bool FULL, bool TOP>
 __global__ void __launch_bounds__(NT)
     k_logprobs(ach_logits_desc d, const typename Elem<TYPE>::T *__restrict__ logits,
                const int32_t *__restrict__ ids, int k, LogprobsOut o, int parts, int span,
                Total *__restrict__ part, uint64_t *__restrict__ lists)
 {
     __shared__ StatLds<NT> st;
-    __shared__ TopLds<NT> top;
+    __shared__ typename Pick<TOP, TopLds<NT>, int>::T top_lds;
+    TopLds<NT> &top = *(TopLds<NT> *)&top_lds;  // only with TOP
     const float inv_t = 1.f / d.temperature, c = inv_t * LOG2E;
     for (size_t w = blockIdx.x; w < (size_t)d.rows * parts; w += gridDim.x) {
         const int r = (int)(w / parts), at = (int)(w % parts) * span;
@@ -501,7 +572,8 @@ __global__ void __launch_bounds__(NT)
         const int id = ids ? ids[r] : -1;
         const bool given = id >= 0 && id < d.classes;
         const float x_id = given ? (float)row[id] : INFINITY;
-        const Stat mine = stream<TYPE, NT, ENTROPY, RANK>(g, c, x_id);
+        const Turns<TYPE, NT> turns(g);
+        const Stat mine = stream<TYPE, NT, FULL, TOP>(g, turns, c, x_id, TOP ? &top.groups : nullptr);
         const Total a = total_of<TYPE, NT>(g, mine, c, st);
         const bool bad = !(a.rest < INFINITY);
         if (parts > 1) {
@@ -509,13 +581,13 @@ __global__ void __launch_bounds__(NT)
         }
         const float log_s = parts > 1 ? 0.f
                                       : write_row(o, r, a, given, x_id, inv_t, threadIdx.x == 0);
-        if (k > 0 && bad) {
+        if (TOP && bad) {
             for (int i = threadIdx.x; i < k && parts == 1; i += NT) {
                 o.top_ids[(size_t)r * k + i] = -1;
                 o.top_logprobs[(size_t)r * k + i] = NAN;
             }
-        } else if (k > 0) {
-            const int mk = min(k, g.len), n = candidates<TYPE, NT>(g, mine.m, mk, top);
+        } else if (TOP) {
+            const int mk = min(k, g.len), n = candidates<TYPE, NT>(g, turns, mine.m, mk, top);
             if (parts > 1) {
                 in_order<NT>(top.list, n, mk, [&](int i, uint64_t v) { lists[w * k + i] = v; });
                 for (int i = mk + threadIdx.x; i < k; i += NT) lists[w * k + i] = 0;
@@ -659,19 +731,14 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- distillation ------------------------------------------------------------------
-// A row's listed classes, the teacher's entries and the label, are few: their
-// terms are computed in 64 bits.  All others enter through their maximum and
-// their sums of exponentials alone, so the sum over what the teacher leaves
-// out is a sum of these, not a difference of nearly equal sums.  With
-// e_j = exp((x_j - mo)/T) relative to the maximum mo of the classes that are
-// not listed, the delta of such a class is K e_j + K1 e1_j (e1: at
-// temperature 1), and that of a listed one is written over it afterwards.
-struct Entry {
-    double p;  // the teacher's probability
-    int id;    // -1: dropped
-    float x;   // the student's logit
-};
-
+// A row's listed classes, the teacher's entries and the label, are few, and
+// their terms are formed one by one, sums of them in 64 bits.  All others, the
+// dense ones, enter through their maximum and their sums of exponentials
+// alone, so the sum over what the teacher leaves out is a sum of these, not a
+// difference of nearly equal sums.  With e_j = exp((x_j - mo)/T) relative to
+// the maximum mo of the dense classes, the delta of such a class is
+// K e_j + K1 e1_j (e1: at temperature 1), and that of a listed one is written
+// over it afterwards.
 struct Dense {
     float m, s, s1;
 };
@@ -701,33 +768,35 @@ __device__ __forceinline__ void absorb_dense(Dense &a, const float (&x)[N], floa
 template <int NT> struct DistillLds {
     static constexpr int SEG = NT * 128;  // classes of one bitmap of listed classes
     uint32_t bits[SEG / 32];
-    Entry entry[ACH_TOP_MAX];
-    int dropped[ACH_TOP_MAX];
+    int id[ACH_TOP_MAX];       // as the teacher gives them; -1: none
+    int repeated[ACH_TOP_MAX];
+    int label_listed;          // by the teacher
     Dense wave[NT / 64];
-    // the row's constants, from one wave
-    double ref, total, total1, P, mt, tail;
-    float K, K1, loss;
-    int y_listed;
+    float most[NT / 64], most_value[NT / 64];
+    double sum[4][NT / 64];
 };
 
+// A thread's statistics of the dense classes of a range.
 template <int TYPE, int NT, bool TWO>
-__device__ Dense stream_dense(const Range<TYPE> &all, float c, int k, int y, DistillLds<NT> &sh)
+__device__ __forceinline__ Dense stream_dense(const Range<TYPE> &all, float c, int k, int y,
+                                              DistillLds<NT> &sh)
 {
-    constexpr int V = Row<TYPE>::VEC, U = UNROLL, SEG = DistillLds<NT>::SEG;
+    constexpr int V = Row<TYPE>::VEC, U = UNROLL_D, SEG = DistillLds<NT>::SEG;
+    typedef typename Row<TYPE>::Chunk Chunk;
     Dense a = {-FLT_MAX, 0.f, 0.f};
     for (int at = 0; at < all.len; at += SEG) {
         const Range<TYPE> g = {all.p + at, all.begin + at, min(SEG, all.len - at)};
-        __syncthreads();
+        if (at > 0) __syncthreads();
         for (int i = threadIdx.x; i < (g.len + 31) / 32; i += NT) sh.bits[i] = 0;
         __syncthreads();
         for (int i = threadIdx.x; i <= k; i += NT) {
-            const int j = (i < k ? sh.entry[i].id : y) - g.begin;
+            const int j = (i < k ? sh.id[i] : y) - g.begin;
             if (j >= 0 && j < g.len) atomicOr(&sh.bits[j >> 5], 1u << (j & 31));
         }
         __syncthreads();
         const int n = g.chunks();
-        // the listed classes of a chunk read as masked
-        const auto fetch = [&](const typename Row<TYPE>::Chunk &v, int q, float *x) {
+        // a chunk with its listed classes masked
+        const auto fetch = [&](const Chunk &v, int q, float *x) {
             const uint32_t mask = (sh.bits[q * V >> 5] >> (q * V & 31)) & ((1u << V) - 1);
 #pragma unroll
             for (int i = 0; i < V; ++i) x[i] = (float)v[i];
@@ -738,7 +807,7 @@ __device__ Dense stream_dense(const Range<TYPE> &all, float c, int k, int y, Dis
         };
         int q = threadIdx.x;
         for (; q + (U - 1) * NT < n; q += U * NT) {
-            typename Row<TYPE>::Chunk v[U];
+            Chunk v[U];
             float x[U * V];
 #pragma unroll
             for (int u = 0; u < U; ++u) v[u] = Row<TYPE>::load(g.p + (size_t)(q + u * NT) * V);
@@ -758,154 +827,34 @@ __device__ Dense stream_dense(const Range<TYPE> &all, float c, int k, int y, Dis
             absorb_dense<TWO>(a, x, c);
         }
     }
-    raise_dense<TWO>(a, wave_most(a.m), c);
-    a.s = wave_total(a.s);
-    if (TWO) a.s1 = wave_total(a.s1);
-    if (NT == 64) return a;
-    if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = a;
-    __syncthreads();
-    a = sh.wave[0];
-#pragma unroll
-    for (int i = 1; i < NT / 64; ++i) {
-        Dense b = sh.wave[i];
-        const float m = fmaxf(a.m, b.m);
-        raise_dense<TWO>(a, m, c);
-        raise_dense<TWO>(b, m, c);
-        a.s += b.s;
-        if (TWO) a.s1 += b.s1;
-    }
     return a;
 }
 
-__device__ __forceinline__ double load_any(const void *p, int type, size_t i)
+// The same of the wave, in all its lanes.
+template <bool TWO> __device__ __forceinline__ void wave_dense(Dense &a, float c)
+{
+    raise_dense<TWO>(a, wave_most(a.m), c);
+    a.s = wave_total(a.s);
+    if (TWO) a.s1 = wave_total(a.s1);
+}
+
+__device__ __forceinline__ float load_any(const void *p, int type, size_t i)
 {
     return type == ACH_F32    ? ((const float *)p)[i]
            : type == ACH_BF16 ? (float)((const __bf16 *)p)[i]
                               : (float)((const _Float16 *)p)[i];
 }
 
-// The teacher's entries of a row into sh.entry.
-template <int TYPE, int NT>
-__device__ void read_teacher(const typename Elem<TYPE>::T *row, int classes,
-                             const int32_t *teacher_ids, const void *values, int type, size_t at,
-                             int k, bool tail, double inv_t, DistillLds<NT> &sh)
-{
-    __syncthreads();
-    for (int i = threadIdx.x; i < k; i += NT) {
-        const int id = teacher_ids[at + i];
-        const bool some = id >= 0 && id < classes;
-        sh.entry[i].id = some ? id : -1;
-        sh.entry[i].x = some ? (float)row[id] : 0.f;
-        sh.dropped[i] = !some;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < k * k; i += NT) {  // repeated: the first one counts
-        const int a = i / k, b = i % k;
-        if (b < a && sh.entry[a].id == sh.entry[b].id) sh.dropped[a] = 1;
-    }
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        double v[2], p[2], sum = 0, most = -INFINITY;
-        for (int e = 0; e < 2; ++e) {
-            const int i = threadIdx.x + e * 64;
-            v[e] = i < k && !sh.dropped[i] ? load_any(values, type, at + i) : -INFINITY;
-            if (!tail) v[e] *= inv_t;
-            most = fmax(most, v[e]);
-        }
-        most = tail ? 0 : wave_all(most, Max());
-        for (int e = 0; e < 2; ++e) {
-            p[e] = v[e] == -INFINITY ? 0 : exp(v[e] - most);
-            sum += p[e];
-        }
-        sum = wave_all(sum, Add());
-        for (int e = 0; e < 2; ++e) {
-            const int i = threadIdx.x + e * 64;
-            if (i >= k) continue;
-            sh.entry[i].p = tail || sum == 0 ? p[e] : p[e] / sum;
-            if (sh.dropped[i]) sh.entry[i].id = -1;
-        }
-    }
-    __syncthreads();
-}
-
-// The row's constants from its listed classes and the dense part, by the
-// first wave.
-template <int NT>
-__device__ void constants(const Dense &a, const ach_distill_desc &t, int k, bool tail,
-                          double temperature, int y, float x_y, float w, DistillLds<NT> &sh)
-{
-    if (threadIdx.x >= 64) return;
-    const double inv_t = 1. / temperature;
-    const int lane = threadIdx.x;
-    float m = a.m;
-    bool listed = false;
-    for (int i = lane; i < k; i += 64)
-        if (sh.entry[i].id >= 0) {
-            m = fmaxf(m, sh.entry[i].x);
-            listed |= sh.entry[i].id == y;
-        }
-    const bool y_listed = __any(listed);
-    const bool extra = y >= 0 && !y_listed;  // the label as a class of its own
-    m = wave_all(m, Max());
-    if (y >= 0) m = fmaxf(m, x_y);
-    const double ref = m;
-    double total = 0, total1 = 0, sp = 0;
-    for (int i = lane; i < k; i += 64)
-        if (sh.entry[i].id >= 0) {
-            const double z = sh.entry[i].x - ref;
-            total += exp(z * inv_t);
-            total1 += exp(z);
-            sp += sh.entry[i].p;
-        }
-    total = wave_all(total, Add());
-    total1 = wave_all(total1, Add());
-    sp = wave_all(sp, Add());
-    // without another class the dense part is empty: its sums are 0
-    const double up = exp((a.m - ref) * inv_t), up1 = exp(a.m - ref);
-    const double e_y = extra ? exp((x_y - ref) * inv_t) : 0;
-    total += a.s * up + e_y;
-    total1 += a.s1 * up1 + (extra ? exp(x_y - ref) : 0);
-    const double lse = log(total);
-    double kd = 0;
-    for (int i = lane; i < k; i += 64) {
-        const double p = sh.entry[i].p;
-        if (sh.entry[i].id >= 0 && p != 0)
-            kd += p * (log(p) - ((sh.entry[i].x - ref) * inv_t - lse));
-    }
-    kd = wave_all(kd, Add());
-    // the rest: all classes that the teacher does not list, relative to their maximum mt
-    const double mt = extra ? fmaxf(a.m, x_y) : a.m;
-    const double sum_t = a.s * exp((a.m - mt) * inv_t) + (extra ? exp((x_y - mt) * inv_t) : 0);
-    double P = sp, rest = 0;
-    if (tail && k > 0 && sum_t != 0) {
-        rest = sp > 1 ? 0 : 1 - sp;
-        if (rest != 0) kd += rest * (log(rest) - (log(sum_t) + (mt - ref) * inv_t - lse));
-        P += rest;
-    }
-    const double per_tail = rest == 0 ? 0 : rest / sum_t;
-    double value = k > 0 ? t.soft * temperature * temperature * kd : 0;
-    if (y >= 0) value += t.hard * (log(total1) - (x_y - ref));
-    const bool empty = total == 0;
-    const double soft = k > 0 ? -w * t.soft * temperature : 0, hard = y >= 0 ? -w * t.hard : 0;
-    if (lane == 0) {
-        sh.loss = empty ? 0.f : (float)(w * value);
-        sh.K = empty || soft == 0 ? 0.f
-                                  : (float)(soft * (P * up / total -
-                                                    per_tail * exp((a.m - mt) * inv_t)));
-        sh.K1 = empty || hard == 0 ? 0.f : (float)(hard * up1 / total1);
-        sh.ref = ref;
-        sh.total = empty ? INFINITY : total;
-        sh.total1 = empty ? INFINITY : total1;
-        sh.P = P;
-        sh.mt = mt;
-        sh.tail = per_tail;
-        sh.y_listed = y_listed;
-    }
-}
-
 // What a launch does: all of it, a row to a workgroup; or, for rows in parts,
-// the statistics, then the delta.
+// the statistics of the dense classes, then all else.
 enum { WHOLE, STATS, DELTA };
+
+// Where the first of two launches leaves its results: the parts' statistics,
+// and the logits of the listed classes, which the second may overwrite.
+struct Between {
+    Dense *dense;
+    float *x;  // [row][ACH_TOP_MAX + 1], the label's at [k]
+};
 
 template <int TYPE, int NT, bool TWO, int MODE>
 __global__ void __launch_bounds__(NT)
@@ -913,113 +862,237 @@ __global__ void __launch_bounds__(NT)
               const int32_t *__restrict__ teacher_ids, const void *__restrict__ teacher_values,
               const int32_t *__restrict__ labels, const float *__restrict__ row_weights,
               float *loss, typename Elem<TYPE>::T *delta, int64_t delta_stride, float *row_loss,
-              int parts, int span, Dense *dense, Entry *entries)
+              int parts, int span, Between between)
 {
     using T = typename Elem<TYPE>::T;
     typedef typename Row<TYPE>::Chunk Chunk;
-    constexpr int V = Row<TYPE>::VEC;
+    constexpr int V = Row<TYPE>::VEC, W = NT / 64;
+    constexpr int E = (ACH_TOP_MAX + NT) / NT;  // listed classes of a thread, i = thread + e NT
     __shared__ DistillLds<NT> sh;
     const int k = t.soft != 0.f ? t.k : 0;
     const bool tail = t.mode == ACH_DISTILL_TAIL;
-    const float c = LOG2E / d.temperature;
+    const float inv_t = 1.f / d.temperature, c = inv_t * LOG2E;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (size_t b = blockIdx.x; b < (size_t)d.rows * parts; b += gridDim.x) {
         const int r = (int)(b / parts), part = (int)(b % parts), at = part * span;
         const T *row = logits + (size_t)r * d.stride;
         const Range<TYPE> g = {row + at, at, min(span, d.classes - at)};
         const float w = row_weights ? row_weights[r] : 1.f;
-        if (MODE == STATS && w == 0.f) continue;
-        int y = t.hard != 0.f ? labels[r] : -1;
-        if (y >= d.classes) y = -1;
-        if (w != 0.f) {
-            Dense a;
-            Entry *mine = MODE == WHOLE ? nullptr : entries + (size_t)r * (ACH_TOP_MAX + 1);
-            float x_y = 0.f;
-            if (MODE != DELTA) {
-                x_y = y >= 0 ? (float)row[y] : 0.f;
-                read_teacher<TYPE, NT>(row, d.classes, teacher_ids, teacher_values, t.teacher_type,
-                                       (size_t)r * k, k, tail, 1. / d.temperature, sh);
-                a = stream_dense<TYPE, NT, TWO>(g, c, k, y, sh);
-                if (!TWO) a.s1 = a.s;
-            }
-            if (MODE == STATS) {
-                if (threadIdx.x == 0) dense[b] = a;
-                if (part == 0) {
-                    for (int i = threadIdx.x; i < k; i += NT) mine[i] = sh.entry[i];
-                    if (threadIdx.x == 0) mine[ACH_TOP_MAX].x = x_y;
-                }
-                __syncthreads();
-                continue;
-            }
-            if (MODE == DELTA) {
-                __syncthreads();
-                for (int i = threadIdx.x; i < k; i += NT) sh.entry[i] = mine[i];
-                x_y = y >= 0 ? mine[ACH_TOP_MAX].x : 0.f;
-                const int lane = threadIdx.x & 63;
-                a = {-FLT_MAX, 0.f, 0.f};
-                if (lane < parts) a = dense[(size_t)r * parts + lane];
-                const float m = wave_all(a.m, Max());
-                raise_dense<true>(a, m, c);
-                a.s = wave_all(a.s, Add());
-                a.s1 = wave_all(a.s1, Add());
-            }
-            __syncthreads();
-            constants<NT>(a, t, k, tail, d.temperature, y, x_y, w, sh);
-            __syncthreads();
-            if (threadIdx.x == 0 && part == 0) {
-                if (loss) loss[r] = sh.loss;
-                if (row_loss) row_loss[r] = sh.loss;
-            }
-            if (delta) {
-                T *out = delta + (size_t)r * delta_stride + at;
-                const float K = TWO ? sh.K : sh.K + sh.K1, K1 = sh.K1;
-                const auto grad = [&](float x) {
-                    float v = K * exp2_fast((x - a.m) * c);
-                    if (TWO) v = fmaf(K1, exp2_fast((x - a.m) * LOG2E), v);
-                    return v;
-                };
-                const int n = g.chunks();
-                for (int q = threadIdx.x; q < n; q += NT) {
-                    const Chunk x = Row<TYPE>::load(g.p + (size_t)q * V);
-                    Chunk v;
-#pragma unroll
-                    for (int i = 0; i < V; ++i) v[i] = (T)grad((float)x[i]);
-                    Row<TYPE>::store(out + (size_t)q * V, v);
-                }
-                if (threadIdx.x < g.rest()) {
-                    const int j = n * V + threadIdx.x;
-                    out[j] = (T)grad((float)g.p[j]);
-                }
-                __syncthreads();  // the listed classes over what was written for them
-                for (int i = threadIdx.x; i <= k; i += NT) {
-                    const bool teacher = i < k;
-                    const int id = teacher ? sh.entry[i].id : sh.y_listed ? -1 : y;
-                    if (id < at || id >= at + g.len) continue;
-                    const double x = teacher ? sh.entry[i].x : x_y, inv_t = 1. / d.temperature;
-                    double v = 0;
-                    if (k > 0) {
-                        v = sh.P * exp((x - sh.ref) * inv_t) / sh.total;
-                        v -= teacher ? sh.entry[i].p : sh.tail * exp((x - sh.mt) * inv_t);
-                        v *= -w * t.soft * d.temperature;
-                    }
-                    if (y >= 0) v -= w * t.hard * (exp(x - sh.ref) / sh.total1 - (id == y));
-                    if (sh.total == INFINITY) v = 0;  // no distribution
-                    out[id - at] = (T)(float)v;
-                }
-            }
-        } else {
-            if (delta) {
+        if (w == 0.f) {
+            if (MODE != STATS && delta) {
                 T *out = delta + (size_t)r * delta_stride + at;
                 const Chunk zero = {};
                 for (int q = threadIdx.x; q < g.chunks(); q += NT)
                     Row<TYPE>::store(out + (size_t)q * V, zero);
                 if (threadIdx.x < g.rest()) out[g.chunks() * V + threadIdx.x] = (T)0.f;
             }
-            if (threadIdx.x == 0 && part == 0) {
+            if (MODE != STATS && threadIdx.x == 0 && part == 0) {
                 if (loss) loss[r] = 0.f;
                 if (row_loss) row_loss[r] = 0.f;
             }
+            continue;
+        }
+        int y = t.hard != 0.f ? labels[r] : -1;
+        if (y < 0 || y >= d.classes) y = -1;
+
+        // The listed classes: id -1 where there is none.
+        int id[E];
+        float x[E], value[E];
+        float *kept = MODE == WHOLE ? nullptr : between.x + (size_t)r * (ACH_TOP_MAX + 1);
+        __syncthreads();  // of the last row
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = threadIdx.x + e * NT;
+            id[e] = i < k ? teacher_ids[(size_t)r * k + i] : i == k ? y : -1;
+            if (id[e] < 0 || id[e] >= d.classes) id[e] = -1;
+            value[e] = i < k ? load_any(teacher_values, t.teacher_type, (size_t)r * k + i) : 0.f;
+            x[e] = id[e] < 0 ? -INFINITY : MODE == DELTA ? kept[i] : (float)row[id[e]];
+            if (i < k) {
+                sh.id[i] = id[e];
+                sh.repeated[i] = 0;
+            }
+            if (MODE == STATS && part == 0 && i <= k) kept[i] = x[e];
+        }
+        if (threadIdx.x == 0) sh.label_listed = 0;
+
+        // The dense classes.
+        Dense a;
+        if (MODE == DELTA) {
+            a = {-FLT_MAX, 0.f, 0.f};
+            if (lane < parts) a = between.dense[(size_t)r * parts + lane];
+            wave_dense<true>(a, c);
+            __syncthreads();
+        } else {
+            a = stream_dense<TYPE, NT, TWO>(g, c, k, y, sh);
+            wave_dense<TWO>(a, c);
+            if (!TWO) a.s1 = a.s;
+        }
+        const auto join = [&] {
+            a = sh.wave[0];
+#pragma unroll
+            for (int i = 1; i < W; ++i) {
+                Dense o = sh.wave[i];
+                const float m = fmaxf(a.m, o.m);
+                raise_dense<TWO>(a, m, c);
+                raise_dense<TWO>(o, m, c);
+                a.s += o.s;
+                a.s1 = TWO ? a.s1 + o.s1 : a.s;
+            }
+        };
+        if (MODE == STATS) {
+            if (lane == 0) sh.wave[wave] = a;
+            __syncthreads();
+            join();
+            if (threadIdx.x == 0) between.dense[b] = a;
+            continue;
+        }
+
+        // Of entries with the same id the first counts.
+        int width = 1, shift = 0;
+        while (width < k) width <<= 1, ++shift;
+        for (int i = threadIdx.x; i < k << shift; i += NT) {
+            const int later = i >> shift, former = i & (width - 1);
+            if (former < later && sh.id[former] == sh.id[later]) sh.repeated[later] = 1;
+        }
+        if (y >= 0)
+            for (int i = threadIdx.x; i < k; i += NT)
+                if (sh.id[i] == y) sh.label_listed = 1;
+        float most = -INFINITY, most_value = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (id[e] >= 0) {
+                most = fmaxf(most, x[e]);
+                if ((int)threadIdx.x + e * NT < k) most_value = fmaxf(most_value, value[e]);
+            }
+        most = wave_most(most);
+        most_value = wave_most(most_value);
+        if (lane == 0) {
+            sh.wave[wave] = a;
+            sh.most[wave] = most;
+            sh.most_value[wave] = most_value;
         }
         __syncthreads();
+        if (MODE == WHOLE) join();
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            most = fmaxf(most, sh.most[i]);
+            most_value = fmaxf(most_value, sh.most_value[i]);
+        }
+        const float ref = fmaxf(most, a.m);  // the row's maximum
+        const bool extra = y >= 0 && !sh.label_listed;  // the label as a class of its own
+
+        // The listed classes' exponentials e, e1, probabilities p (RENORM: times
+        // their sum), and four sums: of e, e1, p, and p (log p - (x - ref)/T).
+        float ex[E], ex1[E];
+        double p[E], sum[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = threadIdx.x + e * NT;
+            if (i < k ? sh.repeated[i] : !extra) id[e] = -1;
+            p[e] = 0;
+            ex[e] = ex1[e] = 0.f;
+            if (id[e] < 0) continue;
+            const float z = (x[e] - ref) * inv_t;
+            ex[e] = exp2_fast((x[e] - ref) * c);
+            ex1[e] = TWO ? exp2_fast((x[e] - ref) * LOG2E) : ex[e];
+            sum[0] += ex[e];
+            sum[1] += ex1[e];
+            if (i >= k || value[e] == -INFINITY) continue;
+            const double l = tail ? (double)value[e] : ((double)value[e] - most_value) / d.temperature;
+            p[e] = exp(l);
+            sum[2] += p[e];
+            if (p[e] != 0) sum[3] += p[e] * (l - z);
+        }
+        const int waves = min(W, (k >> 6) + 1);  // that hold listed classes
+        if (wave < waves)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sum[i] = wave_all(sum[i], Add());
+                if (lane == 0) sh.sum[i][wave] = sum[i];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sum[i] = sh.sum[i][0];
+            for (int j = 1; j < waves; ++j) sum[i] += sh.sum[i][j];
+        }
+
+        // The row's constants, by every thread.  Without a dense class of finite logit s is 0.
+        const float up = exp2_fast((a.m - ref) * c),
+                    up1 = TWO ? exp2_fast((a.m - ref) * LOG2E) : up;
+        const double total = sum[0] + (double)a.s * up, total1 = sum[1] + (double)a.s1 * up1;
+        const bool empty = total == 0;
+        // the largest logit counts exactly 1 in total
+        const float lse = log1pf((float)(total - 1)), lse1 = TWO ? log1pf((float)(total1 - 1)) : lse;
+        const float x_y = y < 0        ? 0.f
+                          : MODE == DELTA ? kept[k]
+                                          : (float)row[y];
+        double kd = 0, scale = 1, P = 0, rest = 0;
+        // the rest: the classes that the teacher does not list, relative to their maximum
+        const float top_rest = extra ? fmaxf(a.m, x_y) : a.m;
+        const float down = exp2_fast((a.m - top_rest) * c);
+        const float y_rest = extra ? exp2_fast((x_y - top_rest) * c) : 0.f;
+        const float sum_rest = a.s * down + y_rest;
+        if (k > 0 && tail) {
+            P = sum[2];
+            kd = sum[3] + lse * P;
+            if (sum_rest != 0.f) {
+                rest = P > 1 ? 0 : 1 - P;
+                if (rest != 0)
+                    kd += rest * (logf((float)rest) - (logf(sum_rest) + (top_rest - ref) * inv_t - lse));
+                P += rest;
+            }
+        } else if (k > 0 && sum[2] != 0) {
+            scale = 1 / sum[2];
+            P = sum[2] * scale;  // 1, or NaN
+            kd = sum[3] * scale - logf((float)sum[2]) + lse;
+        }
+        const float per_rest = rest == 0 ? 0.f : (float)(rest / sum_rest);
+        if (threadIdx.x == 0 && part == 0) {
+            double v = k > 0 ? (double)t.soft * d.temperature * d.temperature * kd : 0;
+            if (y >= 0) v += (double)t.hard * ((double)lse1 - ((double)x_y - ref));
+            const float l = empty ? 0.f : (float)(w * v);
+            if (loss) loss[r] = l;
+            if (row_loss) row_loss[r] = l;
+        }
+        if (!delta) continue;
+        const float soft = k > 0 ? -w * t.soft * d.temperature : 0.f, hard = y >= 0 ? -w * t.hard : 0.f;
+        const float P_total = empty ? 0.f : (float)(P / total),
+                    one_total = empty ? 0.f : (float)(1 / total1);
+        T *out = delta + (size_t)r * delta_stride + at;
+        {
+            float K = soft == 0.f ? 0.f : soft * (P_total * up - per_rest * down);
+            const float K1 = hard == 0.f ? 0.f : hard * one_total * up1;
+            if (!TWO) K += K1;
+            const auto grad = [&](float v) {
+                float o = K * exp2_fast((v - a.m) * c);
+                if (TWO) o = fmaf(K1, exp2_fast((v - a.m) * LOG2E), o);
+                return (T)o;
+            };
+            // from the end, which the caches hold
+            const int n = g.chunks();
+            for (int q = n - 1 - threadIdx.x; q >= 0; q -= NT) {
+                const Chunk v = Row<TYPE>::load(g.p + (size_t)q * V);
+                Chunk o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = grad((float)v[i]);
+                Row<TYPE>::store(out + (size_t)q * V, o);
+            }
+            if (threadIdx.x < g.rest()) out[n * V + threadIdx.x] = grad((float)g.p[n * V + threadIdx.x]);
+        }
+        __syncthreads();  // the listed classes over what was written for them
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (id[e] < at || id[e] >= at + g.len) continue;
+            float v = 0.f;
+            if (soft != 0.f) {
+                const float less = (int)threadIdx.x + e * NT < k ? (float)(p[e] * scale)
+                                                                 : per_rest * y_rest;
+                v = soft * (P_total * ex[e] - less);
+            }
+            if (hard != 0.f) v += hard * (one_total * ex1[e] - (id[e] == y ? 1.f : 0.f));
+            out[id[e] - at] = (T)(empty ? 0.f : v);
+        }
     }
 }
 
@@ -1130,26 +1203,26 @@ int ach_logprobs_fwd(const ach_logits_desc *desc, const void *logits, const int3
     uint64_t *lists = (uint64_t *)(part + (size_t)d.rows * sp.parts);
     const LogprobsOut o = {logprobs, ranks, entropy, stats, top_ids, top_logprobs};
     hipStream_t st = as_stream(s);
-#define GO_(TYPE, NT, E, R)                                                                       \
-    hipLaunchKernelGGL((k_logprobs<TYPE, NT, E, R>), grid, dim3(NT), 0, st, d,                    \
+#define GO(TYPE, NT, FULL, TOP)                                                                   \
+    hipLaunchKernelGGL((k_logprobs<TYPE, NT, FULL, TOP>), grid, dim3(NT), 0, st, d,               \
                        (const Elem<TYPE>::T *)logits, ids, k, o, sp.parts, sp.span, part, lists)
-#define GO(TYPE, NT)                                                                              \
+#define WITH(TYPE, FULL, TOP)                                                                     \
     do {                                                                                          \
-        if (entropy && ranks) GO_(TYPE, NT, true, true);                                          \
-        else if (entropy) GO_(TYPE, NT, true, false);                                             \
-        else if (ranks) GO_(TYPE, NT, false, true);                                               \
-        else GO_(TYPE, NT, false, false);                                                         \
+        if (nt == 64) GO(TYPE, 64, FULL, TOP);                                                    \
+        else GO(TYPE, 256, FULL, TOP);                                                            \
     } while (0)
 #define CALL(TYPE)                                                                                \
     do {                                                                                          \
-        if (nt == 64) GO(TYPE, 64);                                                               \
-        else if (nt == 256) GO(TYPE, 256);                                                        \
-        else GO(TYPE, 1024);                                                                      \
+        if (entropy || ranks) {                                                                   \
+            if (k) WITH(TYPE, true, true);                                                        \
+            else WITH(TYPE, true, false);                                                         \
+        } else if (k) WITH(TYPE, false, true);                                                    \
+        else WITH(TYPE, false, false);                                                            \
     } while (0)
     FOR_TYPE(d.type, CALL);
 #undef CALL
+#undef WITH
 #undef GO
-#undef GO_
     const int rc = check_launch();
     if (rc || sp.parts == 1) return rc;
 #define CALL(TYPE)                                                                                \
@@ -1195,8 +1268,7 @@ size_t ach_distill_workspace(const ach_logits_desc *desc, const ach_distill_desc
     const Split s = split_rows(d.rows, d.classes);
     size_t n = round16((size_t)d.rows * sizeof(float));
     if (s.parts > 1)
-        n += round16((size_t)d.rows * s.parts * sizeof(Dense)) +
-             (size_t)d.rows * (ACH_TOP_MAX + 1) * sizeof(Entry);
+        n += (size_t)d.rows * (s.parts * sizeof(Dense) + (ACH_TOP_MAX + 1) * sizeof(float));
     return n;
 }
 
@@ -1223,26 +1295,23 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
     hipStream_t st = as_stream(s);
     if (d.rows > 0) {
         const Split sp = split_rows(d.rows, d.classes);
-        const int nt = threads_for(sp.span, 0);
+        const int nt = sp.span <= T64 ? 64 : (size_t)sp.span * elem_size(d.type) <= D256 ? 256 : 1024;
         const bool two = t.soft != 0.f && t.hard != 0.f && d.temperature != 1.f;
         if (t.soft == 0.f) d.temperature = 1.f;  // the label's term is at temperature 1
         const dim3 grid(grid_of((size_t)d.rows * sp.parts));
         float *row_loss = (float *)ws;
         Dense *dense = (Dense *)((char *)ws + round16((size_t)d.rows * sizeof(float)));
-        Entry *entries =
-            (Entry *)((char *)dense + round16((size_t)d.rows * sp.parts * sizeof(Dense)));
+        const Between between = {dense, (float *)(dense + (size_t)d.rows * sp.parts)};
 #define GO(TYPE, NT, TWO, MODE)                                                                   \
     hipLaunchKernelGGL((k_distill<TYPE, NT, TWO, MODE>), grid, dim3(NT), 0, st, d, t,             \
                        (const Elem<TYPE>::T *)logits, teacher_ids, teacher_values, labels,        \
                        row_weights, loss, (Elem<TYPE>::T *)delta, delta_stride, row_loss,         \
-                       sp.parts, sp.span, dense, entries)
+                       sp.parts, sp.span, between)
 #define WITH(TYPE, TWO)                                                                           \
     do {                                                                                          \
         if (sp.parts > 1) {                                                                       \
-            if (nt == 256) GO(TYPE, 256, TWO, STATS);                                             \
-            else GO(TYPE, 1024, TWO, STATS);                                                      \
-            if (nt == 256) GO(TYPE, 256, TWO, DELTA);                                             \
-            else GO(TYPE, 1024, TWO, DELTA);                                                      \
+            GO(TYPE, 256, TWO, STATS);                                                            \
+            GO(TYPE, 256, TWO, DELTA);                                                            \
         } else if (nt == 64) GO(TYPE, 64, TWO, WHOLE);                                            \
         else if (nt == 256) GO(TYPE, 256, TWO, WHOLE);                                            \
         else GO(TYPE, 1024, TWO, WHOLE);                                                          \
