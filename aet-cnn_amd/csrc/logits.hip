@@ -16,8 +16,31 @@
 namespace ach {
 namespace {
 
+#ifndef MINW
+#define MINW 4
+#endif
+#ifndef MINF
+#define MINF 1
+#endif
+#ifndef SPLITN
+#define SPLITN 512
+#endif
+#ifndef SPLITM
+#define SPLITM 4096
+#endif
+#ifndef N512
+#define N512 1024
+#endif
+#ifndef N1K
+#define N1K 0
+#endif
+#ifndef DLDS
+#define DLDS 0
+#endif
 #ifndef T64
 #define T64 2048
+#endif
+#ifndef T256
 #define T256 16384
 #endif
 #ifndef D256
@@ -41,7 +64,12 @@ template <int TYPE> struct Row {
     static constexpr int VEC = 16 / sizeof(T);
     typedef T Chunk __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
     static __device__ __forceinline__ Chunk load(const T *p) { return *(const Chunk *)p; }
-    static __device__ __forceinline__ void store(T *p, Chunk v) { *(Chunk *)p = v; }
+    // PAST the caches: for gradients that these would not hold until they are read
+    template <bool PAST> static __device__ __forceinline__ void store(T *p, Chunk v)
+    {
+        if (PAST) __builtin_nontemporal_store(v, (Chunk *)p);
+        else *(Chunk *)p = v;
+    }
 };
 
 // Order of logits: larger values have larger keys, -0 equals +0.
@@ -108,6 +136,18 @@ __device__ __forceinline__ float wave_most(float v)
     v = fmaxf(v, dpp<0x142, 0xa>(v, v));
     v = fmaxf(v, dpp<0x143, 0xc>(v, v));
     return lane_value(v, 63);
+}
+
+template <bool B> struct Flag {
+    static constexpr bool value = B;
+};
+
+// Orders a wave's LDS accesses among its lanes.
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // Sum of v over the workgroup; every thread gets it.  sh holds one V per
@@ -194,9 +234,6 @@ __device__ __forceinline__ float absorb(Stat &a, const float (&x)[N], float c, f
 // the maxima of what a thread reads in 2^shift turns, a group, and of what is
 // left are kept.
 constexpr int UNROLL = 4, GROUPS = 16;
-#ifndef UNROLL_D
-#define UNROLL_D 4
-#endif
 
 template <int TYPE, int NT> struct Turns {
     int full, shift;
@@ -248,15 +285,17 @@ __device__ __forceinline__ Stat stream(const Range<TYPE> &g, const Turns<TYPE, N
         }
     }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);
-    for (int q = turns.full * U * NT + wave; q < n; q += NT) {
+    const int left = turns.full * U * NT + wave;  // fewer than U turns of one chunk
+    Chunk v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (left + u * NT + lane < n) v[u] = Row<TYPE>::load(g.p + (size_t)(left + u * NT + lane) * V);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (left + u * NT >= n) break;
         float x[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = -INFINITY;
-        if (q + lane < n) {
-            const Chunk v = Row<TYPE>::load(g.p + (size_t)(q + lane) * V);
-#pragma unroll
-            for (int i = 0; i < V; ++i) x[i] = (float)v[i];
-        }
+        for (int i = 0; i < V; ++i) x[i] = left + u * NT + lane < n ? (float)v[u][i] : -INFINITY;
         most = fmaxf(most, absorb<FULL>(a, x, c, x_id));
     }
     if (wave == 0) {
@@ -371,17 +410,17 @@ __device__ __forceinline__ Total total_of(const Range<TYPE> &g, Stat a, float c,
 template <int NT> struct TopLds {
     // logits above the bound, and at it; groups to be read again
     static constexpr int CAP = NT == 64 ? 256 : 1024, EQUAL = NT == 64 ? 128 : 512, HOT = 512;
-    uint64_t list[CAP + EQUAL];
+    alignas(16) uint64_t list[CAP + EQUAL + 8];
     uint64_t equal[EQUAL];
     GroupLds<NT> groups;
     uint32_t bound[NT / 64];
     int hot[HOT];
-    int sum[NT / 64];
+    int sum[NT / 64], places[64];
     int nhot, nlist, nequal;
 };
 
-// f(x, class) for every logit of the groups whose maximum reaches `low`,
-// which are listed unless they are too many.
+// f(logits, first class) for every chunk of the groups whose maximum reaches
+// `low`, which are listed unless they are too many, and the single elements.
 template <int TYPE, int NT, class F>
 __device__ __forceinline__ void each_hot(const Range<TYPE> &g, const Turns<TYPE, NT> &turns,
                                          const TopLds<NT> &sh, float low, F f)
@@ -390,8 +429,10 @@ __device__ __forceinline__ void each_hot(const Range<TYPE> &g, const Turns<TYPE,
     const auto chunk = [&](int q) {
         if (q < 0) return;
         const typename Row<TYPE>::Chunk v = Row<TYPE>::load(g.p + (size_t)q * V);
+        float x[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) f((float)v[e], g.begin + q * V + e);
+        for (int e = 0; e < V; ++e) x[e] = (float)v[e];
+        f(x, g.begin + q * V);
     };
     const int each = UNROLL << turns.shift;
     if (sh.nhot <= TopLds<NT>::HOT) {
@@ -408,8 +449,42 @@ __device__ __forceinline__ void each_hot(const Range<TYPE> &g, const Turns<TYPE,
     }
     if (threadIdx.x < g.rest()) {
         const int j = g.chunks() * V + threadIdx.x;
-        f((float)g.p[j], g.begin + j);
+        const float x[1] = {(float)g.p[j]};
+        f(x, g.begin + j);
     }
+}
+
+// Appends the logits that are (above or at the bound) to a list.
+template <int N>
+__device__ __forceinline__ void append(uint64_t *list, int cap, int *count, const float (&x)[N],
+                                       int j, const bool (&is)[N])
+{
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) n += is[e];
+    if (n == 0) return;
+    int at = atomicAdd(count, n);
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        if (is[e]) {
+            if (at < cap) list[at] = compound(x[e], j + e);
+            ++at;
+        }
+}
+
+// The upper 16 bits of the nth largest key of the wave's lanes: a lower bound,
+// 0 if there are not so many lanes.
+__device__ __forceinline__ uint32_t nth_largest(uint32_t key, int nth)
+{
+    uint32_t bound = 0;
+#pragma unroll
+    for (int b = 30; b >= 16; b -= 2) {  // two bits at a time
+        const int n1 = __popcll(__ballot(key >= (bound | 1u << b))),
+                  n2 = __popcll(__ballot(key >= (bound | 2u << b))),
+                  n3 = __popcll(__ballot(key >= (bound | 3u << b)));
+        bound |= (uint32_t)(n3 >= nth ? 3 : n2 >= nth ? 2 : n1 >= nth ? 1 : 0) << b;
+    }
+    return bound;
 }
 
 // Leaves in sh.list a superset of the k largest of the range (k <= its
@@ -422,11 +497,7 @@ __device__ __forceinline__ int candidates(const Range<TYPE> &g, const Turns<TYPE
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int nth = (k + W - 1) / W;
     const uint32_t key = order_key(mine);
-    uint32_t bound = 0;  // 16 bits of it: lower is as right
-    for (int b = 31; b >= 16; --b) {
-        const uint32_t up = bound | (1u << b);
-        if (__popcll(__ballot(key >= up)) >= nth) bound = up;
-    }
+    uint32_t bound = nth_largest(key, nth);
     __syncthreads();
     if (lane == 0) sh.bound[wave] = bound;
     if (threadIdx.x == 0) sh.nhot = sh.nlist = sh.nequal = 0;
@@ -435,24 +506,27 @@ __device__ __forceinline__ int candidates(const Range<TYPE> &g, const Turns<TYPE
     // up to -FLT_MAX, where a thread that has seen -inf alone starts: anything
     float low = bound <= order_key(-FLT_MAX) ? -INFINITY : key_value(bound);
     const float first_low = low;
-    if (mine >= low)
-        for (int group = 0; group <= GROUPS; ++group) {
-            if (group < GROUPS && (group << turns.shift) >= turns.full) continue;
-            if (sh.groups.most[group][threadIdx.x] >= low) {
-                const int i = atomicAdd(&sh.nhot, 1);
-                if (i < TopLds<NT>::HOT) sh.hot[i] = group * NT + threadIdx.x;
-            }
+    if (mine >= low) {
+        const int groups = (turns.full + (1 << turns.shift) - 1) >> turns.shift;
+        for (int i = 0; i <= groups; ++i) {
+            const int group = i < groups ? i : GROUPS;
+            if (sh.groups.most[group][threadIdx.x] < low) continue;
+            const int to = atomicAdd(&sh.nhot, 1);
+            if (to < TopLds<NT>::HOT) sh.hot[to] = group * NT + threadIdx.x;
         }
+    }
     __syncthreads();
     while (true) {
-        each_hot<TYPE, NT>(g, turns, sh, first_low, [&](float x, int j) {
-            if (x > low) {
-                const int i = atomicAdd(&sh.nlist, 1);
-                if (i < CAP) sh.list[i] = compound(x, j);
-            } else if (x == low && low != -INFINITY) {
-                const int i = atomicAdd(&sh.nequal, 1);
-                if (i < EQUAL) sh.equal[i] = compound(x, j);
+        each_hot<TYPE, NT>(g, turns, sh, first_low, [&](const auto &x, int j) {
+            constexpr int N = sizeof(x) / sizeof(float);
+            bool above[N], equal[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                above[e] = x[e] > low;
+                equal[e] = x[e] == low && low != -INFINITY;
             }
+            append(sh.list, CAP, &sh.nlist, x, j, above);
+            append(sh.equal, EQUAL, &sh.nequal, x, j, equal);
         });
         __syncthreads();
         if (sh.nlist <= CAP) break;
@@ -462,7 +536,9 @@ __device__ __forceinline__ int candidates(const Range<TYPE> &g, const Turns<TYPE
         for (int b = 31; b >= 0; --b) {
             const uint32_t up = kth | (1u << b);
             int count = 0;
-            each_hot<TYPE, NT>(g, turns, sh, first_low, [&](float x, int) { count += order_key(x) >= up; });
+            each_hot<TYPE, NT>(g, turns, sh, first_low, [&](const auto &x, int) {
+                for (float v : x) count += order_key(v) >= up;
+            });
             if (block_sum<NT>(count, sh.sum) >= k) kth = up;
         }
         low = key_value(kth);
@@ -498,14 +574,43 @@ __device__ __forceinline__ int candidates(const Range<TYPE> &g, const Turns<TYPE
     return k;
 }
 
-// emit(place, compound) for the k largest of list[0..n), largest first.
-template <int NT, class F>
-__device__ __forceinline__ void in_order(const uint64_t *list, int n, int k, F emit)
+// emit(place, compound) for the k largest of list[0..n), largest first, by
+// counting for each how many are before it.  The list is filled up with zeros,
+// which no logit's compound is below, to a multiple of 8 (there has to be
+// room).  Up to 64 are counted by all waves together, each against its share.
+__device__ __forceinline__ int count_larger(const uint64_t *list, int from, int to, uint64_t v)
 {
+    int n = 0;
+    for (int j = from; j < to; j += 8) {
+        uint64_t w[8];
+#pragma unroll
+        for (int l = 0; l < 8; ++l) w[l] = list[j + l];
+#pragma unroll
+        for (int l = 0; l < 8; ++l) n += w[l] > v;
+    }
+    return n;
+}
+
+template <int NT, class F>
+__device__ __forceinline__ void in_order(uint64_t *list, int n, int k, int *places, F emit)
+{
+    const int n8 = (n + 7) & ~7, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if ((int)threadIdx.x < n8 - n) list[n + threadIdx.x] = 0;
+    if (NT > 64 && n <= 64) {
+        if (wave == 0) places[lane] = 0;
+        __syncthreads();
+        const uint64_t v = lane < n ? list[lane] : 0;
+        const int share = (n8 / 8 + NT / 64 - 1) / (NT / 64) * 8, from = wave * share;
+        if (from < n8 && lane < n)
+            atomicAdd(&places[lane], count_larger(list, from, min(from + share, n8), v));
+        __syncthreads();
+        if (wave == 0 && lane < n && places[lane] < k) emit(places[lane], v);
+        return;
+    }
+    __syncthreads();
     for (int i = threadIdx.x; i < n; i += NT) {
         const uint64_t v = list[i];
-        int place = 0;
-        for (int j = 0; j < n; ++j) place += list[j] > v;
+        const int place = count_larger(list, 0, n8, v);
         if (place < k) emit(place, v);
     }
 }
@@ -556,7 +661,7 @@ template <class X, class Y> struct Pick<false, X, Y> {
 };
 
 template <int TYPE, int NT, bool FULL, bool TOP>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, MINF)
     k_logprobs(ach_logits_desc d, const typename Elem<TYPE>::T *__restrict__ logits,
                const int32_t *__restrict__ ids, int k, LogprobsOut o, int parts, int span,
                Total *__restrict__ part, uint64_t *__restrict__ lists)
@@ -589,10 +694,10 @@ __global__ void __launch_bounds__(NT)
         } else if (TOP) {
             const int mk = min(k, g.len), n = candidates<TYPE, NT>(g, turns, mine.m, mk, top);
             if (parts > 1) {
-                in_order<NT>(top.list, n, mk, [&](int i, uint64_t v) { lists[w * k + i] = v; });
+                in_order<NT>(top.list, n, mk, top.places, [&](int i, uint64_t v) { lists[w * k + i] = v; });
                 for (int i = mk + threadIdx.x; i < k; i += NT) lists[w * k + i] = 0;
             } else {
-                in_order<NT>(top.list, n, k, [&](int i, uint64_t v) {
+                in_order<NT>(top.list, n, k, top.places, [&](int i, uint64_t v) {
                     write_top(o, (size_t)r * k + i, v, a.m, inv_t, log_s);
                 });
             }
@@ -602,9 +707,12 @@ __global__ void __launch_bounds__(NT)
 }
 
 // Joins the parts of a row.  Of the parts' lists, for every m the m-th largest
-// of their ceil(k/m)-th entries bounds the k-th largest of all from below;
-// with m = 1, 2, 4, ... parts no more than k (2 + log2 parts) entries pass
-// the best of these bounds, however the large logits are spread.
+// of their ceil(k/m)-th entries bounds the k-th largest of all from below: one
+// part may hold the largest, or all parts evenly.  Entries that pass the best
+// of four such bounds, of 16 bits, are put in order.  If these are too many,
+// logits being equal or spread unevenly, the same bounds are taken exactly and
+// for every power of two: then, for m = 1, 2, 4, ..., no more than m lists have
+// ceil(k/m) entries that pass, which adds up to k (2 + log2 parts).
 constexpr int MOST_PARTS = 64;
 
 template <int TYPE, int NT>
@@ -613,30 +721,48 @@ __global__ void __launch_bounds__(NT)
                     const int32_t *__restrict__ ids, int k, LogprobsOut o, int parts,
                     const Total *__restrict__ part, const uint64_t *__restrict__ lists)
 {
+    constexpr int STAGE = 2048, CAP = ACH_TOP_MAX * 8, W = NT / 64;
+    static_assert(W == 4 && CAP >= ACH_TOP_MAX * 8, "four bounds; room for the exact ones");
     const float inv_t = 1.f / d.temperature, c = inv_t * LOG2E;
-    __shared__ uint64_t list[ACH_TOP_MAX * 8];
-    __shared__ uint64_t bounds[8];
-    __shared__ int n;
+    alignas(16) __shared__ uint64_t list[CAP + 8];
+    __shared__ uint64_t stage[STAGE], bounds[8], nth_of[W][64];
+    __shared__ int n, places[64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int r = blockIdx.x; r < d.rows; r += gridDim.x) {
-        // every wave joins the totals by itself
+        const int id = ids ? ids[r] : -1;
+        // the lists, where they fit, to be read from LDS
+        const uint64_t *from = lists + (size_t)r * parts * k;
+        const int entries = parts * k;
+        const bool staged = entries <= STAGE;
+        uint64_t staging[STAGE / NT];
+        if (staged)
+#pragma unroll
+            for (int i = 0; i < STAGE / NT; ++i)
+                if ((int)threadIdx.x + i * NT < entries) staging[i] = from[threadIdx.x + i * NT];
         Total a = {-INFINITY, 0.f, 0.f, 0};
         if (lane < parts) a = part[(size_t)r * parts + lane];
+        const bool given = id >= 0 && id < d.classes;
+        const float x_id = given ? (float)logits[(size_t)r * d.stride + id] : 0.f;
+        __syncthreads();  // of the last row
+        if (staged)
+#pragma unroll
+            for (int i = 0; i < STAGE / NT; ++i)
+                if ((int)threadIdx.x + i * NT < entries) stage[threadIdx.x + i * NT] = staging[i];
+        if (threadIdx.x == 0) n = 0;
+        const auto entry = [&](int i) { return staged ? stage[i] : from[i]; };
+        // every wave joins the totals by itself
         const bool bad = __any(!(a.rest < INFINITY));
-        const float m = wave_all(a.m, Max());
+        const float m = wave_most(a.m);
         const uint64_t at_max = __ballot(a.m == m && lane < parts);
         const int owner = at_max ? __ffsll((unsigned long long)at_max) - 1 : 0;
         const float z = m == -INFINITY ? 0.f : fmaxf((a.m - m) * c, FAR);
         const float f = a.m == -INFINITY ? 0.f : exp2_fast(z), s = 1.f + a.rest;
-        const float mine = a.m == -INFINITY ? 0.f : lane == owner ? a.rest : s * f;
         Total t;
         t.m = m;
-        t.rest = bad ? NAN : wave_all(mine, Add());
-        t.t = wave_all(a.m == -INFINITY ? 0.f : f * (a.t + s * z), Add());
+        t.rest = wave_total(a.m == -INFINITY ? 0.f : lane == owner ? a.rest : s * f);
+        if (bad) t.rest = NAN;
+        t.t = wave_total(a.m == -INFINITY ? 0.f : f * (a.t + s * z));
         t.above = wave_all(a.above, Add());
-        const int id = ids ? ids[r] : -1;
-        const bool given = id >= 0 && id < d.classes;
-        const float x_id = given ? (float)logits[(size_t)r * d.stride + id] : 0.f;
         const float log_s = write_row(o, r, t, given, x_id, inv_t, threadIdx.x == 0);
         if (k == 0) continue;
         if (bad) {
@@ -646,35 +772,56 @@ __global__ void __launch_bounds__(NT)
             }
             continue;
         }
-        const uint64_t *from = lists + (size_t)r * parts * k;
-        __syncthreads();
-        if (threadIdx.x < 8) bounds[threadIdx.x] = 0;
-        if (threadIdx.x == 0) n = 0;
-        __syncthreads();
-        for (int b = wave; b < 7 && (1 << b) <= parts; b += NT / 64) {
-            const int nth = (k + (1 << b) - 1) >> b;
-            const uint64_t v = lane < parts ? from[lane * k + nth - 1] : 0;
-            int before = 0;
-            for (int i = 0; i < parts; ++i) {
-                const uint64_t other = __shfl(v, i, 64);
-                before += other > v || (other == v && i < lane);
-            }
-            if (lane < parts && before == (1 << b) - 1) bounds[b] = v;
-        }
         __syncthreads();
         uint64_t low = 1;  // 0 fills up short lists
-        for (int b = 0; b < 7; ++b) low = max(low, bounds[b]);
-        for (int i = threadIdx.x; i < parts * k; i += NT) {
-            const uint64_t v = from[i];
-            if (v < low) continue;
-            const int to = atomicAdd(&n, 1);
-            if (to < ACH_TOP_MAX * 8) list[to] = v;
+        {
+            int most = 1;
+            while (most * 2 <= parts) most *= 2;
+            const int of[4] = {1, 4, 16, most}, mine = min(of[wave], most);
+            const int nth = (k + mine - 1) / mine;
+            const uint64_t v = lane < parts ? entry(lane * k + nth - 1) : 0;
+            const uint64_t bound = (uint64_t)nth_largest((uint32_t)(v >> 32), mine) << 32;
+            if (lane == 0) bounds[wave] = bound;
         }
         __syncthreads();
-        in_order<NT>(list, min(n, ACH_TOP_MAX * 8), k, [&](int i, uint64_t v) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) low = max(low, bounds[i]);
+        const auto collect = [&] {
+            for (int i = threadIdx.x; i < entries; i += NT) {
+                const uint64_t v = entry(i);
+                if (v < low) continue;
+                const int to = atomicAdd(&n, 1);
+                if (to < CAP) list[to] = v;
+            }
+            __syncthreads();
+        };
+        collect();
+        if (n > CAP) {
+            __syncthreads();
+            if (threadIdx.x < 8) bounds[threadIdx.x] = 0;
+            if (threadIdx.x == 0) n = 0;
+            __syncthreads();
+            for (int b = wave; b < 7 && (1 << b) <= parts; b += W) {
+                const int nth = (k + (1 << b) - 1) >> b;
+                const uint64_t v = lane < parts ? entry(lane * k + nth - 1) : 0;
+                nth_of[wave][lane] = v;
+                wave_sync();
+                int before = 0;
+                for (int i = 0; i < parts; ++i) {
+                    const uint64_t other = nth_of[wave][i];
+                    before += other > v || (other == v && i < lane);
+                }
+                wave_sync();
+                if (lane < parts && before == (1 << b) - 1) bounds[b] = v;
+            }
+            __syncthreads();
+            low = 1;
+            for (int b = 0; b < 7; ++b) low = max(low, bounds[b]);
+            collect();
+        }
+        in_order<NT>(list, min(n, CAP), k, places, [&](int i, uint64_t v) {
             write_top(o, (size_t)r * k + i, v, m, inv_t, log_s);
         });
-        __syncthreads();
     }
 }
 
@@ -687,7 +834,7 @@ __global__ void __launch_bounds__(256)
                    const int32_t *__restrict__ ids, const float *__restrict__ stats,
                    const float *__restrict__ entropy, const float *__restrict__ dlogprobs,
                    const float *__restrict__ dentropy, typename Elem<TYPE>::T *dlogits,
-                   int64_t dstride, int parts, int span)
+                   int64_t dstride, int parts, int span, bool past)
 {
     using T = typename Elem<TYPE>::T;
     constexpr int V = Row<TYPE>::VEC;
@@ -714,15 +861,19 @@ __global__ void __launch_bounds__(256)
             return v;
         };
         const int last = min(first + span, chunks);
-        for (int q = first + threadIdx.x; q < last; q += 256) {
-            Chunk v = {};
-            if (!none) {
-                const Chunk x = Row<TYPE>::load(row + (size_t)q * V);
+        const auto write = [&](auto PAST) {
+            for (int q = first + threadIdx.x; q < last; q += 256) {
+                Chunk v = {};
+                if (!none) {
+                    const Chunk x = Row<TYPE>::load(row + (size_t)q * V);
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = (T)grad((float)x[i], q * V + i);
+                    for (int i = 0; i < V; ++i) v[i] = (T)grad((float)x[i], q * V + i);
+                }
+                Row<TYPE>::template store<PAST.value>(out + (size_t)q * V, v);
             }
-            Row<TYPE>::store(out + (size_t)q * V, v);
-        }
+        };
+        if (past) write(Flag<true>());
+        else write(Flag<false>());
         if (last == chunks && threadIdx.x < rest) {
             const int j = chunks * V + threadIdx.x;
             out[j] = none ? (T)0.f : (T)grad((float)row[j], j);
@@ -751,23 +902,31 @@ __device__ __forceinline__ void raise_dense(Dense &a, float m, float c)
     a.m = m;
 }
 
+// N logits, unless they are to be left out.
 template <bool TWO, int N>
-__device__ __forceinline__ void absorb_dense(Dense &a, const float (&x)[N], float c)
+__device__ __forceinline__ void absorb_dense(Dense &a, const float (&x)[N], float c, bool out)
 {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
-    if (m > a.m) raise_dense<TWO>(a, m, c);
+    if (m > a.m && !out) raise_dense<TWO>(a, m, c);
+    float s = 0.f, s1 = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        a.s += exp2_fast((x[i] - a.m) * c);
-        if (TWO) a.s1 += exp2_fast((x[i] - a.m) * LOG2E);
+        s += exp2_fast((x[i] - a.m) * c);
+        if (TWO) s1 += exp2_fast((x[i] - a.m) * LOG2E);
     }
+    a.s += out ? 0.f : s;
+    if (TWO) a.s1 += out ? 0.f : s1;
 }
 
 template <int NT> struct DistillLds {
-    static constexpr int SEG = NT * 128;  // classes of one bitmap of listed classes
+    // classes whose listed ones are marked at once; at most 32 turns
+    static constexpr int SEG = NT * 512 < 131072 ? NT * 512 : 131072;
     uint32_t bits[SEG / 32];
+    uint32_t dirty[NT];        // by thread: the turns that read a listed class
+    int turn[ACH_TOP_MAX + 1]; // these, as turn * NT + thread
+    int nturn;
     int id[ACH_TOP_MAX];       // as the teacher gives them; -1: none
     int repeated[ACH_TOP_MAX];
     int label_listed;          // by the teacher
@@ -776,55 +935,78 @@ template <int NT> struct DistillLds {
     double sum[4][NT / 64];
 };
 
-// A thread's statistics of the dense classes of a range.
+// A thread's statistics of the dense classes of a range.  A turn that reads a
+// listed class is left out (by the one thread), and its chunks are read again
+// with the listed classes masked.
 template <int TYPE, int NT, bool TWO>
 __device__ __forceinline__ Dense stream_dense(const Range<TYPE> &all, float c, int k, int y,
                                               DistillLds<NT> &sh)
 {
-    constexpr int V = Row<TYPE>::VEC, U = UNROLL_D, SEG = DistillLds<NT>::SEG;
+    constexpr int V = Row<TYPE>::VEC, U = UNROLL, SEG = DistillLds<NT>::SEG;
     typedef typename Row<TYPE>::Chunk Chunk;
+    static_assert(SEG / (U * V * NT) <= 32, "turns of a segment");
     Dense a = {-FLT_MAX, 0.f, 0.f};
     for (int at = 0; at < all.len; at += SEG) {
         const Range<TYPE> g = {all.p + at, all.begin + at, min(SEG, all.len - at)};
+        const int n = g.chunks(), full = n / (U * NT);
         if (at > 0) __syncthreads();
         for (int i = threadIdx.x; i < (g.len + 31) / 32; i += NT) sh.bits[i] = 0;
+        sh.dirty[threadIdx.x] = 0;
+        if (threadIdx.x == 0) sh.nturn = 0;
         __syncthreads();
         for (int i = threadIdx.x; i <= k; i += NT) {
             const int j = (i < k ? sh.id[i] : y) - g.begin;
-            if (j >= 0 && j < g.len) atomicOr(&sh.bits[j >> 5], 1u << (j & 31));
+            if (j < 0 || j >= g.len) continue;
+            atomicOr(&sh.bits[j >> 5], 1u << (j & 31));
+            const int q = j / V, turn = q / (U * NT), thread = q % NT;
+            if (turn < full && !(atomicOr(&sh.dirty[thread], 1u << turn) >> turn & 1))
+                sh.turn[atomicAdd(&sh.nturn, 1)] = turn * NT + thread;
         }
         __syncthreads();
-        const int n = g.chunks();
-        // a chunk with its listed classes masked
-        const auto fetch = [&](const Chunk &v, int q, float *x) {
-            const uint32_t mask = (sh.bits[q * V >> 5] >> (q * V & 31)) & ((1u << V) - 1);
-#pragma unroll
-            for (int i = 0; i < V; ++i) x[i] = (float)v[i];
-            if (mask)
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (mask >> i & 1) x[i] = -INFINITY;
-        };
-        int q = threadIdx.x;
-        for (; q + (U - 1) * NT < n; q += U * NT) {
+        uint32_t dirty = sh.dirty[threadIdx.x];
+        const auto *p = g.p + (size_t)threadIdx.x * V;
+        for (int turn = 0; turn < full; ++turn, dirty >>= 1, p += (size_t)U * NT * V) {
             Chunk v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = Row<TYPE>::load(p + (size_t)u * NT * V);
             float x[U * V];
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = Row<TYPE>::load(g.p + (size_t)(q + u * NT) * V);
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int u = 0; u < U; ++u) fetch(v[u], q + u * NT, x + u * V);
-            absorb_dense<TWO>(a, x, c);
+                for (int i = 0; i < V; ++i) x[u * V + i] = (float)v[u][i];
+            absorb_dense<TWO>(a, x, c, dirty & 1);
         }
-        for (; q < n; q += NT) {
-            float x[V];
-            fetch(Row<TYPE>::load(g.p + (size_t)q * V), q, x);
-            absorb_dense<TWO>(a, x, c);
+        const int again = sh.nturn * U, left = full * U * NT, items = again + n - left;
+        for (int first = threadIdx.x; first < items; first += U * NT) {
+            Chunk v[U];
+            int at[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = first + u * NT;
+                at[u] = -1;
+                if (i >= items) continue;
+                at[u] = left + i - again;
+                if (i < again) {
+                    const int turn = sh.turn[i / U];
+                    at[u] = (turn / NT * U + i % U) * NT + turn % NT;
+                }
+                v[u] = Row<TYPE>::load(g.p + (size_t)at[u] * V);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (at[u] < 0) break;
+                const uint32_t mask = sh.bits[at[u] * V >> 5] >> (at[u] * V & 31);
+                float x[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[e] = mask >> e & 1 ? -INFINITY : (float)v[u][e];
+                absorb_dense<TWO>(a, x, c, false);
+            }
         }
         if (threadIdx.x < g.rest()) {
             const int j = n * V + threadIdx.x;
             const bool listed = sh.bits[j >> 5] >> (j & 31) & 1;
             const float x[1] = {listed ? -INFINITY : (float)g.p[j]};
-            absorb_dense<TWO>(a, x, c);
+            absorb_dense<TWO>(a, x, c, false);
         }
     }
     return a;
@@ -857,12 +1039,12 @@ struct Between {
 };
 
 template <int TYPE, int NT, bool TWO, int MODE>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, MINW)
     k_distill(ach_logits_desc d, ach_distill_desc t, const typename Elem<TYPE>::T *logits,
               const int32_t *__restrict__ teacher_ids, const void *__restrict__ teacher_values,
               const int32_t *__restrict__ labels, const float *__restrict__ row_weights,
               float *loss, typename Elem<TYPE>::T *delta, int64_t delta_stride, float *row_loss,
-              int parts, int span, Between between)
+              int parts, int span, Between between, bool past)
 {
     using T = typename Elem<TYPE>::T;
     typedef typename Row<TYPE>::Chunk Chunk;
@@ -883,7 +1065,7 @@ __global__ void __launch_bounds__(NT)
                 T *out = delta + (size_t)r * delta_stride + at;
                 const Chunk zero = {};
                 for (int q = threadIdx.x; q < g.chunks(); q += NT)
-                    Row<TYPE>::store(out + (size_t)q * V, zero);
+                    Row<TYPE>::template store<false>(out + (size_t)q * V, zero);
                 if (threadIdx.x < g.rest()) out[g.chunks() * V + threadIdx.x] = (T)0.f;
             }
             if (MODE != STATS && threadIdx.x == 0 && part == 0) {
@@ -1071,13 +1253,25 @@ __global__ void __launch_bounds__(NT)
             };
             // from the end, which the caches hold
             const int n = g.chunks();
-            for (int q = n - 1 - threadIdx.x; q >= 0; q -= NT) {
-                const Chunk v = Row<TYPE>::load(g.p + (size_t)q * V);
-                Chunk o;
+            const auto write = [&](auto PAST) {
+                constexpr int U = UNROLL;
+                for (int q = n - 1 - (int)threadIdx.x; q >= 0; q -= U * NT) {
+                    Chunk v[U];
 #pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = grad((float)v[i]);
-                Row<TYPE>::store(out + (size_t)q * V, o);
-            }
+                    for (int u = 0; u < U; ++u)
+                        if (q - u * NT >= 0) v[u] = Row<TYPE>::load(g.p + (size_t)(q - u * NT) * V);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        if (q - u * NT < 0) break;
+                        Chunk o;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) o[i] = grad((float)v[u][i]);
+                        Row<TYPE>::template store<PAST.value>(out + (size_t)(q - u * NT) * V, o);
+                    }
+                }
+            };
+            if (past) write(Flag<true>());
+            else write(Flag<false>());
             if (threadIdx.x < g.rest()) out[n * V + threadIdx.x] = grad((float)g.p[n * V + threadIdx.x]);
         }
         __syncthreads();  // the listed classes over what was written for them
@@ -1138,8 +1332,8 @@ struct Split {
 
 Split split_rows(int rows, int classes)
 {
-    int parts = rows > 0 ? 512 / rows : 1;
-    parts = parts < classes / 4096 ? parts : classes / 4096;
+    int parts = rows > 0 ? SPLITN / rows : 1;
+    parts = parts < classes / SPLITM ? parts : classes / SPLITM;
     if (parts > MOST_PARTS) parts = MOST_PARTS;
     if (parts < 2) return {1, classes};
     const int span = (int)((((int64_t)classes + parts - 1) / parts + 63) / 64 * 64);
@@ -1152,6 +1346,14 @@ int threads_for(int span, int k)
 {
     if (span <= T64 && k <= 32) return 64;
     return span <= T256 ? 256 : 1024;
+}
+
+// Gradients of more than the L2 caches hold (8 of 4 MB) are stored past them:
+// what reads them next finds them in memory either way, and the logits that
+// the kernel reads a second time stay cached.
+bool past_caches(const ach_logits_desc &d)
+{
+    return (size_t)d.rows * d.classes * elem_size(d.type) > (size_t)32 << 20;
 }
 
 unsigned grid_of(size_t n) { return (unsigned)(n < (1u << 20) ? n : 1u << 20); }
@@ -1197,7 +1399,7 @@ int ach_logprobs_fwd(const ach_logits_desc *desc, const void *logits, const int3
     if (need && (!ws || ws_bytes < need || !aligned(ws, 16))) return ACH_EWORKSPACE;
     if (d.rows == 0) return ACH_OK;
     const Split sp = split_rows(d.rows, d.classes);
-    const int nt = threads_for(sp.span, k);
+    const int nt = d.rows * sp.parts <= N1K && sp.span >= 32768 ? 1024 : d.rows * sp.parts < N512 && sp.span >= 32768 ? 512 : sp.span <= T64 && k <= 32 ? 64 : 256;
     const dim3 grid(grid_of((size_t)d.rows * sp.parts));
     Total *part = (Total *)ws;
     uint64_t *lists = (uint64_t *)(part + (size_t)d.rows * sp.parts);
@@ -1209,6 +1411,8 @@ int ach_logprobs_fwd(const ach_logits_desc *desc, const void *logits, const int3
 #define WITH(TYPE, FULL, TOP)                                                                     \
     do {                                                                                          \
         if (nt == 64) GO(TYPE, 64, FULL, TOP);                                                    \
+        else if (nt == 512) GO(TYPE, 512, FULL, TOP);                                             \
+        else if (nt == 1024) GO(TYPE, 1024, FULL, TOP);                                           \
         else GO(TYPE, 256, FULL, TOP);                                                            \
     } while (0)
 #define CALL(TYPE)                                                                                \
@@ -1249,11 +1453,12 @@ int ach_logprobs_bwd(const ach_logits_desc *desc, const void *logits, const int3
     const int chunks = d.classes / (16 / (int)elem_size(d.type)), span = 1024;
     const int parts = chunks > span ? (chunks + span - 1) / span : 1;
     const dim3 grid(grid_of((size_t)d.rows * parts)), block(256);
+    const bool past = past_caches(d);
     hipStream_t st = as_stream(s);
 #define CALL(TYPE)                                                                                \
     hipLaunchKernelGGL((k_logprobs_bwd<TYPE>), grid, block, 0, st, d,                             \
                        (const Elem<TYPE>::T *)logits, ids, stats, entropy, dlogprobs, dentropy,   \
-                       (Elem<TYPE>::T *)dlogits, dstride, parts, span)
+                       (Elem<TYPE>::T *)dlogits, dstride, parts, span, past)
     FOR_TYPE(d.type, CALL);
 #undef CALL
     return check_launch();
@@ -1295,18 +1500,19 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
     hipStream_t st = as_stream(s);
     if (d.rows > 0) {
         const Split sp = split_rows(d.rows, d.classes);
-        const int nt = sp.span <= T64 ? 64 : (size_t)sp.span * elem_size(d.type) <= D256 ? 256 : 1024;
+        const int nt = sp.span <= T64 ? 64 : (size_t)sp.span * elem_size(d.type) <= D256 ? 256 : 512;
         const bool two = t.soft != 0.f && t.hard != 0.f && d.temperature != 1.f;
         if (t.soft == 0.f) d.temperature = 1.f;  // the label's term is at temperature 1
         const dim3 grid(grid_of((size_t)d.rows * sp.parts));
+        const bool past = past_caches(d);
         float *row_loss = (float *)ws;
         Dense *dense = (Dense *)((char *)ws + round16((size_t)d.rows * sizeof(float)));
         const Between between = {dense, (float *)(dense + (size_t)d.rows * sp.parts)};
 #define GO(TYPE, NT, TWO, MODE)                                                                   \
-    hipLaunchKernelGGL((k_distill<TYPE, NT, TWO, MODE>), grid, dim3(NT), 0, st, d, t,             \
+    hipLaunchKernelGGL((k_distill<TYPE, NT, TWO, MODE>), grid, dim3(NT), DLDS, st, d, t,            \
                        (const Elem<TYPE>::T *)logits, teacher_ids, teacher_values, labels,        \
                        row_weights, loss, (Elem<TYPE>::T *)delta, delta_stride, row_loss,         \
-                       sp.parts, sp.span, between)
+                       sp.parts, sp.span, between, past)
 #define WITH(TYPE, TWO)                                                                           \
     do {                                                                                          \
         if (sp.parts > 1) {                                                                       \
@@ -1314,7 +1520,7 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
             GO(TYPE, 256, TWO, DELTA);                                                            \
         } else if (nt == 64) GO(TYPE, 64, TWO, WHOLE);                                            \
         else if (nt == 256) GO(TYPE, 256, TWO, WHOLE);                                            \
-        else GO(TYPE, 1024, TWO, WHOLE);                                                          \
+        else GO(TYPE, 512, TWO, WHOLE);                                                           \
     } while (0)
 #define CALL(TYPE)                                                                                \
     do {                                                                                          \
