@@ -34,6 +34,21 @@ namespace {
 #ifndef N1K
 #define N1K 0
 #endif
+#ifndef R64
+#define R64 8192
+#endif
+#ifndef S512
+#define S512 16384
+#endif
+#ifndef N512D
+#define N512D 0
+#endif
+#ifndef NOIN
+#define NOIN __forceinline__
+#endif
+#ifndef NOIN2
+#define NOIN2 __forceinline__
+#endif
 #ifndef DLDS
 #define DLDS 0
 #endif
@@ -69,6 +84,34 @@ template <int TYPE> struct Row {
     {
         if (PAST) __builtin_nontemporal_store(v, (Chunk *)p);
         else *(Chunk *)p = v;
+    }
+};
+
+// The elements of a chunk one after the other, in a loop that is not unrolled:
+// what a workgroup does once per row costs more to fetch than to run.
+template <int TYPE> struct Walk {
+    static constexpr int VEC = Row<TYPE>::VEC;
+    uint32_t w[4];
+    __device__ explicit Walk(const typename Row<TYPE>::T *p)
+    {
+        const typename Row<TYPE>::Chunk v = Row<TYPE>::load(p);
+        __builtin_memcpy(w, &v, 16);
+    }
+    __device__ __forceinline__ float next()
+    {
+        const uint32_t first = w[0];
+        if (TYPE == ACH_F32) {
+            w[0] = w[1], w[1] = w[2], w[2] = w[3];
+            return __uint_as_float(first);
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i) w[i] = w[i] >> 16 | w[i + 1] << 16;
+        w[3] >>= 16;
+        if (TYPE == ACH_BF16) return __uint_as_float(first << 16);
+        const uint16_t half = (uint16_t)first;
+        _Float16 h;
+        __builtin_memcpy(&h, &half, 2);
+        return (float)h;
     }
 };
 
@@ -233,9 +276,11 @@ __device__ __forceinline__ float absorb(Stat &a, const float (&x)[N], float c, f
 // chunk q by thread q % NT, then what is left.  With alternatives to be found,
 // the maxima of what a thread reads in 2^shift turns, a group, and of what is
 // left are kept.
-constexpr int UNROLL = 4, GROUPS = 16;
+constexpr int UNROLL = 4;
+constexpr int groups_of(int threads) { return threads == 64 ? 8 : 16; }
 
 template <int TYPE, int NT> struct Turns {
+    static constexpr int GROUPS = groups_of(NT);
     int full, shift;
     __device__ explicit Turns(const Range<TYPE> &g)
         : full(g.chunks() / (UNROLL * NT)), shift(0)
@@ -253,7 +298,7 @@ template <int TYPE, int NT> struct Turns {
 };
 
 template <int NT> struct GroupLds {
-    float most[GROUPS + 1][NT];
+    float most[groups_of(NT) + 1][NT];
 };
 
 template <int TYPE, int NT, bool FULL, bool TOP>
@@ -302,7 +347,7 @@ __device__ __forceinline__ Stat stream(const Range<TYPE> &g, const Turns<TYPE, N
         const float x[1] = {lane < g.rest() ? (float)g.p[(size_t)n * V + lane] : -INFINITY};
         most = fmaxf(most, absorb<FULL>(a, x, c, x_id));
     }
-    if (TOP) groups->most[GROUPS][threadIdx.x] = most;
+    if (TOP) groups->most[groups_of(NT)][threadIdx.x] = most;
     return a;
 }
 
@@ -409,7 +454,8 @@ __device__ __forceinline__ Total total_of(const Range<TYPE> &g, Stat a, float c,
 // how many are before it.
 template <int NT> struct TopLds {
     // logits above the bound, and at it; groups to be read again
-    static constexpr int CAP = NT == 64 ? 256 : 1024, EQUAL = NT == 64 ? 128 : 512, HOT = 512;
+    static constexpr int CAP = NT == 64 ? 256 : 1024, EQUAL = NT == 64 ? 128 : 512,
+                         HOT = NT == 64 ? 128 : 512, GROUPS = groups_of(NT);
     alignas(16) uint64_t list[CAP + EQUAL + 8];
     uint64_t equal[EQUAL];
     GroupLds<NT> groups;
@@ -419,20 +465,18 @@ template <int NT> struct TopLds {
     int nhot, nlist, nequal;
 };
 
-// f(logits, first class) for every chunk of the groups whose maximum reaches
-// `low`, which are listed unless they are too many, and the single elements.
+// f(x, class) for every logit of the groups whose maximum reaches `low`,
+// which are listed unless they are too many, and the single elements.
 template <int TYPE, int NT, class F>
 __device__ __forceinline__ void each_hot(const Range<TYPE> &g, const Turns<TYPE, NT> &turns,
                                          const TopLds<NT> &sh, float low, F f)
 {
-    constexpr int V = Row<TYPE>::VEC;
+    constexpr int V = Row<TYPE>::VEC, GROUPS = groups_of(NT);
     const auto chunk = [&](int q) {
         if (q < 0) return;
-        const typename Row<TYPE>::Chunk v = Row<TYPE>::load(g.p + (size_t)q * V);
-        float x[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = (float)v[e];
-        f(x, g.begin + q * V);
+        Walk<TYPE> walk(g.p + (size_t)q * V);
+#pragma unroll 1
+        for (int e = 0; e < V; ++e) f(walk.next(), g.begin + q * V + e);
     };
     const int each = UNROLL << turns.shift;
     if (sh.nhot <= TopLds<NT>::HOT) {
@@ -449,27 +493,8 @@ __device__ __forceinline__ void each_hot(const Range<TYPE> &g, const Turns<TYPE,
     }
     if (threadIdx.x < g.rest()) {
         const int j = g.chunks() * V + threadIdx.x;
-        const float x[1] = {(float)g.p[j]};
-        f(x, g.begin + j);
+        f((float)g.p[j], g.begin + j);
     }
-}
-
-// Appends the logits that are (above or at the bound) to a list.
-template <int N>
-__device__ __forceinline__ void append(uint64_t *list, int cap, int *count, const float (&x)[N],
-                                       int j, const bool (&is)[N])
-{
-    int n = 0;
-#pragma unroll
-    for (int e = 0; e < N; ++e) n += is[e];
-    if (n == 0) return;
-    int at = atomicAdd(count, n);
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-        if (is[e]) {
-            if (at < cap) list[at] = compound(x[e], j + e);
-            ++at;
-        }
 }
 
 // The upper 16 bits of the nth largest key of the wave's lanes: a lower bound,
@@ -477,12 +502,10 @@ __device__ __forceinline__ void append(uint64_t *list, int cap, int *count, cons
 __device__ __forceinline__ uint32_t nth_largest(uint32_t key, int nth)
 {
     uint32_t bound = 0;
-#pragma unroll
-    for (int b = 30; b >= 16; b -= 2) {  // two bits at a time
-        const int n1 = __popcll(__ballot(key >= (bound | 1u << b))),
-                  n2 = __popcll(__ballot(key >= (bound | 2u << b))),
-                  n3 = __popcll(__ballot(key >= (bound | 3u << b)));
-        bound |= (uint32_t)(n3 >= nth ? 3 : n2 >= nth ? 2 : n1 >= nth ? 1 : 0) << b;
+#pragma unroll 1
+    for (int b = 31; b >= 16; --b) {
+        const uint32_t up = bound | 1u << b;
+        if (__popcll(__ballot(key >= up)) >= nth) bound = up;
     }
     return bound;
 }
@@ -494,6 +517,7 @@ __device__ __forceinline__ int candidates(const Range<TYPE> &g, const Turns<TYPE
                                           float mine, int k, TopLds<NT> &sh)
 {
     constexpr int CAP = TopLds<NT>::CAP, EQUAL = TopLds<NT>::EQUAL, W = NT / 64;
+    constexpr int GROUPS = groups_of(NT);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int nth = (k + W - 1) / W;
     const uint32_t key = order_key(mine);
@@ -517,16 +541,11 @@ __device__ __forceinline__ int candidates(const Range<TYPE> &g, const Turns<TYPE
     }
     __syncthreads();
     while (true) {
-        each_hot<TYPE, NT>(g, turns, sh, first_low, [&](const auto &x, int j) {
-            constexpr int N = sizeof(x) / sizeof(float);
-            bool above[N], equal[N];
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                above[e] = x[e] > low;
-                equal[e] = x[e] == low && low != -INFINITY;
-            }
-            append(sh.list, CAP, &sh.nlist, x, j, above);
-            append(sh.equal, EQUAL, &sh.nequal, x, j, equal);
+        each_hot<TYPE, NT>(g, turns, sh, first_low, [&](float x, int j) {
+            if (!(x >= low) || x == -INFINITY) return;
+            const bool above = x > low;
+            const int i = atomicAdd(above ? &sh.nlist : &sh.nequal, 1);
+            if (i < (above ? CAP : EQUAL)) (above ? sh.list : sh.equal)[i] = compound(x, j);
         });
         __syncthreads();
         if (sh.nlist <= CAP) break;
@@ -536,9 +555,8 @@ __device__ __forceinline__ int candidates(const Range<TYPE> &g, const Turns<TYPE
         for (int b = 31; b >= 0; --b) {
             const uint32_t up = kth | (1u << b);
             int count = 0;
-            each_hot<TYPE, NT>(g, turns, sh, first_low, [&](const auto &x, int) {
-                for (float v : x) count += order_key(v) >= up;
-            });
+            each_hot<TYPE, NT>(g, turns, sh, first_low,
+                               [&](float x, int) { count += order_key(x) >= up; });
             if (block_sum<NT>(count, sh.sum) >= k) kth = up;
         }
         low = key_value(kth);
@@ -894,7 +912,19 @@ struct Dense {
     float m, s, s1;
 };
 
-template <bool TWO>
+// Whether the label's exponentials, at temperature 1, are wanted next to the
+// teacher's, and how they are had: not apart (ONE), on their own, or at
+// temperatures 2 and 4 as powers of these, a third less work for a row.
+enum { ONE = 0, BOTH = 1, SQUARE = 2, FOURTH = 4 };
+
+template <int TWO> __device__ __forceinline__ float second(float e, float d)
+{
+    if (TWO == BOTH) return exp2_fast(d * LOG2E);
+    const float e2 = e * e;
+    return TWO == SQUARE ? e2 : e2 * e2;
+}
+
+template <int TWO>
 __device__ __forceinline__ void raise_dense(Dense &a, float m, float c)
 {
     a.s *= exp2_fast(fmaxf((a.m - m) * c, FAR));
@@ -903,7 +933,7 @@ __device__ __forceinline__ void raise_dense(Dense &a, float m, float c)
 }
 
 // N logits, unless they are to be left out.
-template <bool TWO, int N>
+template <int TWO, int N>
 __device__ __forceinline__ void absorb_dense(Dense &a, const float (&x)[N], float c, bool out)
 {
     float m = x[0];
@@ -913,33 +943,113 @@ __device__ __forceinline__ void absorb_dense(Dense &a, const float (&x)[N], floa
     float s = 0.f, s1 = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        s += exp2_fast((x[i] - a.m) * c);
-        if (TWO) s1 += exp2_fast((x[i] - a.m) * LOG2E);
+        const float d = x[i] - a.m, e = exp2_fast(d * c);
+        s += e;
+        if (TWO) s1 += second<TWO>(e, d);
     }
     a.s += out ? 0.f : s;
     if (TWO) a.s1 += out ? 0.f : s1;
 }
 
+// A wave's listed classes (classes 64 w to 64 w + 63 of the list): their
+// maximum `most` (0 if none is finite) and that of the teacher's values, and
+// relative to these the sums of e, e1, p, and p (log p - (x - most)/T).
+struct Listed {
+    float most, most_value;
+    double e, e1, p, l;
+};
+constexpr int LISTED_WAVES = (ACH_TOP_MAX + 1 + 63) / 64;
+
+// One listed class: relative to its wave's maxima.
+struct Entry {
+    int id;  // -1: none
+    float e, e1, p;
+};
+
 template <int NT> struct DistillLds {
     // classes whose listed ones are marked at once; at most 32 turns
     static constexpr int SEG = NT * 512 < 131072 ? NT * 512 : 131072;
     uint32_t bits[SEG / 32];
-    uint32_t dirty[NT];        // by thread: the turns that read a listed class
-    int turn[ACH_TOP_MAX + 1]; // these, as turn * NT + thread
+    uint32_t dirty[NT];         // by thread: the turns that read a listed class
+    int turn[ACH_TOP_MAX + 1];  // these, as turn * NT + thread
     int nturn;
-    int id[ACH_TOP_MAX];       // as the teacher gives them; -1: none
-    int repeated[ACH_TOP_MAX];
-    int label_listed;          // by the teacher
+    int id[ACH_TOP_MAX + 1];    // as they are given, the label at [k]; -1: none
+    int repeated[ACH_TOP_MAX + 1];
     Dense wave[NT / 64];
-    float most[NT / 64], most_value[NT / 64];
-    double sum[4][NT / 64];
+    Listed listed[LISTED_WAVES];
+    float x_y;                  // the label's logit
+    int extra;                  // the label is a class that the teacher does not list
 };
+
+// Marks the listed classes of a range, and the turns of `each` chunks a thread
+// that read them (the first `full` turns).  Starts and ends with a barrier.
+template <int TYPE, int NT>
+__device__ __forceinline__ void mark(const Range<TYPE> &g, int k, int each, int full,
+                                     DistillLds<NT> &sh)
+{
+    constexpr int V = Row<TYPE>::VEC;
+    __syncthreads();
+    for (int i = threadIdx.x; i < (g.len + 31) / 32; i += NT) sh.bits[i] = 0;
+    sh.dirty[threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.nturn = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i <= k; i += NT) {
+        const int j = sh.id[i] - g.begin;
+        if (j < 0 || j >= g.len) continue;
+        atomicOr(&sh.bits[j >> 5], 1u << (j & 31));
+        const int q = j / V, turn = q / (each * NT), thread = q % NT;
+        if (turn < full && !(atomicOr(&sh.dirty[thread], 1u << turn) >> turn & 1))
+            sh.turn[atomicAdd(&sh.nturn, 1)] = turn * NT + thread;
+    }
+    __syncthreads();
+}
+
+// The chunks of the marked turns, the chunks from `left` on and the single
+// elements, with the listed classes masked.
+template <int TYPE, int NT, int TWO>
+__device__ __forceinline__ void absorb_masked(Dense &a, const Range<TYPE> &g, float c, int each,
+                                              int left, const DistillLds<NT> &sh)
+{
+    constexpr int V = Row<TYPE>::VEC, U = UNROLL;
+    const int n = g.chunks(), again = sh.nturn * each, items = again + n - left;
+    for (int first = threadIdx.x; first < items; first += U * NT) {
+        typename Row<TYPE>::Chunk v[U];
+        int at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = first + u * NT;
+            at[u] = -1;
+            if (i >= items) continue;
+            at[u] = left + i - again;
+            if (i < again) {
+                const int turn = sh.turn[i / each];
+                at[u] = (turn / NT * each + i % each) * NT + turn % NT;
+            }
+            v[u] = Row<TYPE>::load(g.p + (size_t)at[u] * V);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (at[u] < 0) break;
+            const uint32_t mask = sh.bits[at[u] * V >> 5] >> (at[u] * V & 31);
+            float x[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = mask >> e & 1 ? -INFINITY : (float)v[u][e];
+            absorb_dense<TWO>(a, x, c, false);
+        }
+    }
+    if (threadIdx.x < g.rest()) {
+        const int j = n * V + threadIdx.x;
+        const bool listed = sh.bits[j >> 5] >> (j & 31) & 1;
+        const float x[1] = {listed ? -INFINITY : (float)g.p[j]};
+        absorb_dense<TWO>(a, x, c, false);
+    }
+}
 
 // A thread's statistics of the dense classes of a range.  A turn that reads a
 // listed class is left out (by the one thread), and its chunks are read again
 // with the listed classes masked.
-template <int TYPE, int NT, bool TWO>
-__device__ __forceinline__ Dense stream_dense(const Range<TYPE> &all, float c, int k, int y,
+template <int TYPE, int NT, int TWO>
+__device__ __forceinline__ Dense stream_dense(const Range<TYPE> &all, float c, int k,
                                               DistillLds<NT> &sh)
 {
     constexpr int V = Row<TYPE>::VEC, U = UNROLL, SEG = DistillLds<NT>::SEG;
@@ -948,21 +1058,8 @@ __device__ __forceinline__ Dense stream_dense(const Range<TYPE> &all, float c, i
     Dense a = {-FLT_MAX, 0.f, 0.f};
     for (int at = 0; at < all.len; at += SEG) {
         const Range<TYPE> g = {all.p + at, all.begin + at, min(SEG, all.len - at)};
-        const int n = g.chunks(), full = n / (U * NT);
-        if (at > 0) __syncthreads();
-        for (int i = threadIdx.x; i < (g.len + 31) / 32; i += NT) sh.bits[i] = 0;
-        sh.dirty[threadIdx.x] = 0;
-        if (threadIdx.x == 0) sh.nturn = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i <= k; i += NT) {
-            const int j = (i < k ? sh.id[i] : y) - g.begin;
-            if (j < 0 || j >= g.len) continue;
-            atomicOr(&sh.bits[j >> 5], 1u << (j & 31));
-            const int q = j / V, turn = q / (U * NT), thread = q % NT;
-            if (turn < full && !(atomicOr(&sh.dirty[thread], 1u << turn) >> turn & 1))
-                sh.turn[atomicAdd(&sh.nturn, 1)] = turn * NT + thread;
-        }
-        __syncthreads();
+        const int full = g.chunks() / (U * NT);
+        mark<TYPE, NT>(g, k, U, full, sh);
         uint32_t dirty = sh.dirty[threadIdx.x];
         const auto *p = g.p + (size_t)threadIdx.x * V;
         for (int turn = 0; turn < full; ++turn, dirty >>= 1, p += (size_t)U * NT * V) {
@@ -976,44 +1073,13 @@ __device__ __forceinline__ Dense stream_dense(const Range<TYPE> &all, float c, i
                 for (int i = 0; i < V; ++i) x[u * V + i] = (float)v[u][i];
             absorb_dense<TWO>(a, x, c, dirty & 1);
         }
-        const int again = sh.nturn * U, left = full * U * NT, items = again + n - left;
-        for (int first = threadIdx.x; first < items; first += U * NT) {
-            Chunk v[U];
-            int at[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = first + u * NT;
-                at[u] = -1;
-                if (i >= items) continue;
-                at[u] = left + i - again;
-                if (i < again) {
-                    const int turn = sh.turn[i / U];
-                    at[u] = (turn / NT * U + i % U) * NT + turn % NT;
-                }
-                v[u] = Row<TYPE>::load(g.p + (size_t)at[u] * V);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (at[u] < 0) break;
-                const uint32_t mask = sh.bits[at[u] * V >> 5] >> (at[u] * V & 31);
-                float x[V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) x[e] = mask >> e & 1 ? -INFINITY : (float)v[u][e];
-                absorb_dense<TWO>(a, x, c, false);
-            }
-        }
-        if (threadIdx.x < g.rest()) {
-            const int j = n * V + threadIdx.x;
-            const bool listed = sh.bits[j >> 5] >> (j & 31) & 1;
-            const float x[1] = {listed ? -INFINITY : (float)g.p[j]};
-            absorb_dense<TWO>(a, x, c, false);
-        }
+        absorb_masked<TYPE, NT, TWO>(a, g, c, U, full * U * NT, sh);
     }
     return a;
 }
 
 // The same of the wave, in all its lanes.
-template <bool TWO> __device__ __forceinline__ void wave_dense(Dense &a, float c)
+template <int TWO> __device__ __forceinline__ void wave_dense(Dense &a, float c)
 {
     raise_dense<TWO>(a, wave_most(a.m), c);
     a.s = wave_total(a.s);
@@ -1027,19 +1093,169 @@ __device__ __forceinline__ float load_any(const void *p, int type, size_t i)
                               : (float)((const _Float16 *)p)[i];
 }
 
-// What a launch does: all of it, a row to a workgroup; or, for rows in parts,
-// the statistics of the dense classes, then all else.
-enum { WHOLE, STATS, DELTA };
+// The listed classes of a row.  Class i of the list belongs to thread i, or
+// i mod NT; `entry` are the thread's, the waves' sums are left in sh.listed.
+// sh.id has been filled in, and a barrier has been since.
+template <int TYPE, int NT, int TWO, int E>
+__device__ NOIN void listed_terms(Entry (&entry)[E], const typename Elem<TYPE>::T *row,
+                                             const void *values, int type, size_t at, int k,
+                                             bool tail, float temperature, DistillLds<NT> &sh)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float inv_t = 1.f / temperature, c = inv_t * LOG2E;
+    if (wave >= min(NT / 64, (k >> 6) + 1)) {  // of the waves, those that have some
+#pragma unroll
+        for (int e = 0; e < E; ++e) entry[e].id = -1;
+        return;
+    }
+    Listed sum = {-INFINITY, -INFINITY, 0, 0, 0, 0};
+    float x[E], value[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int i = threadIdx.x + e * NT;
+        entry[e].id = i <= k ? sh.id[i] : -1;
+        x[e] = value[e] = -INFINITY;
+        if (entry[e].id < 0) continue;
+        // of entries with the same id the first counts; the label, at [k], is last
+        if (sh.repeated[i]) {
+            if (i == k) sh.x_y = (float)row[entry[e].id];
+            entry[e].id = -1;
+            continue;
+        }
+        x[e] = (float)row[entry[e].id];
+        if (i < k) value[e] = load_any(values, type, at + i);
+        else sh.x_y = x[e];
+        sum.most = fmaxf(sum.most, x[e]);
+        sum.most_value = fmaxf(sum.most_value, value[e]);
+    }
+    sum.most = wave_most(sum.most);
+    sum.most_value = wave_most(sum.most_value);
+    if (sum.most == -INFINITY) sum.most = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        entry[e].e = entry[e].e1 = entry[e].p = 0.f;
+        if (entry[e].id < 0) continue;
+        entry[e].e = exp2_fast((x[e] - sum.most) * c);
+        entry[e].e1 = TWO ? exp2_fast((x[e] - sum.most) * LOG2E) : entry[e].e;
+        sum.e += entry[e].e;
+        sum.e1 += entry[e].e1;
+        if (value[e] == -INFINITY) continue;
+        const double l = tail ? (double)value[e] : ((double)value[e] - sum.most_value) / temperature;
+        const double p = exp(l);
+        entry[e].p = (float)p;
+        sum.p += p;
+        if (p != 0) sum.l += p * (l - (x[e] - sum.most) * inv_t);
+    }
+    sum.e = wave_all(sum.e, Add());
+    sum.e1 = wave_all(sum.e1, Add());
+    sum.p = wave_all(sum.p, Add());
+    sum.l = wave_all(sum.l, Add());
+    if (lane == 0) sh.listed[wave] = sum;
+}
 
-// Where the first of two launches leaves its results: the parts' statistics,
-// and the logits of the listed classes, which the second may overwrite.
-struct Between {
-    Dense *dense;
-    float *x;  // [row][ACH_TOP_MAX + 1], the label's at [k]
+// What the delta and the loss of a row are made of.
+struct RowTerms {
+    float m;              // of the dense classes
+    float K, K1;          // their factors
+    float P_total, one_total, soft, hard, scale, y_rest;
+    float to_e[LISTED_WAVES], to_e1[LISTED_WAVES], to_p[LISTED_WAVES];  // from a wave's maxima
+    float loss;
+    bool empty;
 };
 
-template <int TYPE, int NT, bool TWO, int MODE>
-__global__ void __launch_bounds__(NT, MINW)
+template <int TWO>
+__device__ NOIN2 RowTerms row_terms(const Dense &a, const Listed *listed, int waves,
+                                              const ach_distill_desc &t, int k, float temperature,
+                                              bool label, bool extra, float x_y, float w)
+{
+    const bool tail = t.mode == ACH_DISTILL_TAIL;
+    const float inv_t = 1.f / temperature, c = inv_t * LOG2E;
+    RowTerms o;
+    o.m = a.m;
+    float ref = a.m, most_value = -INFINITY;  // the row's maximum
+    for (int i = 0; i < waves; ++i) {
+        if (listed[i].e != 0) ref = fmaxf(ref, listed[i].most);
+        most_value = fmaxf(most_value, listed[i].most_value);
+    }
+    double e = 0, e1 = 0, p = 0, l = 0;
+#pragma unroll
+    for (int i = 0; i < LISTED_WAVES; ++i) {
+        o.to_e[i] = o.to_e1[i] = o.to_p[i] = 0.f;
+        if (i >= waves) continue;
+        const Listed &s = listed[i];
+        o.to_e[i] = exp2_fast((s.most - ref) * c);
+        o.to_e1[i] = TWO ? exp2_fast((s.most - ref) * LOG2E) : o.to_e[i];
+        const float lower = tail || s.most_value == -INFINITY ? 0.f : s.most_value - most_value;
+        o.to_p[i] = exp2_fast(lower * c);
+        if (s.e != 0) {
+            e += s.e * o.to_e[i];
+            e1 += s.e1 * o.to_e1[i];
+        }
+        if (s.p == 0) continue;
+        p += s.p * o.to_p[i];
+        l += o.to_p[i] * (s.l + s.p * ((double)lower - ((double)s.most - ref)) * inv_t);
+    }
+    // without a dense class of finite logit a.s is 0
+    const float up = exp2_fast((a.m - ref) * c), up1 = TWO ? exp2_fast((a.m - ref) * LOG2E) : up;
+    const double total = e + (double)a.s * up, total1 = e1 + (double)a.s1 * up1;
+    o.empty = total == 0;
+    // the largest logit counts exactly 1 in total
+    const float lse = log1pf((float)(total - 1)), lse1 = TWO ? log1pf((float)(total1 - 1)) : lse;
+    double kd = 0, P = 0, rest = 0;
+    // the rest: the classes that the teacher does not list, relative to their maximum
+    const float top_rest = extra ? fmaxf(a.m, x_y) : a.m;
+    const float down = exp2_fast((a.m - top_rest) * c);
+    o.y_rest = extra ? exp2_fast((x_y - top_rest) * c) : 0.f;
+    const float sum_rest = a.s * down + o.y_rest;
+    o.scale = 1.f;
+    if (k > 0 && tail) {
+        P = p;
+        kd = l + lse * p;
+        if (sum_rest != 0.f) {
+            rest = p > 1 ? 0 : 1 - p;
+            if (rest != 0)
+                kd += rest * (logf((float)rest) - (logf(sum_rest) + (top_rest - ref) * inv_t - lse));
+            P += rest;
+        }
+    } else if (k > 0 && p != 0) {
+        o.scale = (float)(1 / p);
+        P = p / p;  // 1, or NaN
+        kd = l / p - logf((float)p) + lse;
+    }
+    const float per_rest = rest == 0 ? 0.f : (float)(rest / sum_rest);
+    o.y_rest *= per_rest;
+    double v = k > 0 ? (double)t.soft * temperature * temperature * kd : 0;
+    if (label) v += (double)t.hard * ((double)lse1 - ((double)x_y - ref));
+    o.loss = o.empty ? 0.f : (float)(w * v);
+    o.soft = k > 0 ? -w * t.soft * temperature : 0.f;
+    o.hard = label ? -w * t.hard : 0.f;
+    o.P_total = o.empty ? 0.f : (float)(P / total);
+    o.one_total = o.empty ? 0.f : (float)(1 / total1);
+    o.K = o.soft == 0.f ? 0.f : o.soft * (o.P_total * up - per_rest * down);
+    o.K1 = o.hard == 0.f ? 0.f : o.hard * o.one_total * up1;
+    if (!TWO) o.K += o.K1;
+    return o;
+}
+
+// What a launch does: all of it, a row to a workgroup; or, for rows in parts,
+// first the statistics of the dense classes, a workgroup each part, and the
+// listed classes, one workgroup more; then the delta.
+enum { WHOLE, STATS, DELTA };
+
+// What the first of two launches leaves for the second.
+struct RowList {
+    Listed listed[LISTED_WAVES];
+    float x_y;
+    int extra;
+    Entry entry[ACH_TOP_MAX + 1];
+};
+struct Between {
+    RowList *list;
+    Dense *dense;
+};
+
+template <int TYPE, int NT, int TWO, int MODE>
+__global__ void __launch_bounds__(NT, 4)
     k_distill(ach_logits_desc d, ach_distill_desc t, const typename Elem<TYPE>::T *logits,
               const int32_t *__restrict__ teacher_ids, const void *__restrict__ teacher_values,
               const int32_t *__restrict__ labels, const float *__restrict__ row_weights,
@@ -1049,14 +1265,15 @@ __global__ void __launch_bounds__(NT, MINW)
     using T = typename Elem<TYPE>::T;
     typedef typename Row<TYPE>::Chunk Chunk;
     constexpr int V = Row<TYPE>::VEC, W = NT / 64;
-    constexpr int E = (ACH_TOP_MAX + NT) / NT;  // listed classes of a thread, i = thread + e NT
+    constexpr int E = (ACH_TOP_MAX + NT) / NT;  // listed classes of a thread
     __shared__ DistillLds<NT> sh;
     const int k = t.soft != 0.f ? t.k : 0;
     const bool tail = t.mode == ACH_DISTILL_TAIL;
-    const float inv_t = 1.f / d.temperature, c = inv_t * LOG2E;
+    const float c = LOG2E / d.temperature;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (size_t b = blockIdx.x; b < (size_t)d.rows * parts; b += gridDim.x) {
-        const int r = (int)(b / parts), part = (int)(b % parts), at = part * span;
+    const int groups = MODE == STATS ? parts + 1 : parts;
+    for (size_t b = blockIdx.x; b < (size_t)d.rows * groups; b += gridDim.x) {
+        const int r = (int)(b / groups), part = (int)(b % groups), at = part * span;
         const T *row = logits + (size_t)r * d.stride;
         const Range<TYPE> g = {row + at, at, min(span, d.classes - at)};
         const float w = row_weights ? row_weights[r] : 1.f;
@@ -1076,42 +1293,57 @@ __global__ void __launch_bounds__(NT, MINW)
         }
         int y = t.hard != 0.f ? labels[r] : -1;
         if (y < 0 || y >= d.classes) y = -1;
-
-        // The listed classes: id -1 where there is none.
-        int id[E];
-        float x[E], value[E];
-        float *kept = MODE == WHOLE ? nullptr : between.x + (size_t)r * (ACH_TOP_MAX + 1);
-        __syncthreads();  // of the last row
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = threadIdx.x + e * NT;
-            id[e] = i < k ? teacher_ids[(size_t)r * k + i] : i == k ? y : -1;
-            if (id[e] < 0 || id[e] >= d.classes) id[e] = -1;
-            value[e] = i < k ? load_any(teacher_values, t.teacher_type, (size_t)r * k + i) : 0.f;
-            x[e] = id[e] < 0 ? -INFINITY : MODE == DELTA ? kept[i] : (float)row[id[e]];
-            if (i < k) {
-                sh.id[i] = id[e];
+        RowList *list = MODE == WHOLE ? nullptr : between.list + r;
+        const int waves = min(W, (k >> 6) + 1);  // that have listed classes
+        Entry entry[E];
+        Dense a = {-FLT_MAX, 0.f, 0.f};
+        if (MODE != DELTA) {
+            __syncthreads();  // of the last row
+            for (int i = threadIdx.x; i <= k; i += NT) {
+                const int id = i < k ? teacher_ids[(size_t)r * k + i] : y;
+                sh.id[i] = id < 0 || id >= d.classes ? -1 : id;
                 sh.repeated[i] = 0;
             }
-            if (MODE == STATS && part == 0 && i <= k) kept[i] = x[e];
+            if (threadIdx.x == 0) sh.x_y = 0.f;
         }
-        if (threadIdx.x == 0) sh.label_listed = 0;
-
-        // The dense classes.
-        Dense a;
-        if (MODE == DELTA) {
-            a = {-FLT_MAX, 0.f, 0.f};
-            if (lane < parts) a = between.dense[(size_t)r * parts + lane];
-            wave_dense<true>(a, c);
+        if (MODE == WHOLE || (MODE == STATS && part == parts)) {
             __syncthreads();
+            int width = 1, shift = 0;
+            while (width <= k) width <<= 1, ++shift;
+            for (int i = threadIdx.x; i < (k + 1) << shift; i += NT) {
+                const int later = i >> shift, former = i & (width - 1);
+                if (former < later && sh.id[former] == sh.id[later]) sh.repeated[later] = 1;
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) sh.extra = y >= 0 && !sh.repeated[k];
+            listed_terms<TYPE, NT, TWO>(entry, row, teacher_values, t.teacher_type, (size_t)r * k, k,
+                                        tail, d.temperature, sh);
+        }
+        if (MODE == STATS && part == parts) {
+            __syncthreads();
+            if ((int)threadIdx.x < waves) list->listed[threadIdx.x] = sh.listed[threadIdx.x];
+            if (threadIdx.x == 0) {
+                list->x_y = sh.x_y;
+                list->extra = sh.extra;
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int i = threadIdx.x + e * NT;
+                if (i <= k) list->entry[i] = entry[e];
+            }
+            continue;
+        }
+        if (MODE == DELTA) {
+            if (lane < parts) a = between.dense[(size_t)r * parts + lane];
+            wave_dense<BOTH>(a, c);
         } else {
-            a = stream_dense<TYPE, NT, TWO>(g, c, k, y, sh);
+            a = stream_dense<TYPE, NT, TWO>(g, c, k, sh);
             wave_dense<TWO>(a, c);
             if (!TWO) a.s1 = a.s;
-        }
-        const auto join = [&] {
+            if (lane == 0) sh.wave[wave] = a;
+            __syncthreads();
             a = sh.wave[0];
-#pragma unroll
+#pragma unroll 1
             for (int i = 1; i < W; ++i) {
                 Dense o = sh.wave[i];
                 const float m = fmaxf(a.m, o.m);
@@ -1120,172 +1352,68 @@ __global__ void __launch_bounds__(NT, MINW)
                 a.s += o.s;
                 a.s1 = TWO ? a.s1 + o.s1 : a.s;
             }
-        };
+        }
         if (MODE == STATS) {
-            if (lane == 0) sh.wave[wave] = a;
-            __syncthreads();
-            join();
-            if (threadIdx.x == 0) between.dense[b] = a;
+            if (threadIdx.x == 0) between.dense[(size_t)r * parts + part] = a;
             continue;
         }
-
-        // Of entries with the same id the first counts.
-        int width = 1, shift = 0;
-        while (width < k) width <<= 1, ++shift;
-        for (int i = threadIdx.x; i < k << shift; i += NT) {
-            const int later = i >> shift, former = i & (width - 1);
-            if (former < later && sh.id[former] == sh.id[later]) sh.repeated[later] = 1;
-        }
-        if (y >= 0)
-            for (int i = threadIdx.x; i < k; i += NT)
-                if (sh.id[i] == y) sh.label_listed = 1;
-        float most = -INFINITY, most_value = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (id[e] >= 0) {
-                most = fmaxf(most, x[e]);
-                if ((int)threadIdx.x + e * NT < k) most_value = fmaxf(most_value, value[e]);
-            }
-        most = wave_most(most);
-        most_value = wave_most(most_value);
-        if (lane == 0) {
-            sh.wave[wave] = a;
-            sh.most[wave] = most;
-            sh.most_value[wave] = most_value;
-        }
-        __syncthreads();
-        if (MODE == WHOLE) join();
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            most = fmaxf(most, sh.most[i]);
-            most_value = fmaxf(most_value, sh.most_value[i]);
-        }
-        const float ref = fmaxf(most, a.m);  // the row's maximum
-        const bool extra = y >= 0 && !sh.label_listed;  // the label as a class of its own
-
-        // The listed classes' exponentials e, e1, probabilities p (RENORM: times
-        // their sum), and four sums: of e, e1, p, and p (log p - (x - ref)/T).
-        float ex[E], ex1[E];
-        double p[E], sum[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = threadIdx.x + e * NT;
-            if (i < k ? sh.repeated[i] : !extra) id[e] = -1;
-            p[e] = 0;
-            ex[e] = ex1[e] = 0.f;
-            if (id[e] < 0) continue;
-            const float z = (x[e] - ref) * inv_t;
-            ex[e] = exp2_fast((x[e] - ref) * c);
-            ex1[e] = TWO ? exp2_fast((x[e] - ref) * LOG2E) : ex[e];
-            sum[0] += ex[e];
-            sum[1] += ex1[e];
-            if (i >= k || value[e] == -INFINITY) continue;
-            const double l = tail ? (double)value[e] : ((double)value[e] - most_value) / d.temperature;
-            p[e] = exp(l);
-            sum[2] += p[e];
-            if (p[e] != 0) sum[3] += p[e] * (l - z);
-        }
-        const int waves = min(W, (k >> 6) + 1);  // that hold listed classes
-        if (wave < waves)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sum[i] = wave_all(sum[i], Add());
-                if (lane == 0) sh.sum[i][wave] = sum[i];
-            }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sum[i] = sh.sum[i][0];
-            for (int j = 1; j < waves; ++j) sum[i] += sh.sum[i][j];
-        }
-
-        // The row's constants, by every thread.  Without a dense class of finite logit s is 0.
-        const float up = exp2_fast((a.m - ref) * c),
-                    up1 = TWO ? exp2_fast((a.m - ref) * LOG2E) : up;
-        const double total = sum[0] + (double)a.s * up, total1 = sum[1] + (double)a.s1 * up1;
-        const bool empty = total == 0;
-        // the largest logit counts exactly 1 in total
-        const float lse = log1pf((float)(total - 1)), lse1 = TWO ? log1pf((float)(total1 - 1)) : lse;
-        const float x_y = y < 0        ? 0.f
-                          : MODE == DELTA ? kept[k]
-                                          : (float)row[y];
-        double kd = 0, scale = 1, P = 0, rest = 0;
-        // the rest: the classes that the teacher does not list, relative to their maximum
-        const float top_rest = extra ? fmaxf(a.m, x_y) : a.m;
-        const float down = exp2_fast((a.m - top_rest) * c);
-        const float y_rest = extra ? exp2_fast((x_y - top_rest) * c) : 0.f;
-        const float sum_rest = a.s * down + y_rest;
-        if (k > 0 && tail) {
-            P = sum[2];
-            kd = sum[3] + lse * P;
-            if (sum_rest != 0.f) {
-                rest = P > 1 ? 0 : 1 - P;
-                if (rest != 0)
-                    kd += rest * (logf((float)rest) - (logf(sum_rest) + (top_rest - ref) * inv_t - lse));
-                P += rest;
-            }
-        } else if (k > 0 && sum[2] != 0) {
-            scale = 1 / sum[2];
-            P = sum[2] * scale;  // 1, or NaN
-            kd = sum[3] * scale - logf((float)sum[2]) + lse;
-        }
-        const float per_rest = rest == 0 ? 0.f : (float)(rest / sum_rest);
+        const RowTerms terms =
+            row_terms<TWO>(a, MODE == DELTA ? list->listed : sh.listed, waves, t, k, d.temperature,
+                           y >= 0, MODE == DELTA ? list->extra : sh.extra,
+                           MODE == DELTA ? list->x_y : sh.x_y, w);
         if (threadIdx.x == 0 && part == 0) {
-            double v = k > 0 ? (double)t.soft * d.temperature * d.temperature * kd : 0;
-            if (y >= 0) v += (double)t.hard * ((double)lse1 - ((double)x_y - ref));
-            const float l = empty ? 0.f : (float)(w * v);
-            if (loss) loss[r] = l;
-            if (row_loss) row_loss[r] = l;
+            if (loss) loss[r] = terms.loss;
+            if (row_loss) row_loss[r] = terms.loss;
         }
         if (!delta) continue;
-        const float soft = k > 0 ? -w * t.soft * d.temperature : 0.f, hard = y >= 0 ? -w * t.hard : 0.f;
-        const float P_total = empty ? 0.f : (float)(P / total),
-                    one_total = empty ? 0.f : (float)(1 / total1);
         T *out = delta + (size_t)r * delta_stride + at;
-        {
-            float K = soft == 0.f ? 0.f : soft * (P_total * up - per_rest * down);
-            const float K1 = hard == 0.f ? 0.f : hard * one_total * up1;
-            if (!TWO) K += K1;
-            const auto grad = [&](float v) {
-                float o = K * exp2_fast((v - a.m) * c);
-                if (TWO) o = fmaf(K1, exp2_fast((v - a.m) * LOG2E), o);
-                return (T)o;
-            };
+        const auto grad = [&](float v) {
+            const float x = v - terms.m, e = exp2_fast(x * c);
+            float o = terms.K * e;
+            if (TWO) o = fmaf(terms.K1, second<TWO>(e, x), o);
+            return (T)o;
+        };
+        const int n = g.chunks();
+        const auto write = [&](auto PAST) {
             // from the end, which the caches hold
-            const int n = g.chunks();
-            const auto write = [&](auto PAST) {
-                constexpr int U = UNROLL;
-                for (int q = n - 1 - (int)threadIdx.x; q >= 0; q -= U * NT) {
-                    Chunk v[U];
+            constexpr int U = UNROLL;
+            for (int q = n - 1 - (int)threadIdx.x; q >= 0; q -= U * NT) {
+                Chunk v[U];
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (q - u * NT >= 0) v[u] = Row<TYPE>::load(g.p + (size_t)(q - u * NT) * V);
+                for (int u = 0; u < U; ++u)
+                    if (q - u * NT >= 0) v[u] = Row<TYPE>::load(g.p + (size_t)(q - u * NT) * V);
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        if (q - u * NT < 0) break;
-                        Chunk o;
+                for (int u = 0; u < U; ++u) {
+                    if (q - u * NT < 0) break;
+                    Chunk o;
 #pragma unroll
-                        for (int i = 0; i < V; ++i) o[i] = grad((float)v[u][i]);
-                        Row<TYPE>::template store<PAST.value>(out + (size_t)(q - u * NT) * V, o);
-                    }
+                    for (int i = 0; i < V; ++i) o[i] = grad((float)v[u][i]);
+                    Row<TYPE>::template store<PAST.value>(out + (size_t)(q - u * NT) * V, o);
                 }
-            };
-            if (past) write(Flag<true>());
-            else write(Flag<false>());
-            if (threadIdx.x < g.rest()) out[n * V + threadIdx.x] = grad((float)g.p[n * V + threadIdx.x]);
-        }
+            }
+        };
+        if (past) write(Flag<true>());
+        else write(Flag<false>());
+        if (threadIdx.x < g.rest()) out[n * V + threadIdx.x] = grad((float)g.p[n * V + threadIdx.x]);
         __syncthreads();  // the listed classes over what was written for them
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            if (id[e] < at || id[e] >= at + g.len) continue;
+            const int i = threadIdx.x + e * NT;
+            if (i > k) continue;
+            if (MODE == DELTA) entry[e] = list->entry[i];
+            const Entry &l = entry[e];
+            if (l.id < at || l.id >= at + g.len) continue;
+            const int of = NT == 64 ? 0 : i >> 6;
+            const float to_e = of == 0 ? terms.to_e[0] : of == 1 ? terms.to_e[1] : terms.to_e[2],
+                        to_e1 = of == 0 ? terms.to_e1[0] : of == 1 ? terms.to_e1[1] : terms.to_e1[2],
+                        to_p = of == 0 ? terms.to_p[0] : of == 1 ? terms.to_p[1] : terms.to_p[2];
             float v = 0.f;
-            if (soft != 0.f) {
-                const float less = (int)threadIdx.x + e * NT < k ? (float)(p[e] * scale)
-                                                                 : per_rest * y_rest;
-                v = soft * (P_total * ex[e] - less);
-            }
-            if (hard != 0.f) v += hard * (one_total * ex1[e] - (id[e] == y ? 1.f : 0.f));
-            out[id[e] - at] = (T)(empty ? 0.f : v);
+            if (terms.soft != 0.f)
+                v = terms.soft * (terms.P_total * l.e * to_e -
+                                  (i < k ? l.p * to_p * terms.scale : terms.y_rest));
+            if (terms.hard != 0.f)
+                v += terms.hard * (terms.one_total * l.e1 * to_e1 - (l.id == y ? 1.f : 0.f));
+            out[l.id - at] = (T)(terms.empty ? 0.f : v);
         }
     }
 }
@@ -1330,12 +1458,12 @@ struct Split {
     int parts, span;
 };
 
-Split split_rows(int rows, int classes)
+Split split_rows(int rows, int classes, int least)
 {
     int parts = rows > 0 ? SPLITN / rows : 1;
     parts = parts < classes / SPLITM ? parts : classes / SPLITM;
     if (parts > MOST_PARTS) parts = MOST_PARTS;
-    if (parts < 2) return {1, classes};
+    if (parts < 2 || classes < least) return {1, classes};
     const int span = (int)((((int64_t)classes + parts - 1) / parts + 63) / 64 * 64);
     return {(int)(((int64_t)classes + span - 1) / span), span};
 }
@@ -1379,7 +1507,7 @@ size_t ach_logprobs_workspace(const ach_logits_desc *desc, int k)
 {
     ach_logits_desc d;
     if (!logits_desc(desc, &d) || k < 0 || k > ACH_TOP_MAX || k > d.classes) return 0;
-    const Split s = split_rows(d.rows, d.classes);
+    const Split s = split_rows(d.rows, d.classes, 65536);
     if (s.parts == 1) return 0;
     return (size_t)d.rows * s.parts * (sizeof(Total) + (size_t)k * sizeof(uint64_t));
 }
@@ -1398,8 +1526,8 @@ int ach_logprobs_fwd(const ach_logits_desc *desc, const void *logits, const int3
     const size_t need = ach_logprobs_workspace(desc, k);
     if (need && (!ws || ws_bytes < need || !aligned(ws, 16))) return ACH_EWORKSPACE;
     if (d.rows == 0) return ACH_OK;
-    const Split sp = split_rows(d.rows, d.classes);
-    const int nt = d.rows * sp.parts <= N1K && sp.span >= 32768 ? 1024 : d.rows * sp.parts < N512 && sp.span >= 32768 ? 512 : sp.span <= T64 && k <= 32 ? 64 : 256;
+    const Split sp = split_rows(d.rows, d.classes, 65536);
+    const int nt = d.rows * sp.parts <= N1K && sp.span >= 32768 ? 1024 : d.rows * sp.parts < N512 && sp.span >= S512 ? 512 : sp.span <= (d.rows >= 1024 ? R64 : T64) && k <= 32 ? 64 : 256;
     const dim3 grid(grid_of((size_t)d.rows * sp.parts));
     Total *part = (Total *)ws;
     uint64_t *lists = (uint64_t *)(part + (size_t)d.rows * sp.parts);
@@ -1470,10 +1598,10 @@ size_t ach_distill_workspace(const ach_logits_desc *desc, const ach_distill_desc
 {
     ach_logits_desc d;
     if (!logits_desc(desc, &d) || !distill_desc(t)) return 0;
-    const Split s = split_rows(d.rows, d.classes);
+    const Split s = split_rows(d.rows, d.classes, 24576);
     size_t n = round16((size_t)d.rows * sizeof(float));
     if (s.parts > 1)
-        n += (size_t)d.rows * (s.parts * sizeof(Dense) + (ACH_TOP_MAX + 1) * sizeof(float));
+        n += (size_t)d.rows * (sizeof(RowList) + s.parts * sizeof(Dense));
     return n;
 }
 
@@ -1499,33 +1627,38 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
     if (d.rows > 0 && (!ws || ws_bytes < need || !aligned(ws, 16))) return ACH_EWORKSPACE;
     hipStream_t st = as_stream(s);
     if (d.rows > 0) {
-        const Split sp = split_rows(d.rows, d.classes);
-        const int nt = sp.span <= T64 ? 64 : (size_t)sp.span * elem_size(d.type) <= D256 ? 256 : 512;
-        const bool two = t.soft != 0.f && t.hard != 0.f && d.temperature != 1.f;
+        const Split sp = split_rows(d.rows, d.classes, 24576);
+        const int two = t.soft == 0.f || t.hard == 0.f || d.temperature == 1.f ? ONE
+                        : d.temperature == 2.f                                 ? SQUARE
+                        : d.temperature == 4.f                                 ? FOURTH
+                                                                               : BOTH;
         if (t.soft == 0.f) d.temperature = 1.f;  // the label's term is at temperature 1
         const dim3 grid(grid_of((size_t)d.rows * sp.parts));
         const bool past = past_caches(d);
         float *row_loss = (float *)ws;
-        Dense *dense = (Dense *)((char *)ws + round16((size_t)d.rows * sizeof(float)));
-        const Between between = {dense, (float *)(dense + (size_t)d.rows * sp.parts)};
-#define GO(TYPE, NT, TWO, MODE)                                                                   \
-    hipLaunchKernelGGL((k_distill<TYPE, NT, TWO, MODE>), grid, dim3(NT), DLDS, st, d, t,            \
+        RowList *list = (RowList *)((char *)ws + round16((size_t)d.rows * sizeof(float)));
+        const Between between = {list, (Dense *)(list + d.rows)};
+        const dim3 stats_grid(grid_of((size_t)d.rows * (sp.parts + 1)));
+#define GO(TYPE, NT, TWO, MODE, GRID)                                                       \
+    hipLaunchKernelGGL((k_distill<TYPE, NT, TWO, MODE>), GRID, dim3(NT), 0, st, d, t,       \
                        (const Elem<TYPE>::T *)logits, teacher_ids, teacher_values, labels,        \
                        row_weights, loss, (Elem<TYPE>::T *)delta, delta_stride, row_loss,         \
                        sp.parts, sp.span, between, past)
 #define WITH(TYPE, TWO)                                                                           \
     do {                                                                                          \
         if (sp.parts > 1) {                                                                       \
-            GO(TYPE, 256, TWO, STATS);                                                            \
-            GO(TYPE, 256, TWO, DELTA);                                                            \
-        } else if (nt == 64) GO(TYPE, 64, TWO, WHOLE);                                            \
-        else if (nt == 256) GO(TYPE, 256, TWO, WHOLE);                                            \
-        else GO(TYPE, 512, TWO, WHOLE);                                                           \
+            GO(TYPE, 256, TWO, STATS, stats_grid);                                                \
+            GO(TYPE, 256, TWO, DELTA, grid);                                                      \
+        } else if (d.classes <= 2048) GO(TYPE, 64, TWO, WHOLE, grid);                             \
+        else if (d.rows < 256 && d.classes >= 8192) GO(TYPE, 512, TWO, WHOLE, grid);           \
+        else GO(TYPE, 256, TWO, WHOLE, grid);                                                     \
     } while (0)
 #define CALL(TYPE)                                                                                \
     do {                                                                                          \
-        if (two) WITH(TYPE, true);                                                                \
-        else WITH(TYPE, false);                                                                   \
+        if (two == ONE) WITH(TYPE, ONE);                                                          \
+        else if (two == SQUARE) WITH(TYPE, SQUARE);                                               \
+        else if (two == FOURTH) WITH(TYPE, FOURTH);                                               \
+        else WITH(TYPE, BOTH);                                                                    \
     } while (0)
         FOR_TYPE(d.type, CALL);
 #undef CALL
