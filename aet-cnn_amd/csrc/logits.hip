@@ -1254,13 +1254,48 @@ struct Between {
     Dense *dense;
 };
 
+// The losses of rows in parts, and their sum: a workgroup of its own in the
+// second launch, a row to a thread.
+template <int TWO, int NT>
+__device__ __forceinline__ void part_losses(const ach_logits_desc &d, const ach_distill_desc &t,
+                                            const int32_t *labels, const float *row_weights,
+                                            float *loss, float *cost, int parts,
+                                            const Between &between)
+{
+    __shared__ double sums[NT / 64];
+    const int k = t.soft != 0.f ? t.k : 0, r = threadIdx.x;
+    const float c = LOG2E / d.temperature, w = r < d.rows ? row_weights ? row_weights[r] : 1.f : 0.f;
+    float v = 0.f;
+    if (w != 0.f) {
+        Dense a = {-FLT_MAX, 0.f, 0.f};
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) {
+            Dense o = between.dense[(size_t)r * parts + i];
+            const float m = fmaxf(a.m, o.m);
+            raise_dense<BOTH>(a, m, c);
+            raise_dense<BOTH>(o, m, c);
+            a.s += o.s;
+            a.s1 += o.s1;
+        }
+        const int y = t.hard != 0.f ? labels[r] : -1;
+        const RowList &list = between.list[r];
+        v = row_terms<TWO>(a, list.listed, min(NT / 64, (k >> 6) + 1), t, k, d.temperature,
+                           y >= 0 && y < d.classes, list.extra, list.x_y, w)
+                .loss;
+    }
+    if (loss && r < d.rows) loss[r] = v;
+    if (!cost) return;
+    const double sum = block_sum<NT>((double)v, sums);
+    if (r == 0) *cost = (float)sum;
+}
+
 template <int TYPE, int NT, int TWO, int MODE>
 __global__ void __launch_bounds__(NT, 4)
     k_distill(ach_logits_desc d, ach_distill_desc t, const typename Elem<TYPE>::T *logits,
               const int32_t *__restrict__ teacher_ids, const void *__restrict__ teacher_values,
               const int32_t *__restrict__ labels, const float *__restrict__ row_weights,
               float *loss, typename Elem<TYPE>::T *delta, int64_t delta_stride, float *row_loss,
-              int parts, int span, Between between, bool past)
+              int parts, int span, Between between, bool past, float *cost)
 {
     using T = typename Elem<TYPE>::T;
     typedef typename Row<TYPE>::Chunk Chunk;
@@ -1272,6 +1307,10 @@ __global__ void __launch_bounds__(NT, 4)
     const float c = LOG2E / d.temperature;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int groups = MODE == STATS ? parts + 1 : parts;
+    if (MODE == DELTA && blockIdx.x == (unsigned)(d.rows * parts)) {
+        part_losses<TWO, NT>(d, t, labels, row_weights, loss, cost, parts, between);
+        return;
+    }
     for (size_t b = blockIdx.x; b < (size_t)d.rows * groups; b += gridDim.x) {
         const int r = (int)(b / groups), part = (int)(b % groups), at = part * span;
         const T *row = logits + (size_t)r * d.stride;
@@ -1285,7 +1324,7 @@ __global__ void __launch_bounds__(NT, 4)
                     Row<TYPE>::template store<false>(out + (size_t)q * V, zero);
                 if (threadIdx.x < g.rest()) out[g.chunks() * V + threadIdx.x] = (T)0.f;
             }
-            if (MODE != STATS && threadIdx.x == 0 && part == 0) {
+            if (MODE == WHOLE && threadIdx.x == 0) {
                 if (loss) loss[r] = 0.f;
                 if (row_loss) row_loss[r] = 0.f;
             }
@@ -1361,7 +1400,7 @@ __global__ void __launch_bounds__(NT, 4)
             row_terms<TWO>(a, MODE == DELTA ? list->listed : sh.listed, waves, t, k, d.temperature,
                            y >= 0, MODE == DELTA ? list->extra : sh.extra,
                            MODE == DELTA ? list->x_y : sh.x_y, w);
-        if (threadIdx.x == 0 && part == 0) {
+        if (MODE == WHOLE && threadIdx.x == 0) {
             if (loss) loss[r] = terms.loss;
             if (row_loss) row_loss[r] = terms.loss;
         }
@@ -1453,7 +1492,7 @@ bool distill_desc(const ach_distill_desc *t)
 }
 
 // Workgroups per row and the classes of each: one, unless the rows are few
-// and long.
+// (at most 256) and long.
 struct Split {
     int parts, span;
 };
@@ -1638,17 +1677,18 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
         float *row_loss = (float *)ws;
         RowList *list = (RowList *)((char *)ws + round16((size_t)d.rows * sizeof(float)));
         const Between between = {list, (Dense *)(list + d.rows)};
-        const dim3 stats_grid(grid_of((size_t)d.rows * (sp.parts + 1)));
+        // few rows (split_rows): a workgroup each, and one for the losses
+        const dim3 stats_grid(d.rows * (sp.parts + 1)), delta_grid(d.rows * sp.parts + 1);
 #define GO(TYPE, NT, TWO, MODE, GRID)                                                       \
     hipLaunchKernelGGL((k_distill<TYPE, NT, TWO, MODE>), GRID, dim3(NT), 0, st, d, t,       \
                        (const Elem<TYPE>::T *)logits, teacher_ids, teacher_values, labels,        \
                        row_weights, loss, (Elem<TYPE>::T *)delta, delta_stride, row_loss,         \
-                       sp.parts, sp.span, between, past)
+                       sp.parts, sp.span, between, past, cost)
 #define WITH(TYPE, TWO)                                                                           \
     do {                                                                                          \
         if (sp.parts > 1) {                                                                       \
             GO(TYPE, 256, TWO, STATS, stats_grid);                                                \
-            GO(TYPE, 256, TWO, DELTA, grid);                                                      \
+            GO(TYPE, 256, TWO, DELTA, delta_grid);                                                \
         } else if (d.classes <= 2048) GO(TYPE, 64, TWO, WHOLE, grid);                             \
         else if (d.rows < 256 && d.classes >= 8192) GO(TYPE, 512, TWO, WHOLE, grid);           \
         else GO(TYPE, 256, TWO, WHOLE, grid);                                                     \
@@ -1665,7 +1705,7 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
 #undef WITH
 #undef GO
         const int rc = check_launch();
-        if (rc || !cost) return rc;
+        if (rc || !cost || sp.parts > 1) return rc;
     }
     if (!cost) return ACH_OK;
     hipLaunchKernelGGL(k_sum_losses, dim3(1), dim3(256), 0, st, (const float *)ws, d.rows, cost);
