@@ -1093,58 +1093,43 @@ __device__ __forceinline__ float load_any(const void *p, int type, size_t i)
                               : (float)((const _Float16 *)p)[i];
 }
 
-// The listed classes of a row.  Class i of the list belongs to thread i, or
-// i mod NT; `entry` are the thread's, the waves' sums are left in sh.listed.
-// sh.id has been filled in, and a barrier has been since.
-template <int TYPE, int NT, int TWO, int E>
-__device__ NOIN void listed_terms(Entry (&entry)[E], const typename Elem<TYPE>::T *row,
+// The listed classes of a row, k + 1 <= NT.  Class i of the list is thread i's
+// `entry`; the waves' sums are left in sh.listed.  sh.id and sh.repeated have
+// been filled in, and a barrier has been since.
+template <int TYPE, int NT, int TWO>
+__device__ __forceinline__ void listed_terms(Entry &entry, const typename Elem<TYPE>::T *row,
                                              const void *values, int type, size_t at, int k,
                                              bool tail, float temperature, DistillLds<NT> &sh)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = threadIdx.x;
     const float inv_t = 1.f / temperature, c = inv_t * LOG2E;
-    if (wave >= min(NT / 64, (k >> 6) + 1)) {  // of the waves, those that have some
-#pragma unroll
-        for (int e = 0; e < E; ++e) entry[e].id = -1;
-        return;
-    }
+    entry = {-1, 0.f, 0.f, 0.f};
+    if (wave > k >> 6) return;  // no class of this wave is listed
     Listed sum = {-INFINITY, -INFINITY, 0, 0, 0, 0};
-    float x[E], value[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int i = threadIdx.x + e * NT;
-        entry[e].id = i <= k ? sh.id[i] : -1;
-        x[e] = value[e] = -INFINITY;
-        if (entry[e].id < 0) continue;
+    float x = -INFINITY, value = -INFINITY;
+    const int id = i <= k ? sh.id[i] : -1;
+    if (id >= 0) {
+        x = (float)row[id];
+        if (i < k) value = load_any(values, type, at + i);
+        else sh.x_y = x;
         // of entries with the same id the first counts; the label, at [k], is last
-        if (sh.repeated[i]) {
-            if (i == k) sh.x_y = (float)row[entry[e].id];
-            entry[e].id = -1;
-            continue;
-        }
-        x[e] = (float)row[entry[e].id];
-        if (i < k) value[e] = load_any(values, type, at + i);
-        else sh.x_y = x[e];
-        sum.most = fmaxf(sum.most, x[e]);
-        sum.most_value = fmaxf(sum.most_value, value[e]);
+        if (!sh.repeated[i]) entry.id = id;
+        else x = value = -INFINITY;
     }
-    sum.most = wave_most(sum.most);
-    sum.most_value = wave_most(sum.most_value);
+    sum.most = wave_most(x);
+    sum.most_value = wave_most(value);
     if (sum.most == -INFINITY) sum.most = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        entry[e].e = entry[e].e1 = entry[e].p = 0.f;
-        if (entry[e].id < 0) continue;
-        entry[e].e = exp2_fast((x[e] - sum.most) * c);
-        entry[e].e1 = TWO ? exp2_fast((x[e] - sum.most) * LOG2E) : entry[e].e;
-        sum.e += entry[e].e;
-        sum.e1 += entry[e].e1;
-        if (value[e] == -INFINITY) continue;
-        const double l = tail ? (double)value[e] : ((double)value[e] - sum.most_value) / temperature;
-        const double p = exp(l);
-        entry[e].p = (float)p;
-        sum.p += p;
-        if (p != 0) sum.l += p * (l - (x[e] - sum.most) * inv_t);
+    if (entry.id >= 0) {
+        entry.e = exp2_fast((x - sum.most) * c);
+        entry.e1 = TWO ? exp2_fast((x - sum.most) * LOG2E) : entry.e;
+        sum.e = entry.e;
+        sum.e1 = entry.e1;
+        if (value != -INFINITY) {
+            const double l = tail ? (double)value : ((double)value - sum.most_value) / temperature;
+            sum.p = exp(l);
+            entry.p = (float)sum.p;
+            if (sum.p != 0) sum.l = sum.p * (l - (x - sum.most) * inv_t);
+        }
     }
     sum.e = wave_all(sum.e, Add());
     sum.e1 = wave_all(sum.e1, Add());
@@ -1300,7 +1285,6 @@ __global__ void __launch_bounds__(NT, 4)
     using T = typename Elem<TYPE>::T;
     typedef typename Row<TYPE>::Chunk Chunk;
     constexpr int V = Row<TYPE>::VEC, W = NT / 64;
-    constexpr int E = (ACH_TOP_MAX + NT) / NT;  // listed classes of a thread
     __shared__ DistillLds<NT> sh;
     const int k = t.soft != 0.f ? t.k : 0;
     const bool tail = t.mode == ACH_DISTILL_TAIL;
@@ -1334,7 +1318,7 @@ __global__ void __launch_bounds__(NT, 4)
         if (y < 0 || y >= d.classes) y = -1;
         RowList *list = MODE == WHOLE ? nullptr : between.list + r;
         const int waves = min(W, (k >> 6) + 1);  // that have listed classes
-        Entry entry[E];
+        Entry entry;
         Dense a = {-FLT_MAX, 0.f, 0.f};
         if (MODE != DELTA) {
             __syncthreads();  // of the last row
@@ -1365,11 +1349,7 @@ __global__ void __launch_bounds__(NT, 4)
                 list->x_y = sh.x_y;
                 list->extra = sh.extra;
             }
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int i = threadIdx.x + e * NT;
-                if (i <= k) list->entry[i] = entry[e];
-            }
+            if ((int)threadIdx.x <= k) list->entry[threadIdx.x] = entry;
             continue;
         }
         if (MODE == DELTA) {
@@ -1435,24 +1415,19 @@ __global__ void __launch_bounds__(NT, 4)
         else write(Flag<false>());
         if (threadIdx.x < g.rest()) out[n * V + threadIdx.x] = grad((float)g.p[n * V + threadIdx.x]);
         __syncthreads();  // the listed classes over what was written for them
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = threadIdx.x + e * NT;
-            if (i > k) continue;
-            if (MODE == DELTA) entry[e] = list->entry[i];
-            const Entry &l = entry[e];
-            if (l.id < at || l.id >= at + g.len) continue;
-            const int of = NT == 64 ? 0 : i >> 6;
+        const int i = threadIdx.x, of = i >> 6;
+        if (MODE == DELTA && i <= k) entry = list->entry[i];
+        if (i <= k && entry.id >= at && entry.id < at + g.len) {
             const float to_e = of == 0 ? terms.to_e[0] : of == 1 ? terms.to_e[1] : terms.to_e[2],
                         to_e1 = of == 0 ? terms.to_e1[0] : of == 1 ? terms.to_e1[1] : terms.to_e1[2],
                         to_p = of == 0 ? terms.to_p[0] : of == 1 ? terms.to_p[1] : terms.to_p[2];
             float v = 0.f;
             if (terms.soft != 0.f)
-                v = terms.soft * (terms.P_total * l.e * to_e -
-                                  (i < k ? l.p * to_p * terms.scale : terms.y_rest));
+                v = terms.soft * (terms.P_total * entry.e * to_e -
+                                  (i < k ? entry.p * to_p * terms.scale : terms.y_rest));
             if (terms.hard != 0.f)
-                v += terms.hard * (terms.one_total * l.e1 * to_e1 - (l.id == y ? 1.f : 0.f));
-            out[l.id - at] = (T)(terms.empty ? 0.f : v);
+                v += terms.hard * (terms.one_total * entry.e1 * to_e1 - (entry.id == y ? 1.f : 0.f));
+            out[entry.id - at] = (T)(terms.empty ? 0.f : v);
         }
     }
 }
@@ -1637,7 +1612,7 @@ size_t ach_distill_workspace(const ach_logits_desc *desc, const ach_distill_desc
 {
     ach_logits_desc d;
     if (!logits_desc(desc, &d) || !distill_desc(t)) return 0;
-    const Split s = split_rows(d.rows, d.classes, 24576);
+    const Split s = split_rows(d.rows, d.classes, 16384);
     size_t n = round16((size_t)d.rows * sizeof(float));
     if (s.parts > 1)
         n += (size_t)d.rows * (sizeof(RowList) + s.parts * sizeof(Dense));
@@ -1666,13 +1641,14 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
     if (d.rows > 0 && (!ws || ws_bytes < need || !aligned(ws, 16))) return ACH_EWORKSPACE;
     hipStream_t st = as_stream(s);
     if (d.rows > 0) {
-        const Split sp = split_rows(d.rows, d.classes, 24576);
+        const Split sp = split_rows(d.rows, d.classes, 16384);
         const int two = t.soft == 0.f || t.hard == 0.f || d.temperature == 1.f ? ONE
                         : d.temperature == 2.f                                 ? SQUARE
                         : d.temperature == 4.f                                 ? FOURTH
                                                                                : BOTH;
         if (t.soft == 0.f) d.temperature = 1.f;  // the label's term is at temperature 1
         const dim3 grid(grid_of((size_t)d.rows * sp.parts));
+        const int k = t.soft != 0.f ? t.k : 0;
         const bool past = past_caches(d);
         float *row_loss = (float *)ws;
         RowList *list = (RowList *)((char *)ws + round16((size_t)d.rows * sizeof(float)));
@@ -1689,7 +1665,7 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
         if (sp.parts > 1) {                                                                       \
             GO(TYPE, 256, TWO, STATS, stats_grid);                                                \
             GO(TYPE, 256, TWO, DELTA, delta_grid);                                                \
-        } else if (d.classes <= 2048) GO(TYPE, 64, TWO, WHOLE, grid);                             \
+        } else if (d.classes <= 2048 && k < 64) GO(TYPE, 64, TWO, WHOLE, grid);                   \
         else if (d.rows < 256 && d.classes >= 8192) GO(TYPE, 512, TWO, WHOLE, grid);           \
         else GO(TYPE, 256, TWO, WHOLE, grid);                                                     \
     } while (0)
