@@ -16,51 +16,6 @@
 namespace ach {
 namespace {
 
-#ifndef MINW
-#define MINW 4
-#endif
-#ifndef MINF
-#define MINF 1
-#endif
-#ifndef SPLITN
-#define SPLITN 512
-#endif
-#ifndef SPLITM
-#define SPLITM 4096
-#endif
-#ifndef N512
-#define N512 1024
-#endif
-#ifndef N1K
-#define N1K 0
-#endif
-#ifndef R64
-#define R64 8192
-#endif
-#ifndef S512
-#define S512 16384
-#endif
-#ifndef N512D
-#define N512D 0
-#endif
-#ifndef NOIN
-#define NOIN __forceinline__
-#endif
-#ifndef NOIN2
-#define NOIN2 __forceinline__
-#endif
-#ifndef DLDS
-#define DLDS 0
-#endif
-#ifndef T64
-#define T64 2048
-#endif
-#ifndef T256
-#define T256 16384
-#endif
-#ifndef D256
-#define D256 131072
-#endif
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 // An element type: 16 bytes of it as one load from any element's address.
@@ -679,7 +634,7 @@ template <class X, class Y> struct Pick<false, X, Y> {
 };
 
 template <int TYPE, int NT, bool FULL, bool TOP>
-__global__ void __launch_bounds__(NT, MINF)
+__global__ void __launch_bounds__(NT)
     k_logprobs(ach_logits_desc d, const typename Elem<TYPE>::T *__restrict__ logits,
                const int32_t *__restrict__ ids, int k, LogprobsOut o, int parts, int span,
                Total *__restrict__ part, uint64_t *__restrict__ lists)
@@ -1149,7 +1104,7 @@ struct RowTerms {
 };
 
 template <int TWO>
-__device__ NOIN2 RowTerms row_terms(const Dense &a, const Listed *listed, int waves,
+__device__ __forceinline__ RowTerms row_terms(const Dense &a, const Listed *listed, int waves,
                                               const ach_distill_desc &t, int k, float temperature,
                                               bool label, bool extra, float x_y, float w)
 {
@@ -1474,20 +1429,39 @@ struct Split {
 
 Split split_rows(int rows, int classes, int least)
 {
-    int parts = rows > 0 ? SPLITN / rows : 1;
-    parts = parts < classes / SPLITM ? parts : classes / SPLITM;
+    int parts = rows > 0 ? 512 / rows : 1;  // two workgroups a compute unit
+    parts = parts < classes / 4096 ? parts : classes / 4096;
     if (parts > MOST_PARTS) parts = MOST_PARTS;
     if (parts < 2 || classes < least) return {1, classes};
     const int span = (int)((((int64_t)classes + parts - 1) / parts + 63) / 64 * 64);
     return {(int)(((int64_t)classes + span - 1) / span), span};
 }
 
-// Threads of a workgroup for `span` classes; with k alternatives at least 2 k
-// (the bound on the k-th largest is taken from the threads' maxima).
-int threads_for(int span, int k)
+// The second launch is worth its time from about 64 K classes in the forward
+// pass (1 row, bf16, 20 alternatives: 32768 classes 9.3 us in one launch, 11.5
+// in two; 100003 classes, 64 rows: 21 and 15.6), and from 16 K in distillation,
+// whose two passes over a row are both shared out (16 rows of 32768: 16.0 and
+// 11.7 us).
+constexpr int SPLIT_LOGPROBS = 65536, SPLIT_DISTILL = 16384;
+
+// Threads of a workgroup of the forward pass.  A wave by itself needs no
+// barriers, which pays for short rows, or up to 8192 classes where there are
+// enough rows to fill the chip with single waves (2048 x 8192 bf16: 15.3 us, 21.8 with
+// 256 threads); the bound on the k-th largest wants k of its lanes.  Few long
+// rows take 512 (512 x 65536 fp32: 33 us, 40 with 256); more rows 256 (4096 x
+// 32768 bf16: 55 us, 120 with 1024).
+int threads_logprobs(int rows, const Split &s, int k)
 {
-    if (span <= T64 && k <= 32) return 64;
-    return span <= T256 ? 256 : 1024;
+    if (s.span <= (rows >= 1024 ? 8192 : 2048) && k <= 32) return 64;
+    return (int64_t)rows * s.parts < 1024 && s.span >= 16384 ? 512 : 256;
+}
+
+// The same of distillation; the listed classes have a thread each.
+int threads_distill(int rows, const Split &s, int k)
+{
+    if (s.parts > 1) return 256;
+    if (s.span <= 2048 && k < 64) return 64;
+    return rows < 256 && s.span >= 8192 ? 512 : 256;
 }
 
 // Gradients of more than the L2 caches hold (8 of 4 MB) are stored past them:
@@ -1521,7 +1495,7 @@ size_t ach_logprobs_workspace(const ach_logits_desc *desc, int k)
 {
     ach_logits_desc d;
     if (!logits_desc(desc, &d) || k < 0 || k > ACH_TOP_MAX || k > d.classes) return 0;
-    const Split s = split_rows(d.rows, d.classes, 65536);
+    const Split s = split_rows(d.rows, d.classes, SPLIT_LOGPROBS);
     if (s.parts == 1) return 0;
     return (size_t)d.rows * s.parts * (sizeof(Total) + (size_t)k * sizeof(uint64_t));
 }
@@ -1540,8 +1514,8 @@ int ach_logprobs_fwd(const ach_logits_desc *desc, const void *logits, const int3
     const size_t need = ach_logprobs_workspace(desc, k);
     if (need && (!ws || ws_bytes < need || !aligned(ws, 16))) return ACH_EWORKSPACE;
     if (d.rows == 0) return ACH_OK;
-    const Split sp = split_rows(d.rows, d.classes, 65536);
-    const int nt = d.rows * sp.parts <= N1K && sp.span >= 32768 ? 1024 : d.rows * sp.parts < N512 && sp.span >= S512 ? 512 : sp.span <= (d.rows >= 1024 ? R64 : T64) && k <= 32 ? 64 : 256;
+    const Split sp = split_rows(d.rows, d.classes, SPLIT_LOGPROBS);
+    const int nt = threads_logprobs(d.rows, sp, k);
     const dim3 grid(grid_of((size_t)d.rows * sp.parts));
     Total *part = (Total *)ws;
     uint64_t *lists = (uint64_t *)(part + (size_t)d.rows * sp.parts);
@@ -1554,7 +1528,6 @@ int ach_logprobs_fwd(const ach_logits_desc *desc, const void *logits, const int3
     do {                                                                                          \
         if (nt == 64) GO(TYPE, 64, FULL, TOP);                                                    \
         else if (nt == 512) GO(TYPE, 512, FULL, TOP);                                             \
-        else if (nt == 1024) GO(TYPE, 1024, FULL, TOP);                                           \
         else GO(TYPE, 256, FULL, TOP);                                                            \
     } while (0)
 #define CALL(TYPE)                                                                                \
@@ -1612,7 +1585,7 @@ size_t ach_distill_workspace(const ach_logits_desc *desc, const ach_distill_desc
 {
     ach_logits_desc d;
     if (!logits_desc(desc, &d) || !distill_desc(t)) return 0;
-    const Split s = split_rows(d.rows, d.classes, 16384);
+    const Split s = split_rows(d.rows, d.classes, SPLIT_DISTILL);
     size_t n = round16((size_t)d.rows * sizeof(float));
     if (s.parts > 1)
         n += (size_t)d.rows * (sizeof(RowList) + s.parts * sizeof(Dense));
@@ -1641,14 +1614,14 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
     if (d.rows > 0 && (!ws || ws_bytes < need || !aligned(ws, 16))) return ACH_EWORKSPACE;
     hipStream_t st = as_stream(s);
     if (d.rows > 0) {
-        const Split sp = split_rows(d.rows, d.classes, 16384);
+        const Split sp = split_rows(d.rows, d.classes, SPLIT_DISTILL);
         const int two = t.soft == 0.f || t.hard == 0.f || d.temperature == 1.f ? ONE
                         : d.temperature == 2.f                                 ? SQUARE
                         : d.temperature == 4.f                                 ? FOURTH
                                                                                : BOTH;
         if (t.soft == 0.f) d.temperature = 1.f;  // the label's term is at temperature 1
         const dim3 grid(grid_of((size_t)d.rows * sp.parts));
-        const int k = t.soft != 0.f ? t.k : 0;
+        const int nt = threads_distill(d.rows, sp, t.soft != 0.f ? t.k : 0);
         const bool past = past_caches(d);
         float *row_loss = (float *)ws;
         RowList *list = (RowList *)((char *)ws + round16((size_t)d.rows * sizeof(float)));
@@ -1665,8 +1638,8 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
         if (sp.parts > 1) {                                                                       \
             GO(TYPE, 256, TWO, STATS, stats_grid);                                                \
             GO(TYPE, 256, TWO, DELTA, delta_grid);                                                \
-        } else if (d.classes <= 2048 && k < 64) GO(TYPE, 64, TWO, WHOLE, grid);                   \
-        else if (d.rows < 256 && d.classes >= 8192) GO(TYPE, 512, TWO, WHOLE, grid);           \
+        } else if (nt == 64) GO(TYPE, 64, TWO, WHOLE, grid);                                      \
+        else if (nt == 512) GO(TYPE, 512, TWO, WHOLE, grid);                                      \
         else GO(TYPE, 256, TWO, WHOLE, grid);                                                     \
     } while (0)
 #define CALL(TYPE)                                                                                \
