@@ -228,6 +228,10 @@ _NET = {
     "an_train": (_i, [_vp, _vp, _vp, C.POINTER(_f)]),
     "an_forward": (_i, [_vp, _i]),
     "an_predict": (_i, [_vp, _vp, _vp]),
+    "an_predict_top": (_i, [_vp, _vp, _i, _f, _vp, _vp, _vp]),
+    "an_set_distillation": (_i, [_vp, _i, _i, _f, _f, _f]),
+    "an_end_distillation": (_i, [_vp]),
+    "an_set_teacher": (_i, [_vp, _vp, _vp, _vp]),
     "an_fuse_conv_batchnorm": (_i, [_vp]),
     "an_feeder_create_cifar": (_vp, [_vp, _vp, _i, _i, _u64, C.POINTER(Augment), _f]),
     "an_feeder_create_synthetic": (_vp, [_vp, _i, _u64, C.POINTER(Augment)]),
@@ -488,6 +492,11 @@ class Network:
     def stream(self):
         return self.lib.an_stream(self.h)
 
+    def input_size(self):
+        """values of one input image"""
+        s = self.shape(0)
+        return s[4] * s[5] * s[6]
+
     def n_layers(self):
         return self.lib.an_n_layers(self.h)
 
@@ -519,6 +528,40 @@ class Network:
         out = np.empty((self.batch, self.lib.an_classes(self.h)), np.float32)
         check(self.lib.an_predict(self.h, x.ctypes.data, out.ctypes.data), "an_predict")
         return out
+
+    def predict_top(self, x: np.ndarray, k: int, temperature: float = 1.0):
+        """an_predict_top: (ids [batch][k], log probabilities [batch][k],
+        entropies [batch])"""
+        x = np.ascontiguousarray(x, dtype=np.float32)
+        if x.size != self.batch * self.input_size():
+            raise ValueError(f"predict_top: {x.size} values for a batch of {self.batch}")
+        ids, lp = np.empty((self.batch, k), np.int32), np.empty((self.batch, k), np.float32)
+        ent = np.empty(self.batch, np.float32)
+        check(self.lib.an_predict_top(self.h, x.ctypes.data, k, temperature, ids.ctypes.data,
+                                      lp.ctypes.data, ent.ctypes.data), "an_predict_top")
+        return ids, lp, ent
+
+    def set_distillation(self, k: int, mode: int = DISTILL_TAIL, temperature: float = 1.0,
+                         soft: float = 1.0, hard: float = 0.0):
+        """an_set_distillation: train against a teacher's k best classes"""
+        check(self.lib.an_set_distillation(self.h, k, mode, temperature, soft, hard),
+              "an_set_distillation")
+        self._teacher_k = k
+
+    def end_distillation(self):
+        check(self.lib.an_end_distillation(self.h), "an_end_distillation")
+
+    def set_teacher(self, ids: np.ndarray, values: np.ndarray, labels=None):
+        """an_set_teacher: ids and values [batch][k], labels [batch] or None"""
+        shape = (self.batch, getattr(self, "_teacher_k", 0))
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
+        values = np.ascontiguousarray(values, dtype=np.float32)
+        lab = None if labels is None else np.ascontiguousarray(labels, dtype=np.int32)
+        if ids.shape != shape or values.shape != shape or (lab is not None and
+                                                           lab.shape != shape[:1]):
+            raise ValueError(f"set_teacher: ids and values of shape {shape} expected")
+        check(self.lib.an_set_teacher(self.h, ids.ctypes.data, values.ctypes.data,
+                                      None if lab is None else lab.ctypes.data), "an_set_teacher")
 
     def validate(self, list_file: str, labels, topk: int = 1) -> Validation:
         """an_validate_paths (Classifier.validateSingle): top-1 / top-k

@@ -89,6 +89,21 @@ struct an_network {
     ach_nan_span *d_nan_spans;
     int n_nan_spans;
     int32_t *d_nan_flag;
+    /* an_predict_top's outputs on the device (its own allocation, made by
+     * the first call): [batch][ACH_TOP_MAX] ids and log probabilities,
+     * [batch] entropies, the workspace                                     */
+    void *top_mem;
+    /* an_set_distillation: the teacher's entries [batch][k], the labels
+     * [batch] and the workspace, one allocation; teacher_ready once
+     * an_set_teacher has filled them (labelled: with labels)               */
+    int distilling, teacher_ready, labelled;
+    ach_logits_desc distill_logits;
+    ach_distill_desc distill;
+    void *teacher_mem;
+    int32_t *teacher_ids, *teacher_labels;
+    float *teacher_values;
+    void *distill_ws;
+    size_t distill_ws_bytes;
 };
 
 /* ---- randUniform over glibc rand() (DnnUtils.c:196-209) ------------------- */
@@ -579,6 +594,16 @@ int an_add_dropout(an_network *net, float probability)
 /* Softmax + cross-entropy: SoftMaxLayer.c:99-119, :291-316.                */
 static int softmax_forward(an_network *net, an_layer *l, an_state st)
 {
+    if (net->distilling && st.train && l->index == net->n - 1) {
+        /* the output as ever; the loss and the delta against the teacher   */
+        if (!net->teacher_ready || (net->distill.hard != 0.f && !net->labelled))
+            return ACH_EINVAL;
+        AN_CHECK(ach_softmax_xent(st.input, l->batch, l->inputs, l->groups, l->temperature, NULL,
+                                  l->output, NULL, NULL, NULL, NULL, 0, net->stream));
+        return ach_distill_xent(&net->distill_logits, &net->distill, st.input, net->teacher_ids,
+                                net->teacher_values, net->teacher_labels, NULL, l->loss, l->delta,
+                                0, l->cost, net->distill_ws, net->distill_ws_bytes, net->stream);
+    }
     return ach_softmax_xent(st.input, l->batch, l->inputs, l->groups, l->temperature,
                             st.truth, l->output, l->delta, l->loss, l->cost, st.workspace,
                             st.workspace_bytes, net->stream);
@@ -1032,6 +1057,8 @@ void an_free(an_network *net)
         free(net->ev_dgrad);
     }
     if (net->ev_joined) ach_event_destroy(net->ev_joined);
+    ach_free(net->top_mem);
+    ach_free(net->teacher_mem);
     ach_free(net->d_nan_spans);
     ach_free(net->arena);
     if (net->wstream) ach_stream_destroy(net->wstream);
@@ -1250,6 +1277,96 @@ void an_top_k(const float *a, int n, int k, int *index)
             }
         }
     }
+}
+
+/* the last layer if it is a softmax over all its inputs, whose input is the
+ * network's logits                                                         */
+static const an_layer *logits_layer(const an_network *net)
+{
+    if (!net || !net->finalized || net->n < 2) return NULL;
+    const an_layer *l = net->layers[net->n - 1];
+    return l->type == AN_SOFTMAX && l->groups == 1 ? l : NULL;
+}
+
+int an_predict_top(an_network *net, const float *host_input, int k, float temperature, int *ids,
+                   float *logprobs, float *entropy)
+{
+    const an_layer *l = logits_layer(net);
+    if (!l || !host_input || !ids || !logprobs || k <= 0 || k > ACH_TOP_MAX || k > l->inputs)
+        return ACH_EINVAL;
+    if (!(temperature >= 1e-6f && temperature <= 1e6f)) return ACH_EINVAL;
+    const size_t B = (size_t)l->batch;
+    ach_logits_desc d = {l->batch, l->inputs, ACH_F32, temperature, 0};
+    ach_logits_desc any = d;
+    any.temperature = 1.f;
+    const int most = l->inputs < ACH_TOP_MAX ? l->inputs : ACH_TOP_MAX;
+    const size_t ws = ach_logprobs_workspace(&any, most);
+    const size_t list = al(B * most * sizeof(int32_t)), row = al(B * sizeof(float));
+    if (!net->top_mem) AN_CHECK(ach_malloc(&net->top_mem, 2 * list + row + (ws ? ws : 16)));
+    int32_t *dev_ids = (int32_t *)net->top_mem;
+    float *dev_lp = (float *)((char *)net->top_mem + list);
+    float *dev_ent = (float *)((char *)net->top_mem + 2 * list);
+    AN_CHECK(an_set_input(net, host_input, NULL));
+    AN_CHECK(an_forward(net, 0));
+    AN_CHECK(ach_logprobs_fwd(&d, net->layers[net->n - 2]->output, NULL, k, NULL, NULL,
+                              entropy ? dev_ent : NULL, NULL, dev_ids, dev_lp,
+                              (char *)dev_ent + row, ws, net->stream));
+    AN_CHECK(ach_memcpy_d2h(ids, dev_ids, B * k * sizeof(int32_t), net->stream));
+    AN_CHECK(ach_memcpy_d2h(logprobs, dev_lp, B * k * sizeof(float), net->stream));
+    if (entropy) AN_CHECK(ach_memcpy_d2h(entropy, dev_ent, B * sizeof(float), net->stream));
+    return ACH_OK;
+}
+
+int an_set_distillation(an_network *net, int k, int mode, float temperature, float soft,
+                        float hard)
+{
+    const an_layer *l = logits_layer(net);
+    if (!l || k <= 0 || k > l->inputs) return ACH_EINVAL;
+    const ach_logits_desc d = {l->batch, l->inputs, ACH_F32, temperature, 0};
+    const ach_distill_desc t = {k, mode, ACH_F32, soft, hard};
+    const size_t ws = ach_distill_workspace(&d, &t);
+    if (!ws) return ACH_EINVAL; /* a bad temperature, mode, k or factor     */
+    const size_t B = (size_t)l->batch, list = al(B * k * sizeof(int32_t)),
+                 row = al(B * sizeof(int32_t));
+    void *mem = NULL;
+    AN_CHECK(ach_malloc(&mem, 2 * list + row + ws));
+    const int rc = ach_stream_sync(net->stream); /* the last step read the old teacher */
+    if (rc) {
+        ach_free(mem);
+        return rc;
+    }
+    ach_free(net->teacher_mem);
+    net->teacher_mem = mem;
+    net->teacher_ids = (int32_t *)mem;
+    net->teacher_values = (float *)((char *)mem + list);
+    net->teacher_labels = (int32_t *)((char *)mem + 2 * list);
+    net->distill_ws = (char *)mem + 2 * list + row;
+    net->distill_ws_bytes = ws;
+    net->distill_logits = d;
+    net->distill = t;
+    net->distilling = 1;
+    net->teacher_ready = net->labelled = 0;
+    return ACH_OK;
+}
+
+int an_end_distillation(an_network *net)
+{
+    if (!net || !net->finalized) return ACH_EINVAL;
+    net->distilling = 0;
+    return ACH_OK;
+}
+
+int an_set_teacher(an_network *net, const int *ids, const float *values, const int *labels)
+{
+    if (!net || !net->distilling || !ids || !values) return ACH_EINVAL;
+    const size_t B = (size_t)net->batch, n = B * (size_t)net->distill.k;
+    AN_CHECK(ach_memcpy_h2d(net->teacher_ids, ids, n * sizeof(int32_t), net->stream));
+    AN_CHECK(ach_memcpy_h2d(net->teacher_values, values, n * sizeof(float), net->stream));
+    if (labels)
+        AN_CHECK(ach_memcpy_h2d(net->teacher_labels, labels, B * sizeof(int32_t), net->stream));
+    net->labelled = labels != NULL;
+    net->teacher_ready = 1;
+    return ACH_OK;
 }
 
 /* the kernels of one training step: forward, both backward streams and

@@ -394,6 +394,31 @@ int an_fuse_conv_batchnorm(an_network *net);
  * first (ties ordered as the reference's strict-'>' insertion leaves them);
  * host-only                                                                 */
 void an_top_k(const float *a, int n, int k, int *index);
+/* Inference as an_predict, answered with the best classes on the device:
+ * for every image the k (at most ACH_TOP_MAX and the classes) largest logits,
+ * ids[batch][k] largest first and equal ones by ascending id, with their log
+ * probabilities logprobs[batch][k] at `temperature` (ach_logprobs_fwd), and
+ * entropy[batch] of all classes (may be NULL).  Host buffers; synchronous.
+ * For networks that end in a softmax layer of one group, whose own
+ * temperature does not enter; else ACH_EINVAL.  The first call allocates.  */
+int an_predict_top(an_network *net, const float *host_input, int k, float temperature, int *ids,
+                   float *logprobs, float *entropy);
+/* Training from a teacher: from here on the training forward's loss and
+ * delta are ach_distill_xent's (`mode` ACH_DISTILL_RENORM or ACH_DISTILL_TAIL)
+ * against k teacher entries per image, with the factors soft and hard, in
+ * place of the cross-entropy against the truth, which is not read.  The
+ * network has to be finalized and to end in a softmax layer of one group.
+ * The layer's output stays its softmax; the first `batch` values of its loss
+ * buffer are the images' losses.  Synchronises and allocates; a new call
+ * forgets the teacher.  an_end_distillation goes back to the truth.        */
+int an_set_distillation(an_network *net, int k, int mode, float temperature, float soft,
+                        float hard);
+int an_end_distillation(an_network *net);
+/* The teacher's answers for the images of the next training steps: host
+ * ids[batch][k] (negative: none) and values[batch][k], as an_predict_top gives
+ * them, and labels[batch] (negative: none), which may be NULL if hard is 0.
+ * A training step before they are set returns ACH_EINVAL.                  */
+int an_set_teacher(an_network *net, const int *ids, const float *values, const int *labels);
 int an_backward(an_network *net);
 int an_update(an_network *net);
 /* one layer with the NetworkState the loops above would give it
