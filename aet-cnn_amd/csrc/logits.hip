@@ -640,8 +640,7 @@ __global__ void __launch_bounds__(NT)
                Total *__restrict__ part, uint64_t *__restrict__ lists)
 {
     __shared__ StatLds<NT> st;
-    __shared__ typename Pick<TOP, TopLds<NT>, int>::T top_lds;
-    TopLds<NT> &top = *(TopLds<NT> *)&top_lds;  // only with TOP
+    __shared__ typename Pick<TOP, TopLds<NT>, char>::T top;
     const float inv_t = 1.f / d.temperature, c = inv_t * LOG2E;
     for (size_t w = blockIdx.x; w < (size_t)d.rows * parts; w += gridDim.x) {
         const int r = (int)(w / parts), at = (int)(w % parts) * span;
@@ -651,28 +650,27 @@ __global__ void __launch_bounds__(NT)
         const bool given = id >= 0 && id < d.classes;
         const float x_id = given ? (float)row[id] : INFINITY;
         const Turns<TYPE, NT> turns(g);
-        const Stat mine = stream<TYPE, NT, FULL, TOP>(g, turns, c, x_id, TOP ? &top.groups : nullptr);
+        GroupLds<NT> *groups = nullptr;
+        if constexpr (TOP) groups = &top.groups;
+        const Stat mine = stream<TYPE, NT, FULL, TOP>(g, turns, c, x_id, groups);
         const Total a = total_of<TYPE, NT>(g, mine, c, st);
-        const bool bad = !(a.rest < INFINITY);
-        if (parts > 1) {
-            if (threadIdx.x == 0) part[w] = a;
-        }
+        if (parts > 1 && threadIdx.x == 0) part[w] = a;
         const float log_s = parts > 1 ? 0.f
                                       : write_row(o, r, a, given, x_id, inv_t, threadIdx.x == 0);
-        if (TOP && bad) {
-            for (int i = threadIdx.x; i < k && parts == 1; i += NT) {
-                o.top_ids[(size_t)r * k + i] = -1;
-                o.top_logprobs[(size_t)r * k + i] = NAN;
-            }
-        } else if (TOP) {
-            const int mk = min(k, g.len), n = candidates<TYPE, NT>(g, turns, mine.m, mk, top);
-            if (parts > 1) {
-                in_order<NT>(top.list, n, mk, top.places, [&](int i, uint64_t v) { lists[w * k + i] = v; });
-                for (int i = mk + threadIdx.x; i < k; i += NT) lists[w * k + i] = 0;
+        if constexpr (TOP) {
+            if (!(a.rest < INFINITY)) {  // a NaN or a +inf: the join sees it in the total
+                for (int i = threadIdx.x; i < k && parts == 1; i += NT) {
+                    o.top_ids[(size_t)r * k + i] = -1;
+                    o.top_logprobs[(size_t)r * k + i] = NAN;
+                }
             } else {
-                in_order<NT>(top.list, n, k, top.places, [&](int i, uint64_t v) {
-                    write_top(o, (size_t)r * k + i, v, a.m, inv_t, log_s);
+                const int mk = min(k, g.len), n = candidates<TYPE, NT>(g, turns, mine.m, mk, top);
+                in_order<NT>(top.list, n, mk, top.places, [&](int i, uint64_t v) {
+                    if (parts > 1) lists[w * k + i] = v;
+                    else write_top(o, (size_t)r * k + i, v, a.m, inv_t, log_s);
                 });
+                if (parts > 1)
+                    for (int i = mk + threadIdx.x; i < k; i += NT) lists[w * k + i] = 0;
             }
         }
         __syncthreads();
@@ -1392,7 +1390,7 @@ __global__ void __launch_bounds__(256) k_sum_losses(const float *__restrict__ ro
 {
     __shared__ double sh[4];
     double s = 0;
-    for (int i = threadIdx.x; i < rows; i += 256) s += row_loss[i];
+    for (size_t i = threadIdx.x; i < (size_t)rows; i += 256) s += row_loss[i];
     s = block_sum<256>(s, sh);
     if (threadIdx.x == 0) *cost = (float)s;
 }

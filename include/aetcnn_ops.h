@@ -401,7 +401,10 @@ int ach_softmax_xent(const float *in, int batch, int inputs, int groups,
  *  - a row whose logits are all -inf has no distribution: log probabilities
  *    are -inf, ranks 0, the entropy, losses and gradients 0
  *  - a row with a NaN or a +inf gives NaN, and ranks and top ids of -1
- *  - a class id outside [0, classes) stands for "none" (padding)           */
+ *  - a class id outside [0, classes) stands for "none" (padding)
+ * Workspaces are aligned to 16 bytes and belong to one call at a time: calls
+ * that may overlap, on two streams, need one each.  Outputs overlap neither
+ * one another nor the inputs, but for what is said below.                  */
 #define ACH_F32 0
 #define ACH_BF16 1
 #define ACH_F16 2

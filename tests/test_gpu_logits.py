@@ -132,6 +132,9 @@ FORWARD = [
     (3, 4099, F32, 33, 4.0, 1, 2),
     (2, 8191, BF16, 17, 1.0, 0, 1),
     (600, 9000, BF16, 20, 1.0, 0, 0),      # more rows than compute units
+    (1100, 5000, F32, 20, 1.0, 1, 0),      # a wave per row of some thousands
+    (1030, 8192, BF16, 32, 1.0, 0, 0),
+    (1025, 8191, F16, 33, 1.0, 0, 1),      # too many alternatives for that
     (3, 16411, F32, 100, 1.0, 0, 0),
     (2, 50021, F16, 20, 0.5, 3, 1),
     (700, 33000, F32, 3, 1.0, 0, 0),
@@ -175,9 +178,11 @@ def test_ids_that_are_none(gpu):
         assert (got["ranks"][[0, 1, 2, 3, 6]] == -1).all()
 
 
-@pytest.mark.parametrize("n,k", [(12, 12), (500, 40), (3000, 128), (40000, 20), (131072, 64)])
+@pytest.mark.parametrize("n,k,times", [(12, 12, 1), (500, 40, 1), (2000, 32, 1), (3000, 128, 1),
+                                       (40000, 20, 1), (131072, 64, 1), (6000, 30, 120),
+                                       (33000, 64, 32)])
 @pytest.mark.parametrize("kind", [F32, BF16, F16])
-def test_masked_classes(gpu, n, k, kind):
+def test_masked_classes(gpu, n, k, times, kind):
     """-inf: most classes masked, fewer left than alternatives, one left,
     none left; and masks of the type's lowest value"""
     rng = np.random.default_rng(n + k)
@@ -193,7 +198,7 @@ def test_masked_classes(gpu, n, k, kind):
     x[6, rng.random(n) < 0.8] = low
     x[7] = low                                      # an even distribution
     x[8, 1:] = low
-    rows = Rows(x, kind)
+    rows = Rows(np.tile(x, (times, 1)), kind)  # many rows: other kernels
     ids = rows.x.argmax(1)
     ids[1] = int(np.flatnonzero(np.isneginf(rows.x[1]))[0])  # a masked class: -inf
     ids[3] = n - 1
@@ -288,6 +293,7 @@ BACKWARD = [
     (5, 1001, BF16, 0.5, 3, 1, 0, 0),
     (9, 4097, F16, 1.0, 0, 3, 2, 1),
     (515, 5003, F32, 1.0, 1, 0, 0, 3),
+    (300, 30011, F32, 1.0, 0, 0, 0, 0),    # more than the caches hold
     (2, 50021, BF16, 1.0, 0, 0, 0, 0),
     (1, 131072, F32, 3.0, 0, 0, 0, 0),
     (3, 200001, F16, 1.0, 1, 1, 1, 1),
@@ -453,6 +459,9 @@ DISTILL = [
     (3, 8193, F16, 64, 2.0, 1, 0, 0, F32),
     (300, 20011, BF16, 9, 1.0, 0, 0, 0, BF16),
     (2, 50021, F32, 128, 1.0, 0, 0, 1, F32),
+    (2, 40000, BF16, 33, 3.0, 0, 0, 0, F32),   # rows in parts, at other temperatures
+    (5, 20000, F32, 7, 4.0, 0, 0, 0, F32),
+    (300, 30011, F32, 12, 1.0, 0, 0, 0, F32),  # more than the caches hold
     (1, 131072, BF16, 64, 1.0, 0, 0, 0, F32),
     (3, 131073, F32, 64, 2.0, 0, 1, 0, F32),
     (2, 200001, F16, 20, 1.0, 3, 1, 0, F32),
@@ -638,6 +647,36 @@ def test_offsets_past_32_bits(gpu):
     d = Distill(gpu, far, tids, values, ids, None, 1.0, DISTILL_TAIL, 0.5, 0.5, out=far_out)
     d.call()
     d.check()
+
+
+def test_more_rows_than_workgroups(gpu):
+    """over 2^20 rows: a workgroup takes several"""
+    rows, n, period = (1 << 20) + 1000, 3, 1003
+    rng = np.random.default_rng(2)
+    some = sample(rng, period, n)
+    some[5, 1] = -np.inf
+    some[6] = -np.inf
+    x = Rows(np.resize(some, (rows, n)), BF16)
+    few = Rows(some, BF16)
+    ids = np.resize(rng.integers(-1, n, period), rows)
+    f, got = check_forward(gpu, x, ids, 2, 1.0)
+    b = Backward(gpu, x, ids, 1.0, np.ones(rows), np.ones(rows), like(x))
+    b.call()
+    near(b.out.read(), b.want(), "dlogits")
+    tids, values = teacher(rng, few.x, 2, True, 1.0)
+    w = rng.uniform(0, 1, period)
+    w[9] = 0
+    args = [np.resize(a, (rows,) + a.shape[1:]) for a in (tids, values, ids[:period], w)]
+    d = Distill(gpu, x, *args, 1.0, DISTILL_TAIL, 0.5, 0.5)
+    e = Distill(gpu, few, tids, values, ids[:period], w, 1.0, DISTILL_TAIL, 0.5, 0.5)
+    d.call()
+    e.call()
+    e.check()
+    assert np.array_equal(d.out.read(), np.resize(e.out.read(), (rows, n)))
+    loss = d.loss.numpy()
+    assert np.array_equal(loss, np.resize(e.loss.numpy(), rows))
+    total = loss.astype(np.float64).sum()
+    assert abs(d.cost.numpy()[0] - total) <= 2 * ref.U * abs(total)
 
 
 class Hip:
