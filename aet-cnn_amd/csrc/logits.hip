@@ -125,6 +125,23 @@ __device__ __forceinline__ float wave_total(float v)
     v += dpp<0x143, 0xc>(0.f, v);
     return lane_value(v, 63);
 }
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp(double v)
+{
+    const uint64_t u = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false),
+              hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __longlong_as_double((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+}
+__device__ __forceinline__ double wave_total(double v)  // in lane 63 alone
+{
+    v += dpp<0x111, 0xf>(v);
+    v += dpp<0x112, 0xf>(v);
+    v += dpp<0x114, 0xf>(v);
+    v += dpp<0x118, 0xf>(v);
+    v += dpp<0x142, 0xa>(v);
+    v += dpp<0x143, 0xc>(v);
+    return v;
+}
 __device__ __forceinline__ float wave_most(float v)
 {
     v = fmaxf(v, dpp<0x111, 0xf>(v, v));
@@ -926,7 +943,7 @@ template <int NT> struct DistillLds {
     uint32_t dirty[NT];         // by thread: the turns that read a listed class
     int turn[ACH_TOP_MAX + 1];  // these, as turn * NT + thread
     int nturn;
-    int id[ACH_TOP_MAX + 1];    // as they are given, the label at [k]; -1: none
+    alignas(16) int id[ACH_TOP_MAX + 4];  // as they are given, the label at [k]; -1: none
     int repeated[ACH_TOP_MAX + 1];
     Dense wave[NT / 64];
     Listed listed[LISTED_WAVES];
@@ -1046,13 +1063,30 @@ __device__ __forceinline__ float load_any(const void *p, int type, size_t i)
                               : (float)((const _Float16 *)p)[i];
 }
 
+// Marks the listed classes that an earlier one of the list equals: the threads
+// that share a class each look through a part of the list, four at a time.
+template <int NT> __device__ __forceinline__ void find_repeated(int k, DistillLds<NT> &sh)
+{
+    int shift = 0;
+    while (1 << shift <= k) ++shift;
+    const int later = threadIdx.x & ((1 << shift) - 1), share = threadIdx.x >> shift;
+    if (later > k) return;
+    const int id = sh.id[later], step = 4 * (NT >> shift);
+    bool found = false;
+    for (int i = 4 * share; i < later; i += step)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) found |= sh.id[i + j] == id && i + j < later;
+    if (found) sh.repeated[later] = 1;
+}
+
 // The listed classes of a row, k + 1 <= NT.  Class i of the list is thread i's
 // `entry`; the waves' sums are left in sh.listed.  sh.id and sh.repeated have
 // been filled in, and a barrier has been since.
 template <int TYPE, int NT, int TWO>
 __device__ __forceinline__ void listed_terms(Entry &entry, const typename Elem<TYPE>::T *row,
                                              const void *values, int type, size_t at, int k,
-                                             bool tail, float temperature, DistillLds<NT> &sh)
+                                             bool tail, float temperature, double inv_td,
+                                             DistillLds<NT> &sh)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = threadIdx.x;
     const float inv_t = 1.f / temperature, c = inv_t * LOG2E;
@@ -1078,17 +1112,17 @@ __device__ __forceinline__ void listed_terms(Entry &entry, const typename Elem<T
         sum.e = entry.e;
         sum.e1 = entry.e1;
         if (value != -INFINITY) {
-            const double l = tail ? (double)value : ((double)value - sum.most_value) / temperature;
+            const double l = tail ? (double)value : ((double)value - sum.most_value) * inv_td;
             sum.p = exp(l);
             entry.p = (float)sum.p;
             if (sum.p != 0) sum.l = sum.p * (l - (x - sum.most) * inv_t);
         }
     }
-    sum.e = wave_all(sum.e, Add());
-    sum.e1 = wave_all(sum.e1, Add());
-    sum.p = wave_all(sum.p, Add());
-    sum.l = wave_all(sum.l, Add());
-    if (lane == 0) sh.listed[wave] = sum;
+    sum.e = wave_total(sum.e);
+    sum.e1 = wave_total(sum.e1);
+    sum.p = wave_total(sum.p);
+    sum.l = wave_total(sum.l);
+    if (lane == 63) sh.listed[wave] = sum;
 }
 
 // What the delta and the loss of a row are made of.
@@ -1156,19 +1190,20 @@ __device__ __forceinline__ RowTerms row_terms(const Dense &a, const Listed *list
             P += rest;
         }
     } else if (k > 0 && p != 0) {
-        o.scale = (float)(1 / p);
-        P = p / p;  // 1, or NaN
-        kd = l / p - logf((float)p) + lse;
+        const double to_one = 1 / p;
+        o.scale = (float)to_one;
+        P = p * to_one;  // 1, or NaN
+        kd = l * to_one - logf((float)p) + lse;
     }
-    const float per_rest = rest == 0 ? 0.f : (float)(rest / sum_rest);
+    const float per_rest = rest == 0 ? 0.f : (float)rest / sum_rest;
     o.y_rest *= per_rest;
     double v = k > 0 ? (double)t.soft * temperature * temperature * kd : 0;
     if (label) v += (double)t.hard * ((double)lse1 - ((double)x_y - ref));
     o.loss = o.empty ? 0.f : (float)(w * v);
     o.soft = k > 0 ? -w * t.soft * temperature : 0.f;
     o.hard = label ? -w * t.hard : 0.f;
-    o.P_total = o.empty ? 0.f : (float)(P / total);
-    o.one_total = o.empty ? 0.f : (float)(1 / total1);
+    o.P_total = o.empty ? 0.f : (float)P / (float)total;
+    o.one_total = o.empty ? 0.f : 1.f / (float)total1;
     o.K = o.soft == 0.f ? 0.f : o.soft * (o.P_total * up - per_rest * down);
     o.K1 = o.hard == 0.f ? 0.f : o.hard * o.one_total * up1;
     if (!TWO) o.K += o.K1;
@@ -1242,6 +1277,7 @@ __global__ void __launch_bounds__(NT, 4)
     const int k = t.soft != 0.f ? t.k : 0;
     const bool tail = t.mode == ACH_DISTILL_TAIL;
     const float c = LOG2E / d.temperature;
+    const double inv_td = 1. / d.temperature;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int groups = MODE == STATS ? parts + 1 : parts;
     if (MODE == DELTA && blockIdx.x == (unsigned)(d.rows * parts)) {
@@ -1284,16 +1320,11 @@ __global__ void __launch_bounds__(NT, 4)
         }
         if (MODE == WHOLE || (MODE == STATS && part == parts)) {
             __syncthreads();
-            int width = 1, shift = 0;
-            while (width <= k) width <<= 1, ++shift;
-            for (int i = threadIdx.x; i < (k + 1) << shift; i += NT) {
-                const int later = i >> shift, former = i & (width - 1);
-                if (former < later && sh.id[former] == sh.id[later]) sh.repeated[later] = 1;
-            }
+            find_repeated<NT>(k, sh);
             __syncthreads();
             if (threadIdx.x == 0) sh.extra = y >= 0 && !sh.repeated[k];
             listed_terms<TYPE, NT, TWO>(entry, row, teacher_values, t.teacher_type, (size_t)r * k, k,
-                                        tail, d.temperature, sh);
+                                        tail, d.temperature, inv_td, sh);
         }
         if (MODE == STATS && part == parts) {
             __syncthreads();
