@@ -641,8 +641,6 @@ __device__ __forceinline__ void write_top(const LogprobsOut &o, size_t at, uint6
         m == -INFINITY ? -INFINITY : (key_value((uint32_t)(v >> 32)) - m) * inv_t - log_s;
 }
 
-// One workgroup per row, or per part of a row (parts > 1), `span` classes
-// each; the parts' totals and their k largest go to `part` and `lists`.
 template <bool B, class X, class Y> struct Pick {
     using T = X;
 };
@@ -650,6 +648,8 @@ template <class X, class Y> struct Pick<false, X, Y> {
     using T = Y;
 };
 
+// One workgroup per row, or per part of a row (parts > 1), `span` classes
+// each; the parts' totals and their k largest go to `part` and `lists`.
 template <int TYPE, int NT, bool FULL, bool TOP>
 __global__ void __launch_bounds__(NT)
     k_logprobs(ach_logits_desc d, const typename Elem<TYPE>::T *__restrict__ logits,
@@ -1416,13 +1416,26 @@ __global__ void __launch_bounds__(NT, 4)
     }
 }
 
-__global__ void __launch_bounds__(256) k_sum_losses(const float *__restrict__ row_loss, int rows,
-                                                    float *cost)
+// The sum of the rows' losses in a fixed order, eight loads in flight a thread
+// (one after the other, 4096 of them took 256 threads longer than their rows).
+constexpr int SUM_THREADS = 1024;
+__global__ void __launch_bounds__(SUM_THREADS) k_sum_losses(const float *__restrict__ row_loss,
+                                                            int rows, float *cost)
 {
-    __shared__ double sh[4];
+    constexpr int U = 8;
+    __shared__ double sh[SUM_THREADS / 64];
     double s = 0;
-    for (size_t i = threadIdx.x; i < (size_t)rows; i += 256) s += row_loss[i];
-    s = block_sum<256>(s, sh);
+    for (size_t first = threadIdx.x; first < (size_t)rows; first += U * SUM_THREADS) {
+        float v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t i = first + u * SUM_THREADS;
+            v[u] = i < (size_t)rows ? row_loss[i] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) s += v[u];
+    }
+    s = block_sum<SUM_THREADS>(s, sh);
     if (threadIdx.x == 0) *cost = (float)s;
 }
 
@@ -1686,7 +1699,8 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
         if (rc || !cost || sp.parts > 1) return rc;
     }
     if (!cost) return ACH_OK;
-    hipLaunchKernelGGL(k_sum_losses, dim3(1), dim3(256), 0, st, (const float *)ws, d.rows, cost);
+    hipLaunchKernelGGL(k_sum_losses, dim3(1), dim3(SUM_THREADS), 0, st, (const float *)ws, d.rows,
+                       cost);
     return check_launch();
 }
 
