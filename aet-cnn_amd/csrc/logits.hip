@@ -306,7 +306,8 @@ __device__ __forceinline__ Stat stream(const Range<TYPE> &g, const Turns<TYPE, N
     Chunk v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-        if (left + u * NT + lane < n) v[u] = Row<TYPE>::load(g.p + (size_t)(left + u * NT + lane) * V);
+        if (left + u * NT + lane < n)
+            v[u] = Row<TYPE>::load(g.p + (size_t)(left + u * NT + lane) * V);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         if (left + u * NT >= n) break;
@@ -1212,7 +1213,8 @@ __device__ __forceinline__ RowTerms row_terms(const Dense &a, const Listed *list
         if (sum_rest != 0.f) {
             rest = p > 1 ? 0 : 1 - p;
             if (rest != 0)
-                kd += rest * (logf((float)rest) - (logf(sum_rest) + (top_rest - ref) * inv_t - lse));
+                kd += rest *
+                      (logf((float)rest) - (logf(sum_rest) + (top_rest - ref) * inv_t - lse));
             P += rest;
         }
     } else if (k > 0 && p != 0) {
@@ -1263,7 +1265,8 @@ __device__ __forceinline__ void part_losses(const ach_logits_desc &d, const ach_
 {
     __shared__ double sums[NT / 64];
     const int k = t.soft != 0.f ? t.k : 0, r = threadIdx.x;
-    const float c = LOG2E / d.temperature, w = r < d.rows ? row_weights ? row_weights[r] : 1.f : 0.f;
+    const float c = LOG2E / d.temperature;
+    const float w = r >= d.rows ? 0.f : row_weights ? row_weights[r] : 1.f;
     float v = 0.f;
     if (w != 0.f) {
         Dense a = {-FLT_MAX, 0.f, 0.f};
@@ -1349,8 +1352,8 @@ __global__ void __launch_bounds__(NT, 4)
             find_repeated<NT>(k, sh);
             __syncthreads();
             if (threadIdx.x == 0) sh.extra = y >= 0 && !sh.repeated[k];
-            listed_terms<TYPE, NT, TWO>(entry, row, teacher_values, t.teacher_type, (size_t)r * k, k,
-                                        tail, d.temperature, inv_td, sh);
+            listed_terms<TYPE, NT, TWO>(entry, row, teacher_values, t.teacher_type,
+                                        (size_t)r * k, k, tail, d.temperature, inv_td, sh);
         }
         if (MODE == STATS && part == parts) {
             __syncthreads();
@@ -1412,8 +1415,10 @@ __global__ void __launch_bounds__(NT, 4)
                 Chunk v[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (q - u * NT >= stash_chunks) v[u] = Row<TYPE>::load(g.p + (size_t)(q - u * NT) * V);
-                    else if (q - u * NT >= 0) __builtin_memcpy(&v[u], &stash[q - u * NT], 16);
+                    if (q - u * NT >= stash_chunks)
+                        v[u] = Row<TYPE>::load(g.p + (size_t)(q - u * NT) * V);
+                    else if (q - u * NT >= 0)
+                        __builtin_memcpy(&v[u], &stash[q - u * NT], 16);
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     if (q - u * NT < 0) break;
@@ -1426,20 +1431,24 @@ __global__ void __launch_bounds__(NT, 4)
         };
         if (past) write(Flag<true>());
         else write(Flag<false>());
-        if (threadIdx.x < g.rest()) out[n * V + threadIdx.x] = grad((float)g.p[n * V + threadIdx.x]);
+        if (threadIdx.x < g.rest()) {
+            const int j = n * V + threadIdx.x;
+            out[j] = grad((float)g.p[j]);
+        }
         __syncthreads();  // the listed classes over what was written for them
         const int i = threadIdx.x, of = i >> 6;
         if (MODE == DELTA && i <= k) entry = list->entry[i];
         if (i <= k && entry.id >= at && entry.id < at + g.len) {
-            const float to_e = of == 0 ? terms.to_e[0] : of == 1 ? terms.to_e[1] : terms.to_e[2],
-                        to_e1 = of == 0 ? terms.to_e1[0] : of == 1 ? terms.to_e1[1] : terms.to_e1[2],
-                        to_p = of == 0 ? terms.to_p[0] : of == 1 ? terms.to_p[1] : terms.to_p[2];
+            const auto own = [&](const float (&to)[LISTED_WAVES]) {
+                return of == 0 ? to[0] : of == 1 ? to[1] : to[2];
+            };
+            const float e = entry.e * own(terms.to_e), e1 = entry.e1 * own(terms.to_e1),
+                        p = entry.p * own(terms.to_p) * terms.scale;
             float v = 0.f;
             if (terms.soft != 0.f)
-                v = terms.soft * (terms.P_total * entry.e * to_e -
-                                  (i < k ? entry.p * to_p * terms.scale : terms.y_rest));
+                v = terms.soft * (terms.P_total * e - (i < k ? p : terms.y_rest));
             if (terms.hard != 0.f)
-                v += terms.hard * (terms.one_total * entry.e1 * to_e1 - (entry.id == y ? 1.f : 0.f));
+                v += terms.hard * (terms.one_total * e1 - (entry.id == y ? 1.f : 0.f));
             out[entry.id - at] = (T)(terms.empty ? 0.f : v);
         }
     }
@@ -1706,8 +1715,9 @@ int ach_distill_xent(const ach_logits_desc *desc, const ach_distill_desc *teache
         int stashed = (int)((size_t)d.classes * elem_size(d.type) / turn_bytes);
         const int room = sp.parts > 1 || !delta ? 0 : 32768 / turn_bytes;
         stashed = stashed < room ? stashed : room;
-#define GO(TYPE, NT, TWO, MODE, GRID)                                                       \
-    hipLaunchKernelGGL((k_distill<TYPE, NT, TWO, MODE>), GRID, dim3(NT), stashed * turn_bytes, st, d, t,       \
+        const size_t lds = (size_t)stashed * turn_bytes;
+#define GO(TYPE, NT, TWO, MODE, GRID)                                                             \
+    hipLaunchKernelGGL((k_distill<TYPE, NT, TWO, MODE>), GRID, dim3(NT), lds, st, d, t,           \
                        (const Elem<TYPE>::T *)logits, teacher_ids, teacher_values, labels,        \
                        row_weights, loss, (Elem<TYPE>::T *)delta, delta_stride, row_loss,         \
                        sp.parts, sp.span, stashed, between, past, cost)

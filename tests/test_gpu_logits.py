@@ -709,6 +709,12 @@ def stream(gpu):
     check(gpu.ach_stream_destroy(s.value))
 
 
+def bits(f, d):
+    """the bits of all outputs of a forward call and a distillation"""
+    return b"".join([v.tobytes() for _, v in sorted(f.read().items())] +
+                    [a.tobytes() for a in (d.loss.numpy(), d.out.read(), d.cost.numpy())])
+
+
 def test_graph_replays(gpu, stream):
     """captured, then replayed with other inputs, with eager calls between;
     two graphs share a workspace"""
@@ -740,12 +746,11 @@ def test_graph_replays(gpu, stream):
             got = f.read()
             for name, v in got.items():
                 near(v, want[name], name)
-            graph = [f.read()[n].tobytes() for n in sorted(f.out)] + [d.loss.numpy().tobytes(), d.out.read().tobytes()]
+            graph = bits(f, d)
             f.call(stream)   # eager, between the replays
             d.call(stream)
             check(gpu.ach_stream_sync(stream))
-            eager = [f.read()[n].tobytes() for n in sorted(f.out)] + [d.loss.numpy().tobytes(), d.out.read().tobytes()]
-            assert graph == eager
+            assert graph == bits(f, d)
 
 
 def test_two_streams_at_once(gpu, stream):
@@ -784,8 +789,7 @@ def test_runs_are_equal(gpu, n, kind):
     for _ in range(12):
         f.call()
         d.call()
-        seen.add(b"".join([f.read()[k].tobytes() for k in sorted(f.out)] +
-                          [d.loss.numpy().tobytes(), d.out.read().tobytes(), d.cost.numpy().tobytes()]))
+        seen.add(bits(f, d))
     assert len(seen) == 1
 
 

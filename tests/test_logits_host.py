@@ -164,3 +164,21 @@ def test_reference_logprobs_gradient():
     o = ref.logprobs(x, ids, 0, t)
     got, _ = ref.logprobs_bwd(x, ids, t, o["stats"][0], o["entropy"][0], g, h, ref.F32)
     assert np.abs(got - _differences(value, x)).max() < 1e-8
+
+
+def test_launches(tmp_path):
+    """One launch for a forward call but for few long rows, two for these; two
+    for a distillation with its cost; dynamic LDS that needs no limit raised."""
+    p = "p"
+    fwd = [(1, 131072, 2), (64, 100003, 2), (1, 60000, 1), (128, 1000, 1), (1024, 131072, 1),
+           (4096, 100, 1), (256, 65536, 2), (257, 65536, 1)]
+    calls = [["ach_logprobs_fwd", [{"logits": [r, n, 1, 1.0, 0]}, p, p, 20, p, p, p, p, p, p, p, BIG,
+                                   None]] for r, n, _ in fwd]
+    dis = [(1, 200001, 2), (16, 131072, 2), (128, 1000, 2), (2048, 131072, 2), (100, 9000, 2)]
+    calls += [["ach_distill_xent", [{"logits": [r, n, 0, 2.0, 0]}, {"distill": [64, 1, 0, 0.5, 0.5]},
+                                    p, p, p, p, None, p, p, 0, p, p, BIG, None]] for r, n, _ in dis]
+    for call, want, got in zip(calls, [w for *_, w in fwd + dis], record(calls, tmp_path)):
+        assert got["rc"] == 0 and len(got["launches"]) == want, (call, got)
+        for v in got["launches"]:
+            assert v["lds"] <= 32768 and v["grid"][1:] == [1, 1]
+            assert v["grid"][0] * v["block"][0] < 2 ** 32
