@@ -651,6 +651,9 @@ template <class X, class Y> struct Pick<false, X, Y> {
 
 // One workgroup per row, or per part of a row (parts > 1), `span` classes
 // each; the parts' totals and their k largest go to `part` and `lists`.
+// 4096 x 32768 bf16 without alternatives: 55 us, 4.9 TB/s, the vector unit 85%
+// busy with 11 instructions a logit.  1024 x 131072 bf16 with 20: 59 us, 4.5 TB/s;
+// its rows are all in step, so the 4 us of the alternatives show.
 template <int TYPE, int NT, bool FULL, bool TOP>
 __global__ void __launch_bounds__(NT)
     k_logprobs(ach_logits_desc d, const typename Elem<TYPE>::T *__restrict__ logits,
@@ -701,7 +704,8 @@ __global__ void __launch_bounds__(NT)
 // of four such bounds, of 16 bits, are put in order.  If these are too many,
 // logits being equal or spread unevenly, the same bounds are taken exactly and
 // for every power of two: then, for m = 1, 2, 4, ..., no more than m lists have
-// ceil(k/m) entries that pass, which adds up to k (2 + log2 parts).
+// ceil(k/m) entries that pass, which adds up to k (2 + log2 parts).  A chain of
+// waits: 5 us for one row of 32 parts with 20 entries each.
 constexpr int MOST_PARTS = 64;
 
 template <int TYPE, int NT>
@@ -817,6 +821,7 @@ __global__ void __launch_bounds__(NT)
 // Each workgroup writes `span` chunks of a row.  With l = log p,
 // dx = p (a + b l) for a = -(g + h H)/T, b = -h/T; of the given class
 // g (1 - p) = -g expm1(l), which keeps its precision where p is near 1.
+// 4096 x 32768 bf16: 93 us, 5.7 TB/s.
 template <int TYPE>
 __global__ void __launch_bounds__(256)
     k_logprobs_bwd(ach_logits_desc d, const typename Elem<TYPE>::T *logits,
@@ -885,7 +890,8 @@ struct Dense {
 
 // Whether the label's exponentials, at temperature 1, are wanted next to the
 // teacher's, and how they are had: not apart (ONE), on their own, or at
-// temperatures 2 and 4 as powers of these, a third less work for a row.
+// temperatures 2 and 4 as powers of these (1021 x 50021 fp16 at temperature 2:
+// 67 -> 62 us).
 enum { ONE = 0, BOTH = 1, SQUARE = 2, FOURTH = 4 };
 
 template <int TWO> __device__ __forceinline__ float second(float e, float d)
@@ -1291,6 +1297,10 @@ __device__ __forceinline__ void part_losses(const ach_logits_desc &d, const ach_
     if (r == 0) *cost = (float)sum;
 }
 
+// 2048 x 131072 bf16, 64 entries: 266 us, 4.0 TB/s of logits read once and the
+// delta; the second reading comes from HBM in part, as the rows in flight, four a
+// compute unit, fill the 256 MB cache.  Fewer leave the waits of a row's start
+// and middle open (three: 312 us, two: 346).
 template <int TYPE, int NT, int TWO, int MODE>
 __global__ void __launch_bounds__(NT, 4)
     k_distill(ach_logits_desc d, ach_distill_desc t, const typename Elem<TYPE>::T *logits,

@@ -563,6 +563,58 @@ def test_distill_masked_by_the_student(gpu):
         d.check()
 
 
+@pytest.mark.parametrize("n", [12, 3000, 131072])
+def test_labels_of_masked_classes(gpu, n):
+    """the loss of a label that the student has masked is +inf, its delta finite"""
+    rng = np.random.default_rng(n)
+    x = sample(rng, 3, n)
+    x[0, n - 1] = -np.inf
+    x[1, :-1] = -np.inf
+    rows = Rows(x, F32)
+    ids, values = teacher(rng, rows.x, 4, True, 1.0)
+    labels = np.array([n - 1, 0, 5])
+    for soft in (0.0, 0.5):
+        d = Distill(gpu, rows, ids, values, labels, None, 1.0, DISTILL_TAIL, soft, 0.5)
+        d.call()
+        loss, got = d.loss.numpy(), d.out.read()
+        assert np.isposinf(loss[:2]).all() and np.isfinite(loss[2]) and np.isfinite(got).all()
+        assert np.isposinf(d.cost.numpy()[0])
+        near(got, d.want()[2:], "delta")
+
+
+@pytest.mark.parametrize("n", [12, 3000, 131072])
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_largest_numbers(gpu, n, kind):
+    """logits at both ends of the type, whose differences overflow"""
+    rng = np.random.default_rng(n)
+    big = 3.3895313892515355e38
+    x = sample(rng, 4, n)
+    x[0, 3], x[0, 5] = big, -big
+    x[1] = rng.choice([big, -big], n)
+    x[2, ::2] = -big
+    x[3] = -big
+    x[3, n // 2] = big
+    rows = Rows(x, kind)
+    ids = np.array([3, 5, n - 1, n // 2])
+    for t in (1.0, 0.25):
+        f = Forward(gpu, rows, ids, 4, t)
+        f.call()
+        got = f.read()
+        with np.errstate(over="ignore"):
+            want = ref.logprobs(rows.x, ids, 4, t)
+        for name, v in got.items():
+            value, bound = want[name]  # beyond the largest number: -inf
+            if value.dtype == np.float64:
+                value = np.where(np.abs(value) > 3.5e38, np.copysign(np.inf, value), value)
+            near(v, (value, bound), name)
+    d = Distill(gpu, rows, np.array([[3, 1]] * 4), np.log(np.full((4, 2), 0.25)), None,
+                [1.0, 1, 1, 1], 1.0, DISTILL_TAIL, 1.0, 0.0)
+    d.call()
+    got = d.out.read()
+    # a row's deltas add up to 0; their sizes to 2 at most, each rounded by up to 2^-8
+    assert np.isfinite(got).all() and np.abs(got.sum(1)).max() < 2 * 2.0 ** -8 + 1e-3
+
+
 @pytest.mark.parametrize("outputs", [("loss",), ("delta",), ("cost",), ("loss", "cost"),
                                      ("delta", "cost")])
 @pytest.mark.parametrize("n", [100, 4000, 131072])
