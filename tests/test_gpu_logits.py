@@ -267,6 +267,30 @@ def test_large_logits_in_one_place(gpu, n, kind):
     check_forward(gpu, rows, np.arange(10), 20, 1.0)
 
 
+@pytest.mark.parametrize("n", [40003, 60001, 140000])
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_equal_logits_by_groups(gpu, n, kind):
+    """most logits are equal, with larger ones, lower ones or none allowed in
+    whole stretches: groups of logits are left out, or read and hold no others"""
+    rng = np.random.default_rng(n)
+    j = np.arange(n)
+    x = np.ones((10, n))
+    x[1, j < n // 2] = -np.inf                           # half of the groups closed
+    x[2, rng.random(n) > 1e-3] = -np.inf                 # some allowed, all equal
+    x[3, 37::997] = 2 + np.arange(len(j[37::997])) / 64  # larger ones, late too
+    x[4, -5:] = 3                                        # larger ones behind all others
+    x[5, :1500] = 2 + np.arange(1500) % 7                # larger ones, equal too
+    x[6, j != n - 2] = -np.inf                           # fewer than k allowed
+    x[7] = np.where(j % 3, np.finfo(np.float32).min / 2, 1.0)
+    x[7, :n // 2] = np.finfo(np.float32).min / 2         # a mask of large finite values
+    x[8] = np.where(j < 700, j / 8, 0.0)                 # too many for the list
+    x[9, ::2] = -3
+    rows = Rows(x, kind)
+    ids = rng.integers(0, n, len(x))
+    for k in (1, 20, 128):
+        check_forward(gpu, rows, ids, k, 1.0)
+
+
 @pytest.mark.parametrize("n", [10, 1000, 30000, 131072])
 def test_certain_rows(gpu, n):
     """where one class has nearly all the probability, its log probability and
