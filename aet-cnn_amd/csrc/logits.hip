@@ -942,8 +942,9 @@ __device__ __forceinline__ void absorb_dense(Dense &a, const float (&x)[N], floa
 }
 
 // A wave's listed classes (classes 64 w to 64 w + 63 of the list): their
-// maximum `most` (0 if none is finite) and that of the teacher's values, and
-// relative to these the sums of e, e1, p, and p (log p - (x - most)/T).
+// maximum `most` (0 if none is finite: then e is 0, and `most` says nothing of
+// where the row's logits lie) and that of the teacher's values, and relative to
+// these the sums of e, e1, p, and p (log p - (x - most)/T).
 struct Listed {
     float most, most_value;
     double e, e1, p, l;
@@ -1201,14 +1202,16 @@ __device__ __forceinline__ RowTerms row_terms(const Dense &a, const Listed *list
         o.to_e[i] = o.to_e1[i] = o.to_p[i] = 0.f;
         if (i >= waves) continue;
         const Listed &s = listed[i];
-        o.to_e[i] = exp2_fast((s.most - ref) * c);
-        o.to_e1[i] = TWO ? exp2_fast((s.most - ref) * LOG2E) : o.to_e[i];
-        const float lower = tail || s.most_value == -INFINITY ? 0.f : s.most_value - most_value;
-        o.to_p[i] = exp2_fast(lower * c);
+        // where a wave's classes are all masked the factors stay 0: from `most` they
+        // would be infinite in rows of low logits, and 0 times that a NaN
         if (s.e != 0) {
+            o.to_e[i] = exp2_fast((s.most - ref) * c);
+            o.to_e1[i] = TWO ? exp2_fast((s.most - ref) * LOG2E) : o.to_e[i];
             e += s.e * o.to_e[i];
             e1 += s.e1 * o.to_e1[i];
         }
+        const float lower = tail || s.most_value == -INFINITY ? 0.f : s.most_value - most_value;
+        o.to_p[i] = exp2_fast(lower * c);
         if (s.p == 0) continue;
         p += s.p * o.to_p[i];
         l += o.to_p[i] * (s.l + s.p * ((double)lower - ((double)s.most - ref)) * inv_t);
