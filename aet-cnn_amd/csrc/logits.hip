@@ -942,9 +942,10 @@ __device__ __forceinline__ void absorb_dense(Dense &a, const float (&x)[N], floa
 }
 
 // A wave's listed classes (classes 64 w to 64 w + 63 of the list): their
-// maximum `most` (0 if none is finite: then e is 0, and `most` says nothing of
-// where the row's logits lie) and that of the teacher's values, and relative to
-// these the sums of e, e1, p, and p (log p - (x - most)/T).
+// maximum `most` (-inf if none is listed; 0 if none of them is finite: then e is
+// 0, and `most` says nothing of where the row's logits lie) and that of the
+// teacher's values, and relative to these the sums of e, e1, p, and
+// p (log p - (x - most)/T).
 struct Listed {
     float most, most_value;
     double e, e1, p, l;
@@ -1152,7 +1153,7 @@ __device__ __forceinline__ void listed_terms(Entry &entry, const typename Elem<T
     }
     sum.most = wave_most(x);
     sum.most_value = wave_most(value);
-    if (sum.most == -INFINITY) sum.most = 0.f;
+    if (sum.most == -INFINITY && __any(id >= 0)) sum.most = 0.f;
     if (entry.id >= 0) {
         entry.e = exp2_fast((x - sum.most) * c);
         entry.e1 = TWO ? exp2_fast((x - sum.most) * LOG2E) : entry.e;
@@ -1179,7 +1180,7 @@ struct RowTerms {
     float P_total, one_total, soft, hard, scale, y_rest;
     float to_e[LISTED_WAVES], to_e1[LISTED_WAVES], to_p[LISTED_WAVES];  // from a wave's maxima
     float loss;
-    bool empty;
+    bool empty, none;  // no logit, or no listed class: all of it is 0
 };
 
 template <int TWO>
@@ -1192,7 +1193,9 @@ __device__ __forceinline__ RowTerms row_terms(const Dense &a, const Listed *list
     RowTerms o;
     o.m = a.m;
     float ref = a.m, most_value = -INFINITY;  // the row's maximum
+    o.none = true;
     for (int i = 0; i < waves; ++i) {
+        o.none &= listed[i].most == -INFINITY;
         if (listed[i].e != 0) ref = fmaxf(ref, listed[i].most);
         most_value = fmaxf(most_value, listed[i].most_value);
     }
@@ -1244,12 +1247,14 @@ __device__ __forceinline__ RowTerms row_terms(const Dense &a, const Listed *list
         o.scale = (float)to_one;
         P = p * to_one;  // 1, or NaN
         kd = l * to_one - logf((float)p) + lse;
+    } else if (k > 0) {
+        kd = 0.f * lse;  // entries without probability: 0, or NaN
     }
     const float per_rest = rest == 0 ? 0.f : (float)rest / sum_rest;
     o.y_rest *= per_rest;
     double v = k > 0 ? (double)t.soft * temperature * temperature * kd : 0;
     if (label) v += (double)t.hard * ((double)lse1 - ((double)x_y - ref));
-    o.loss = o.empty ? 0.f : (float)(w * v);
+    o.loss = o.empty || o.none ? 0.f : (float)(w * v);
     o.soft = k > 0 ? -w * t.soft * temperature : 0.f;
     o.hard = label ? -w * t.hard : 0.f;
     o.P_total = o.empty ? 0.f : (float)P / (float)total;
@@ -1425,6 +1430,11 @@ __global__ void __launch_bounds__(NT, 4)
         }
         if (!delta) continue;
         T *out = delta + (size_t)r * delta_stride + at;
+        if (terms.none) {  // a short loop: a second copy of the one above costs others 2%
+#pragma unroll 1
+            for (int j = threadIdx.x; j < g.len; j += NT) out[j] = (T)0.f;
+            continue;
+        }
         const auto grad = [&](float v) {
             const float x = v - terms.m, e = exp2_fast(x * c);
             float o = terms.K * e;

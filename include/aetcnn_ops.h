@@ -400,7 +400,8 @@ int ach_softmax_xent(const float *in, int batch, int inputs, int groups,
  *  - a logit of -inf is a masked class: its probability is 0
  *  - a row whose logits are all -inf has no distribution: log probabilities
  *    are -inf, ranks 0, the entropy, losses and gradients 0
- *  - a row with a NaN or a +inf gives NaN, and ranks and top ids of -1
+ *  - a row with a NaN or a +inf gives NaN, and ranks and top ids of -1 (but
+ *    for the rows that are said below to be set to 0)
  *  - a class id outside [0, classes) stands for "none" (padding)
  * Workspaces are aligned to 16 bytes and belong to one call at a time: calls
  * that may overlap, on two streams, need one each.  Outputs overlap neither
@@ -460,10 +461,12 @@ int ach_logprobs_bwd(const ach_logits_desc *d, const void *logits, const int32_t
  *   *cost = sum of loss[r] (in double, rounded once)
  * Either term is left out where its factor is 0 (soft: the teacher may then
  * be NULL and k 0; hard: labels may be NULL); a label that is none has no
- * second term.  row_weights NULL: 1; rows of weight 0 are set to 0 without
- * reading their logits.  delta (of the logits' type, rows delta_stride apart,
- * 0: classes; it may be `logits` itself with the same stride), loss and cost
- * may be NULL, not all three; cost and delta need no loss array.           */
+ * second term.  row_weights NULL: 1.  Rows of weight 0, and rows that are left
+ * with neither an entry nor a label, have loss and delta 0, whatever their
+ * logits hold; in other rows a NaN or a +inf makes both NaN.  delta (of the
+ * logits' type, rows delta_stride apart, 0: classes; it may be `logits` itself
+ * with the same stride), loss and cost may be NULL, not all three; cost and
+ * delta need no loss array.                                                */
 #define ACH_DISTILL_RENORM 0
 #define ACH_DISTILL_TAIL 1
 typedef struct {
