@@ -624,6 +624,13 @@ struct LogprobsOut {
     float *top_logprobs;
 };
 
+// (x - m)/T, also where the difference is beyond the largest number of 32 bits,
+// as for masks of a type's lowest value, and its quotient is not.
+__device__ __forceinline__ float scaled(float x, float m, float inv_t)
+{
+    return (float)(((double)x - m) * inv_t);
+}
+
 // A row's outputs but its alternatives; returns the log of its sum.
 __device__ float write_row(const LogprobsOut &o, int r, const Total &a, bool given, float x_id,
                            float inv_t, bool first_thread)
@@ -632,7 +639,7 @@ __device__ float write_row(const LogprobsOut &o, int r, const Total &a, bool giv
     const float log_s = empty ? -INFINITY : log1pf(a.rest);
     if (first_thread) {
         if (o.logprobs)
-            o.logprobs[r] = !given ? 0.f : empty ? -INFINITY : (x_id - a.m) * inv_t - log_s;
+            o.logprobs[r] = !given ? 0.f : empty ? -INFINITY : scaled(x_id, a.m, inv_t) - log_s;
         if (o.ranks) o.ranks[r] = !given || bad ? -1 : a.above;
         if (o.entropy) o.entropy[r] = empty ? 0.f : log_s - a.t * LN2 / (1.f + a.rest);
         if (o.stats) {
@@ -648,7 +655,7 @@ __device__ __forceinline__ void write_top(const LogprobsOut &o, size_t at, uint6
 {
     o.top_ids[at] = (int)~(uint32_t)v;
     o.top_logprobs[at] =
-        m == -INFINITY ? -INFINITY : (key_value((uint32_t)(v >> 32)) - m) * inv_t - log_s;
+        m == -INFINITY ? -INFINITY : scaled(key_value((uint32_t)(v >> 32)), m, inv_t) - log_s;
 }
 
 template <bool B, class X, class Y> struct Pick {
