@@ -1170,7 +1170,7 @@ __device__ __forceinline__ void listed_terms(Entry &entry, const typename Elem<T
             const double l = tail ? (double)value : ((double)value - sum.most_value) * inv_td;
             sum.p = exp(l);
             entry.p = (float)sum.p;
-            if (sum.p != 0) sum.l = sum.p * (l - (x - sum.most) * inv_t);
+            if (sum.p != 0) sum.l = sum.p * (l - ((double)x - sum.most) * inv_td);
         }
     }
     sum.e = wave_total(sum.e);
@@ -1196,7 +1196,8 @@ __device__ __forceinline__ RowTerms row_terms(const Dense &a, const Listed *list
                                               bool label, bool extra, float x_y, float w)
 {
     const bool tail = t.mode == ACH_DISTILL_TAIL;
-    const float inv_t = 1.f / temperature, c = inv_t * LOG2E;
+    const float c = LOG2E / temperature;
+    const double inv_td = 1. / temperature;
     RowTerms o;
     o.m = a.m;
     float ref = a.m, most_value = -INFINITY;  // the row's maximum
@@ -1220,11 +1221,15 @@ __device__ __forceinline__ RowTerms row_terms(const Dense &a, const Listed *list
             e += s.e * o.to_e[i];
             e1 += s.e1 * o.to_e1[i];
         }
-        const float lower = tail || s.most_value == -INFINITY ? 0.f : s.most_value - most_value;
-        o.to_p[i] = exp2_fast(lower * c);
-        if (s.p == 0) continue;
-        p += s.p * o.to_p[i];
-        l += o.to_p[i] * (s.l + s.p * ((double)lower - ((double)s.most - ref)) * inv_t);
+        // in 64 bits: a class that the student has masked makes s.l infinite,
+        // however little probability the teacher gives it
+        const double lower =
+            tail || s.most_value == -INFINITY ? 0 : (double)s.most_value - most_value;
+        const double to_p = lower == 0 ? 1 : exp(lower * inv_td);
+        o.to_p[i] = (float)to_p;
+        if (s.p == 0 || to_p == 0) continue;
+        p += s.p * to_p;
+        l += to_p * (s.l + s.p * (lower - ((double)s.most - ref)) * inv_td);
     }
     // without a dense class of finite logit a.s is 0
     const float up = exp2_fast((a.m - ref) * c), up1 = TWO ? exp2_fast((a.m - ref) * LOG2E) : up;
@@ -1245,8 +1250,8 @@ __device__ __forceinline__ RowTerms row_terms(const Dense &a, const Listed *list
         if (sum_rest != 0.f) {
             rest = p > 1 ? 0 : 1 - p;
             if (rest != 0)
-                kd += rest *
-                      (logf((float)rest) - (logf(sum_rest) + (top_rest - ref) * inv_t - lse));
+                kd += rest * (logf((float)rest) -
+                              (logf(sum_rest) + ((double)top_rest - ref) * inv_td - lse));
             P += rest;
         }
     } else if (k > 0 && p != 0) {
