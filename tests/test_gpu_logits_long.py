@@ -32,7 +32,8 @@ class Repeated:
         self.dev = D(rows * row, np.uint8)
         self.ptr = self.dev.ptr
         for r in range(0, rows, few.rows):
-            check(gpu.ach_memcpy_d2d(self.ptr + r * row, few.ptr, min(few.rows, rows - r) * row, None))
+            check(gpu.ach_memcpy_d2d(self.ptr + r * row, few.ptr, min(few.rows, rows - r) * row,
+                                     None))
 
     def first(self):
         """the first rows as numbers, after a look at the others"""
@@ -193,7 +194,8 @@ def test_equal_logits_distilled(gpu, rows, n, kind, soft, hard, t, mode):
         for v, value, size in [(g, -dense[r], soft * t / (c[r] - 4) + hard / c[r]) for g in got] + \
                 [(delta[r, lists[i]], -(off[r] - (hard if i == 2 else 0)), soft * t + hard)
                  for i in range(4)]:
-            assert abs(v - value) <= 16 * U * size + half * max(abs(value), ref.TINY[kind]), (r, v, value)
+            tol = 16 * U * size + half * max(abs(value), ref.TINY[kind])
+            assert abs(v - value) <= tol, (r, v, value)
 
 
 @pytest.mark.parametrize("rows,n,kind,k,t,mode", [
@@ -240,7 +242,8 @@ def test_gradient_of_long_rows(gpu):
                 (last.astype(np.int32), stats, log, np.full(len(x), 0.5, np.float32),
                  np.full(len(x), -0.25, np.float32))]
         desc = aetcnn.LogitsDesc(rows, n, kind, 1.0, n)
-        check(gpu.ach_logprobs_bwd(C.byref(desc), big.ptr, *[b.ptr for b in held], out.ptr, 0, None))
+        check(gpu.ach_logprobs_bwd(C.byref(desc), big.ptr, *[b.ptr for b in held], out.ptr, 0,
+                                   None))
         got = out.first()
         half = ref.EPS[kind] / 2
         for r, o in enumerate(on):
