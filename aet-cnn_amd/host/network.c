@@ -591,13 +591,19 @@ int an_add_dropout(an_network *net, float probability)
 }
 
 /* ======================================================================== */
+/* Training against a teacher whose answers, or whose labels, are not set: it is
+ * refused before anything runs that changes the network's state.           */
+static int teacher_missing(const an_network *net)
+{
+    return net->distilling &&
+           (!net->teacher_ready || (net->distill.hard != 0.f && !net->labelled));
+}
+
 /* Softmax + cross-entropy: SoftMaxLayer.c:99-119, :291-316.                */
 static int softmax_forward(an_network *net, an_layer *l, an_state st)
 {
     if (net->distilling && st.train && l->index == net->n - 1) {
         /* the output as ever; the loss and the delta against the teacher   */
-        if (!net->teacher_ready || (net->distill.hard != 0.f && !net->labelled))
-            return ACH_EINVAL;
         AN_CHECK(ach_softmax_xent(st.input, l->batch, l->inputs, l->groups, l->temperature, NULL,
                                   l->output, NULL, NULL, NULL, NULL, 0, net->stream));
         return ach_distill_xent(&net->distill_logits, &net->distill, st.input, net->teacher_ids,
@@ -1108,7 +1114,7 @@ static an_state base_state(an_network *net)
  * layer runs with state.input = previous output.                           */
 int an_forward(an_network *net, int train)
 {
-    if (!net || !net->finalized) return ACH_EINVAL;
+    if (!net || !net->finalized || (train && teacher_missing(net))) return ACH_EINVAL;
     an_state st = base_state(net);
     st.train = train;
     if (!train) st.truth = NULL; /* NNetwork.predict: state.truth = 0 */
@@ -1171,6 +1177,7 @@ int an_layer_forward(an_network *net, int i, int train)
 {
     an_layer *l = an_get_layer(net, i);
     if (!l || !net->finalized) return ACH_EINVAL;
+    if (train && i == net->n - 1 && teacher_missing(net)) return ACH_EINVAL;
     an_state st = base_state(net);
     st.train = train;
     st.index = i;
@@ -1392,7 +1399,7 @@ static int enqueue_step(an_network *net, int update, float rate)
  * the update at the policy's rate.                                        */
 int an_train_step(an_network *net)
 {
-    if (!net || !net->finalized) return ACH_EINVAL;
+    if (!net || !net->finalized || teacher_missing(net)) return ACH_EINVAL;
     net->dropout_step = (uint32_t)(net->seen / (uint64_t)net->batch);
     net->seen += (uint64_t)net->batch;
     const int update = (net->seen / (uint64_t)net->batch) % (uint64_t)net->subdivisions == 0;
@@ -1445,6 +1452,7 @@ int an_get_loss(an_network *net, float *loss)
 
 int an_train(an_network *net, const float *host_input, const float *host_truth, float *loss)
 {
+    if (!net || teacher_missing(net)) return ACH_EINVAL;
     AN_CHECK(an_set_input(net, host_input, host_truth));
     AN_CHECK(an_train_step(net));
     return an_get_loss(net, loss);

@@ -417,7 +417,8 @@ int an_end_distillation(an_network *net);
 /* The teacher's answers for the images of the next training steps: host
  * ids[batch][k] (negative: none) and values[batch][k], as an_predict_top gives
  * them, and labels[batch] (negative: none), which may be NULL if hard is 0.
- * A training step before they are set returns ACH_EINVAL.                  */
+ * A training step or forward before they are set returns ACH_EINVAL and leaves
+ * the network as it was.                                                   */
 int an_set_teacher(an_network *net, const int *ids, const float *values, const int *labels);
 int an_backward(an_network *net);
 int an_update(an_network *net);
