@@ -23,6 +23,7 @@
  * instead of the shared rand() stream, so the batches do not depend on
  * thread scheduling.                                                        */
 #include "aetcnn_net.h"
+#include "teacher.h"
 
 #include <pthread.h>
 #include <stdio.h>
@@ -403,6 +404,7 @@ int an_feeder_next(an_feeder *f)
     if (!rc) rc = ach_event_record(f->copied[s], f->copy_stream);
     if (!rc) rc = ach_stream_wait_event(ns, f->copied[s]);
     if (!rc) rc = an_set_input_device(f->net, f->dev_in[s], f->dev_truth[s]);
+    if (!rc) an_images_fed(f->net);
     if (!rc) rc = ach_event_sync(f->copied[s]);
     /* the device slot is reused two batches later, after the network stream
      * has consumed it: order later copies after this device-to-device move */

@@ -10,6 +10,7 @@
  * (mtcs/MtcsConvLayer.c:618-630).
  */
 #include "aetcnn_net.h"
+#include "teacher.h"
 
 #include <math.h>
 #include <stdio.h>
@@ -95,8 +96,9 @@ struct an_network {
     void *top_mem;
     /* an_set_distillation: the teacher's entries [batch][k], the labels
      * [batch] and the workspace, one allocation; teacher_ready once
-     * an_set_teacher has filled them (labelled: with labels)               */
-    int distilling, teacher_ready, labelled;
+     * an_set_teacher has filled them (labelled: with labels; teacher_used:
+     * a training forward has read them since)                              */
+    int distilling, teacher_ready, teacher_used, labelled;
     ach_logits_desc distill_logits;
     ach_distill_desc distill;
     void *teacher_mem;
@@ -604,6 +606,7 @@ static int softmax_forward(an_network *net, an_layer *l, an_state st)
 {
     if (net->distilling && st.train && l->index == net->n - 1) {
         /* the output as ever; the loss and the delta against the teacher   */
+        net->teacher_used = 1;
         AN_CHECK(ach_softmax_xent(st.input, l->batch, l->inputs, l->groups, l->temperature, NULL,
                                   l->output, NULL, NULL, NULL, NULL, 0, net->stream));
         return ach_distill_xent(&net->distill_logits, &net->distill, st.input, net->teacher_ids,
@@ -1373,7 +1376,13 @@ int an_set_teacher(an_network *net, const int *ids, const float *values, const i
         AN_CHECK(ach_memcpy_h2d(net->teacher_labels, labels, B * sizeof(int32_t), net->stream));
     net->labelled = labels != NULL;
     net->teacher_ready = 1;
+    net->teacher_used = 0;
     return ACH_OK;
+}
+
+void an_images_fed(an_network *net)
+{
+    if (net->teacher_used) net->teacher_ready = 0;
 }
 
 /* the kernels of one training step: forward, both backward streams and

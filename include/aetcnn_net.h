@@ -418,7 +418,9 @@ int an_end_distillation(an_network *net);
  * ids[batch][k] (negative: none) and values[batch][k], as an_predict_top gives
  * them, and labels[batch] (negative: none), which may be NULL if hard is 0.
  * A training step or forward before they are set returns ACH_EINVAL and leaves
- * the network as it was.                                                   */
+ * the network as it was.  an_feeder_next forgets answers that a step has used,
+ * as its images are others: set the new batch's before it, if they are known,
+ * or after it, from the images that an_input holds then.                   */
 int an_set_teacher(an_network *net, const int *ids, const float *values, const int *labels);
 int an_backward(an_network *net);
 int an_update(an_network *net);

@@ -1,4 +1,5 @@
-"""Training from a teacher: a step that is refused leaves the network as it was."""
+"""Training from a teacher: a step that is refused leaves the network as it was,
+and a feeder's new images need answers of their own."""
 import numpy as np
 import pytest
 
@@ -81,3 +82,50 @@ def test_inference_needs_no_teacher(gpu):
     net.forward(0)
     net.end_distillation()
     net.close()
+
+
+def fed(net):
+    """the images that the feeder has made the network's input"""
+    shape = (net.batch,) + tuple(net.shape(0)[4:7])
+    return aetcnn.DeviceArray.wrap(net.lib.an_input(net.h), shape).numpy(net.stream)
+
+
+def test_teacher_of_fed_images(gpu):
+    """A feeder's images, read back, are what the teacher answers for.  The next
+    batch needs answers of its own: a step with those that a step has used is
+    refused, and answers set before the batch is fetched, or after, are taken."""
+    net, twin, teacher = network(4), network(4), network(5)
+    feeder = aetcnn.Feeder(net, threads=2, seed=11)
+    for n in (net, twin):
+        n.set_distillation(4, aetcnn.DISTILL_TAIL, 2.0)
+    for step in range(4):
+        feeder.next()
+        x = fed(net)
+        if step:
+            before = state(net)
+            with pytest.raises(aetcnn.HipError, match=REFUSED):
+                net.train_step()
+            assert equal(state(net), before)
+        ids, lp, _ = teacher.predict_top(x, 4, 2.0)
+        twin.set_input(x, None)
+        for n in (net, twin):
+            n.set_teacher(ids, lp)
+            n.train_step()
+        assert net.loss() == twin.loss()
+        for i in range(net.n_layers()):
+            a, b = net.buffer(i, 2), twin.buffer(i, 2)
+            assert a is b is None or np.array_equal(a, b)
+    net.set_teacher(ids, lp)   # known beforehand
+    feeder.next()
+    net.train_step()
+    net.set_input(x, None)     # the caller's own batches: as the caller says
+    net.set_teacher(ids, lp)
+    net.train_step()
+    net.train_step()
+    net.end_distillation()     # the truth again
+    feeder.next()
+    net.train_step()
+    assert np.isfinite(net.loss())
+    feeder.close()
+    for n in (net, twin, teacher):
+        n.close()
