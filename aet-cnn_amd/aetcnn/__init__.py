@@ -28,7 +28,7 @@ ACH_ENAN = -5
 
 LOGISTIC, RELU, LINEAR, LEAKY = 0, 1, 3, 7
 
-F32, BF16, F16 = 0, 1, 2  # element types of logits
+F32, BF16, F16 = 0, 1, 2  # element types of logits, layer norm rows and checkpointed activations
 TOP_MAX = 128
 DISTILL_RENORM, DISTILL_TAIL = 0, 1
 
@@ -93,6 +93,21 @@ class LogitsDesc(C.Structure):
 class DistillDesc(C.Structure):
     """ach_distill_desc"""
     _fields_ = [("k", _i), ("mode", _i), ("teacher_type", _i), ("soft", _f), ("hard", _f)]
+
+
+class CheckpointDesc(C.Structure):
+    """ach_checkpoint_desc; stride 0 (the default) means features"""
+    _fields_ = [("rows", _i), ("features", _i), ("type", _i), ("stride", _i64)]
+
+
+class LayernormDesc(C.Structure):
+    """ach_layernorm_desc; stride 0 (the default) means features"""
+    _fields_ = [("rows", _i), ("features", _i), ("type", _i), ("eps", _f), ("stride", _i64)]
+
+
+class FcDesc(C.Structure):
+    """ach_fc_desc; stride 0 (the default) means outputs"""
+    _fields_ = [("rows", _i), ("inputs", _i), ("outputs", _i), ("type", _i), ("stride", _i64)]
 
 
 # name -> (restype, argtypes)
@@ -186,6 +201,17 @@ _OPS = {
     "ach_distill_workspace": (_sz, [C.POINTER(LogitsDesc), C.POINTER(DistillDesc)]),
     "ach_distill_xent": (_i, [C.POINTER(LogitsDesc), C.POINTER(DistillDesc), _vp, _vp, _vp, _vp,
                               _vp, _vp, _vp, _i64, _vp, _vp, _sz, _vp]),
+    "ach_checkpoint_bytes": (_sz, [_i, _i]),
+    "ach_checkpoint_pack": (_i, [C.POINTER(CheckpointDesc), _vp, _vp, _vp]),
+    "ach_checkpoint_unpack": (_i, [C.POINTER(CheckpointDesc), _vp, _vp, _vp]),
+    "ach_layernorm_fwd_workspace": (_sz, [C.POINTER(LayernormDesc)]),
+    "ach_layernorm_fwd": (_i, [C.POINTER(LayernormDesc), _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp,
+                               _sz, _vp]),
+    "ach_layernorm_bwd_workspace": (_sz, [C.POINTER(LayernormDesc)]),
+    "ach_layernorm_bwd": (_i, [C.POINTER(LayernormDesc), _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64,
+                               _vp, _vp, _i, _vp, _sz, _vp]),
+    "ach_fc_bwd_filter_checkpoint_workspace": (_sz, [C.POINTER(FcDesc)]),
+    "ach_fc_bwd_filter_checkpoint": (_i, [C.POINTER(FcDesc), _vp, _vp, _vp, _i, _vp, _sz, _vp]),
     "ach_dropout_uniform": (_f, [_u64, _u32, _u32, _u32]),
     "ach_dropout_fwd": (_i, [_vp, _sz, _f, _u64, _u32, _u32, _vp]),
     "ach_dropout_bwd": (_i, [_vp, _sz, _f, _u64, _u32, _u32, _vp]),

@@ -8,7 +8,7 @@
 // serve where rows are not too long, and one write.  A row belongs to one
 // workgroup, or, where there are too few rows to fill the chip, to several
 // whose partial results a second launch joins.
-#include "common.hpp"
+#include "rows.hpp"
 
 #include <float.h>
 #include <math.h>
@@ -17,30 +17,6 @@ namespace ach {
 namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-
-// An element type: 16 bytes of it as one load from any element's address.
-template <int TYPE> struct Elem;
-template <> struct Elem<ACH_F32> {
-    using T = float;
-};
-template <> struct Elem<ACH_BF16> {
-    using T = __bf16;
-};
-template <> struct Elem<ACH_F16> {
-    using T = _Float16;
-};
-template <int TYPE> struct Row {
-    using T = typename Elem<TYPE>::T;
-    static constexpr int VEC = 16 / sizeof(T);
-    typedef T Chunk __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
-    static __device__ __forceinline__ Chunk load(const T *p) { return *(const Chunk *)p; }
-    // PAST the caches: for gradients that these would not hold until they are read
-    template <bool PAST> static __device__ __forceinline__ void store(T *p, Chunk v)
-    {
-        if (PAST) __builtin_nontemporal_store(v, (Chunk *)p);
-        else *(Chunk *)p = v;
-    }
-};
 
 // The elements of a chunk one after the other, in a loop that is not unrolled:
 // what a workgroup does once per row costs more to fetch than to run.
@@ -103,45 +79,6 @@ struct Max {
     template <class V> __device__ V operator()(V a, V b) const { return a > b ? a : b; }
 };
 
-// The same for 32 bits without the LDS crossbar: within rows of 16 lanes by
-// shifts, then from row to row; lane 63 has seen all.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float dpp(float old, float v)
-{
-    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL,
-                                                      ROWS, 0xf, false));
-}
-__device__ __forceinline__ float lane_value(float v, int lane)
-{
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
-}
-__device__ __forceinline__ float wave_total(float v)
-{
-    v += dpp<0x111, 0xf>(0.f, v);
-    v += dpp<0x112, 0xf>(0.f, v);
-    v += dpp<0x114, 0xf>(0.f, v);
-    v += dpp<0x118, 0xf>(0.f, v);
-    v += dpp<0x142, 0xa>(0.f, v);
-    v += dpp<0x143, 0xc>(0.f, v);
-    return lane_value(v, 63);
-}
-template <int CTRL, int ROWS> __device__ __forceinline__ double dpp(double v)
-{
-    const uint64_t u = __double_as_longlong(v);
-    const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false),
-              hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
-    return __longlong_as_double((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
-}
-__device__ __forceinline__ double wave_total(double v)  // in lane 63 alone
-{
-    v += dpp<0x111, 0xf>(v);
-    v += dpp<0x112, 0xf>(v);
-    v += dpp<0x114, 0xf>(v);
-    v += dpp<0x118, 0xf>(v);
-    v += dpp<0x142, 0xa>(v);
-    v += dpp<0x143, 0xc>(v);
-    return v;
-}
 __device__ __forceinline__ float wave_most(float v)
 {
     v = fmaxf(v, dpp<0x111, 0xf>(v, v));
@@ -1528,10 +1465,6 @@ __global__ void __launch_bounds__(SUM_THREADS) k_sum_losses(const float *__restr
 }
 
 // ---- plans ---------------------------------------------------------------------------
-size_t elem_size(int type) { return type == ACH_F32 ? 4 : 2; }
-
-bool aligned(const void *p, size_t size) { return ((uintptr_t)p & (size - 1)) == 0; }
-
 // The descriptor with its stride filled in; false if it describes nothing.
 bool logits_desc(const ach_logits_desc *d, ach_logits_desc *out)
 {
@@ -1610,14 +1543,6 @@ size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 }  // namespace ach
 
 using namespace ach;
-
-// CALL(TYPE) for the element type of a descriptor
-#define FOR_TYPE(type, CALL)                                                                      \
-    do {                                                                                          \
-        if ((type) == ACH_F32) CALL(ACH_F32);                                                     \
-        else if ((type) == ACH_BF16) CALL(ACH_BF16);                                              \
-        else CALL(ACH_F16);                                                                       \
-    } while (0)
 
 extern "C" {
 

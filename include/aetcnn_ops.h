@@ -482,6 +482,105 @@ int ach_distill_xent(const ach_logits_desc *d, const ach_distill_desc *t, const 
                      int64_t delta_stride, float *cost, void *ws, size_t ws_bytes,
                      ach_stream_t stream);
 
+/* ---- activation checkpoints in 8 bits --------------------------------------
+ * No counterpart in the reference, whose layers keep every activation that
+ * their backward reads in 32 bits.
+ *
+ * `rows` rows of `features` (at most 2^30) values of `type` (ACH_F32, ACH_BF16
+ * or ACH_F16), row r at element r*stride (0: features; else >= features; what
+ * lies between the rows is neither read nor written), at any element address,
+ * are kept as one buffer of ach_checkpoint_bytes(), at an address that is a
+ * multiple of 16:
+ *   int8_t  codes[rows][F]      F: features rounded up to a multiple of 32
+ *   uint8_t steps[rows][F/32]   one for each block of 32 codes
+ * A value is code * 2^(step - 133): MXINT8 blocks of the OCP Microscaling
+ * Formats, without code -128 and steps below 7.  For a block whose largest
+ * magnitude is a, step is the smallest, from 7 to 254, with
+ * rint(a * 2^(133 - step)) <= 127, and the codes are the values rounded to
+ * nearest even, at most 2^(step - 134) off, that is a/127, and exact where a is
+ * 0.  (Codes end at 127 where a is above 127.5*2^121; values below 2^-127
+ * are 0.)  A block that holds a NaN or an infinity has step 255 and stands
+ * for NaN throughout.  Codes behind a row's last value are 0.
+ * ach_checkpoint_unpack writes the values, rounded to nearest even where the
+ * type is narrower than they are and no further than its largest finite value.
+ * rows may be 0.  A checkpoint overlaps neither x nor another tensor.       */
+typedef struct {
+    int rows, features;
+    int type;             /* of x                                            */
+    int64_t stride;       /* elements from one row of x to the next          */
+} ach_checkpoint_desc;
+/* 0 for a negative rows or features outside [1, 2^30]                      */
+size_t ach_checkpoint_bytes(int rows, int features);
+int ach_checkpoint_pack(const ach_checkpoint_desc *d, const void *x, void *checkpoint,
+                        ach_stream_t stream);
+int ach_checkpoint_unpack(const ach_checkpoint_desc *d, const void *checkpoint, void *x,
+                          ach_stream_t stream);
+
+/* ---- layer norm -------------------------------------------------------------
+ * No counterpart in the reference, which normalises over the batch only (the
+ * entry points above); the same roles: scales and biases per feature, the
+ * scales' and biases' gradients added into *_updates.
+ *
+ * Rows as of a checkpoint: an image's (or a token's) features, normalised
+ * among themselves.  eps from 1e-12 to 1.  Everything is computed in 32 bits
+ * or more and rounded once where an output has fewer; results do not depend
+ * on the run (no float atomics).  A row that holds a NaN or an infinity (or
+ * whose values differ by more than the largest float) gives NaN in all its
+ * outputs, statistics that are not finite, and NaN in the updates; other rows
+ * are not touched by it.  Workspaces are aligned to 16 bytes and belong to one
+ * call at a time.  Outputs overlap neither one another nor the inputs, but
+ * for what is said below.  rows may be 0.                                  */
+typedef struct {
+    int rows, features;
+    int type;             /* of x, y, delta and dx                           */
+    float eps;
+    int64_t stride;       /* elements from one row of x to the next          */
+} ach_layernorm_desc;
+/* mean = sum x / n, rstd = 1/sqrt(sum (x - mean)^2 / n + eps),
+ * x_norm = (x - mean)*rstd, y = x_norm*scales + biases (float [features];
+ * NULL: 1 and 0).  y has rows y_stride apart (0: features) and may be x itself
+ * with the same stride.  Either of y, stats (float [rows][2], mean and rstd)
+ * and checkpoint (x_norm in 8 bits, from the unrounded values) may be NULL,
+ * not all three.                                                           */
+size_t ach_layernorm_fwd_workspace(const ach_layernorm_desc *d);
+int ach_layernorm_fwd(const ach_layernorm_desc *d, const void *x, const float *scales,
+                      const float *biases, void *y, int64_t y_stride, float *stats,
+                      void *checkpoint, void *ws, size_t ws_bytes, ach_stream_t stream);
+/* From the stats and either x or the checkpoint of x_norm (the other NULL):
+ *   g = delta*scales;  dx = rstd*(g - sum g / n - x_norm * sum(g*x_norm) / n)
+ *   scale_updates[j] (+)= sum_r delta*x_norm;  bias_updates[j] (+)= sum_r delta
+ * added to what is there with accumulate 1 (as ach_bn_bwd's), or replacing it
+ * with accumulate 0 (rows 0 then gives zeros).  delta and dx have rows
+ * delta_stride and dx_stride apart (0: features); dx may be delta itself with
+ * the same stride.  dx, scale_updates and bias_updates may be NULL, not all
+ * three; scales NULL: 1.                                                   */
+size_t ach_layernorm_bwd_workspace(const ach_layernorm_desc *d);
+int ach_layernorm_bwd(const ach_layernorm_desc *d, const void *delta, int64_t delta_stride,
+                      const void *x, const void *checkpoint, const float *stats,
+                      const float *scales, void *dx, int64_t dx_stride, float *scale_updates,
+                      float *bias_updates, int accumulate, void *ws, size_t ws_bytes,
+                      ach_stream_t stream);
+
+/* ---- a fully connected layer's weight gradient from its input's checkpoint --
+ * ach_conv_bwd_filter of a fully connected geometry with the input kept in 8
+ * bits: dw[o][i] (+)= sum_r delta[r][o]*x[r][i], dw float [outputs][inputs]
+ * without gaps, x the checkpoint of rows x inputs (inputs at most 2^30), delta
+ * rows of `outputs` values of `type`, `stride` elements apart (0: outputs), at
+ * any element address.  accumulate as above (rows 0 and accumulate 0: zeros).
+ * Every product is exact and the sums are in 32 bits: an fp32 delta is taken as
+ * three bf16 pieces (fp16: two), of which parts below 2^-126 are lost.  An
+ * infinity or a NaN in delta or a block of NaN in x reaches all that it is
+ * summed into; results do not depend on the run.                           */
+typedef struct {
+    int rows, inputs, outputs;
+    int type;             /* of delta                                        */
+    int64_t stride;       /* elements from one row of delta to the next      */
+} ach_fc_desc;
+size_t ach_fc_bwd_filter_checkpoint_workspace(const ach_fc_desc *d);
+int ach_fc_bwd_filter_checkpoint(const ach_fc_desc *d, const void *checkpoint, const void *delta,
+                                 float *dw, int accumulate, void *ws, size_t ws_bytes,
+                                 ach_stream_t stream);
+
 /* ---- dropout (DropoutLayer.c:55-86) ---------------------------------------
  * r = u(seed, iter, layer, i) from a counter-based generator (SplitMix64
  * finaliser, top 24 bits); r < p -> 0 else x * 1/(1-p).  Same mask forward
