@@ -41,7 +41,7 @@ k_checkpoint(typename Elem<TYPE>::T *x, int64_t stride, int features, int n, Fas
 bool checkpoint_desc(const ach_checkpoint_desc *d, ach_checkpoint_desc *out)
 {
     if (!d || d->rows < 0 || d->features < 1 || d->features > KEPT_MOST || d->stride < 0) return false;
-    if (!elem_type(d->type)) return false;
+    if (d->rows > KEPT_MOST || !elem_type(d->type)) return false;
     *out = *d;
     if (out->stride == 0) out->stride = d->features;
     return out->stride >= d->features;
@@ -93,7 +93,7 @@ extern "C" {
 
 size_t ach_checkpoint_bytes(int rows, int features)
 {
-    if (rows < 0 || features < 1 || features > KEPT_MOST) return 0;
+    if (rows < 0 || rows > KEPT_MOST || features < 1 || features > KEPT_MOST) return 0;
     const size_t blocks = ((size_t)features + KEPT_BLOCK - 1) / KEPT_BLOCK;
     return (size_t)rows * blocks * (KEPT_BLOCK + 1);
 }

@@ -22,7 +22,7 @@ inline Kept kept(const void *checkpoint, int rows, int features)
     k.steps = (uint8_t *)(k.codes + (size_t)rows * k.width);
     return k;
 }
-constexpr int KEPT_MOST = 1 << 30;  // features
+constexpr int KEPT_MOST = 1 << 30;  // rows and features
 
 // The step of a block from the bits of its largest magnitude a: the biased
 // exponent of a, whose power of two is 64 steps, or one more where a is 127.5

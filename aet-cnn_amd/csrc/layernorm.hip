@@ -208,7 +208,7 @@ k_norm_bwd_join(const float *part, int spans, int features, float *scale_updates
 bool layernorm_desc(const ach_layernorm_desc *d, ach_layernorm_desc *out)
 {
     if (!d || d->rows < 0 || d->features < 1 || d->features > KEPT_MOST || d->stride < 0) return false;
-    if (!elem_type(d->type) || !(d->eps >= 1e-12f && d->eps <= 1.f)) return false;
+    if (d->rows > KEPT_MOST || !elem_type(d->type) || !(d->eps >= 1e-12f && d->eps <= 1.f)) return false;
     *out = *d;
     if (out->stride == 0) out->stride = d->features;
     return out->stride >= d->features;

@@ -486,7 +486,7 @@ int ach_distill_xent(const ach_logits_desc *d, const ach_distill_desc *t, const 
  * No counterpart in the reference, whose layers keep every activation that
  * their backward reads in 32 bits.
  *
- * `rows` rows of `features` (at most 2^30) values of `type` (ACH_F32, ACH_BF16
+ * `rows` (0 to 2^30) rows of `features` (1 to 2^30) values of `type` (ACH_F32, ACH_BF16
  * or ACH_F16), row r at element r*stride (0: features; else >= features; what
  * lies between the rows is neither read nor written), at any element address,
  * are kept as one buffer of ach_checkpoint_bytes(), at an address that is a
@@ -503,13 +503,13 @@ int ach_distill_xent(const ach_logits_desc *d, const ach_distill_desc *t, const 
  * for NaN throughout.  Codes behind a row's last value are 0.
  * ach_checkpoint_unpack writes the values, rounded to nearest even where the
  * type is narrower than they are and no further than its largest finite value.
- * rows may be 0.  A checkpoint overlaps neither x nor another tensor.       */
+ * A checkpoint overlaps neither x nor another tensor.                        */
 typedef struct {
     int rows, features;
     int type;             /* of x                                            */
     int64_t stride;       /* elements from one row of x to the next          */
 } ach_checkpoint_desc;
-/* 0 for a negative rows or features outside [1, 2^30]                      */
+/* 0 for rows or features outside these ranges                              */
 size_t ach_checkpoint_bytes(int rows, int features);
 int ach_checkpoint_pack(const ach_checkpoint_desc *d, const void *x, void *checkpoint,
                         ach_stream_t stream);
@@ -529,7 +529,7 @@ int ach_checkpoint_unpack(const ach_checkpoint_desc *d, const void *checkpoint, 
  * outputs, statistics that are not finite, and NaN in the updates; other rows
  * are not touched by it.  Workspaces are aligned to 16 bytes and belong to one
  * call at a time.  Outputs overlap neither one another nor the inputs, but
- * for what is said below.  rows may be 0.                                  */
+ * for what is said below.                                                  */
 typedef struct {
     int rows, features;
     int type;             /* of x, y, delta and dx                           */
@@ -564,13 +564,13 @@ int ach_layernorm_bwd(const ach_layernorm_desc *d, const void *delta, int64_t de
 /* ---- a fully connected layer's weight gradient from its input's checkpoint --
  * ach_conv_bwd_filter of a fully connected geometry with the input kept in 8
  * bits: dw[o][i] (+)= sum_r delta[r][o]*x[r][i], dw float [outputs][inputs]
- * without gaps, x the checkpoint of rows x inputs (inputs at most 2^30), delta
+ * without gaps, x the checkpoint of rows x inputs (each at most 2^30), delta
  * rows of `outputs` values of `type`, `stride` elements apart (0: outputs), at
  * any element address.  accumulate as above (rows 0 and accumulate 0: zeros).
  * Every product is exact and the sums are in 32 bits: an fp32 delta is taken as
- * three bf16 pieces (fp16: two), of which parts below 2^-126 are lost.  An
- * infinity or a NaN in delta or a block of NaN in x reaches all that it is
- * summed into; results do not depend on the run.                           */
+ * three bf16 pieces (fp16: two), of which parts below 2^-126 are lost.  What an
+ * infinity or a NaN in delta, or a block of NaN in x, is summed into is not
+ * finite; results do not depend on the run.                                */
 typedef struct {
     int rows, inputs, outputs;
     int type;             /* of delta                                        */

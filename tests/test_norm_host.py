@@ -39,7 +39,8 @@ NAN, INF = float("nan"), float("inf")
 
 @pytest.mark.parametrize("d", [
     LayernormDesc(-1, 10, F32, 1e-5), LayernormDesc(2, 0, F32, 1e-5), LayernormDesc(2, -1, F32, 1e-5),
-    LayernormDesc(2, (1 << 30) + 1, F32, 1e-5), LayernormDesc(2, 10, 3, 1e-5),
+    LayernormDesc(2, (1 << 30) + 1, F32, 1e-5), LayernormDesc((1 << 30) + 1, 2, F32, 1e-5),
+    LayernormDesc(2, 10, 3, 1e-5),
     LayernormDesc(2, 10, -1, 1e-5), LayernormDesc(2, 10, F32, 0.0), LayernormDesc(2, 10, F32, -1.0),
     LayernormDesc(2, 10, F32, 1e-13), LayernormDesc(2, 10, F32, 2.0), LayernormDesc(2, 10, F32, NAN),
     LayernormDesc(2, 10, F32, INF), LayernormDesc(2, 10, F32, 1e-5, 9),
@@ -81,6 +82,7 @@ def test_layernorm_refusals():
 
 @pytest.mark.parametrize("d", [
     CheckpointDesc(-1, 10, F32), CheckpointDesc(2, 0, F32), CheckpointDesc(2, (1 << 30) + 1, F32),
+    CheckpointDesc((1 << 30) + 1, 2, F32),
     CheckpointDesc(2, 10, 3), CheckpointDesc(2, 10, -1), CheckpointDesc(2, 10, F32, 9),
     CheckpointDesc(2, 10, F32, -10), None])
 def test_bad_checkpoint_descriptors(d):
@@ -100,14 +102,14 @@ def test_checkpoint_refusals_and_sizes():
     assert ops.ach_checkpoint_pack(at(CheckpointDesc(0, 10, F32)), MEM, 2 * MEM, None) == 0  # no rows
     size = ops.ach_checkpoint_bytes
     assert size(3, 1) == size(3, 32) == 3 * 33 and size(3, 33) == 3 * 66 and size(0, 5) == 0
-    assert size(-1, 5) == size(1, 0) == size(1, -4) == size(1, (1 << 30) + 1) == 0
+    assert size(-1, 5) == size(1, 0) == size(1, -4) == size(1, (1 << 30) + 1) == size((1 << 30) + 1, 1) == 0
     assert size(100000, 1 << 30) == 100000 * (1 << 30) // 32 * 33  # past 32 bits
 
 
 @pytest.mark.parametrize("d", [
     FcDesc(-1, 10, 10, F32), FcDesc(2, 0, 10, F32), FcDesc(2, 10, 0, F32), FcDesc(2, 10, 10, 3),
     FcDesc(2, 10, 10, -1), FcDesc(2, 10, 10, F32, 9), FcDesc(2, 10, 10, F32, -10),
-    FcDesc(2, (1 << 30) + 1, 10, F32), None])
+    FcDesc(2, (1 << 30) + 1, 10, F32), FcDesc((1 << 30) + 1, 10, 10, F32), None])
 def test_bad_fc_descriptors(d):
     ops = aetcnn.ops()
     assert fc(ops, d) == ACH_EINVAL
