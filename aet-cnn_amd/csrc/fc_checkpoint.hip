@@ -5,20 +5,21 @@
 // delta (its first 8 bits, the next 8, the last 8; one piece for bf16, two for
 // fp16, three for fp32): every product is exact and is summed in fp32.
 //
-// Tiles of 128 outputs x 128 inputs, a wave 64 x 64 of it.  A stage of 32 rows
-// of both operands is loaded two stages ahead, turned into bf16 and stored as it
-// lies in memory, [row][128]; the matrix instructions want 8 rows of a column in
-// a lane, which the transposing LDS loads give: 16 lanes read 4 rows x 16
-// columns, and each gets a column of it.
+// Eight waves of 64 outputs x 64 inputs each, as a tile of 256 x 128 or 128 x
+// 256.  A stage of 32 rows of both operands is loaded two stages ahead, turned
+// into bf16 and stored as it lies in memory, [row][column]; the matrix
+// instructions want 8 rows of a column in a lane, which the transposing LDS loads
+// give: 16 lanes read 4 rows x 16 columns, and each gets a column of it.
 #include "checkpoint.hpp"
 #include "pieces.hpp"
 
 namespace ach {
 namespace {
 
-constexpr int TILE = 128, DEPTH = 32;
-constexpr int PITCH = TILE + 32;  // 16-bit values of an LDS row
+constexpr int DEPTH = 32;  // rows of a stage
+constexpr int RING = 2;    // stages in flight, an even number
 constexpr int MOST_SLICES = 64;
+constexpr int MOST_COLUMNS = 1 << 23;  // inputs, outputs, stride: a stage's offsets fit 31 bits
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
@@ -47,43 +48,71 @@ __device__ __forceinline__ float below(float x)  // what they leave
     return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u);
 }
 
-// Eight values of a delta as pieces whose sum they are.
+// Eight values of a delta, and the pieces whose sum they are.
 template <int TYPE> struct Eight {
-    using T = typename Elem<TYPE>::T;
-    float f[8];
-    __device__ __forceinline__ void load(const T *p, int left)
+    static constexpr int N = TYPE == ACH_F32 ? 2 : 1;  // loads of 16 bytes
+    v4u w[N];
+    // moves 16-bit value i + by to value i, for a chunk that was loaded `by` early
+    __device__ __forceinline__ void shift(int by)
     {
-        if (left >= 8) {
-            const typename Row<TYPE>::Chunk a = Row<TYPE>::load(p);
+        v4u u = w[0];
 #pragma unroll
-            for (int i = 0; i < Row<TYPE>::VEC; ++i) f[i] = (float)a[i];
-            if constexpr (TYPE == ACH_F32) {
-                const typename Row<TYPE>::Chunk b = Row<TYPE>::load(p + 4);
+        for (int i = 0; i < 4; ++i) u[i] = by & 4 ? u[(i + 2) & 3] : u[i];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) f[4 + i] = b[i];
-            }
-        } else {
+        for (int i = 0; i < 4; ++i) u[i] = by & 2 ? u[(i + 1) & 3] : u[i];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = i < left ? (float)p[i] : 0.f;
-        }
+        for (int i = 0; i < 4; ++i) u[i] = by & 1 ? u[i] >> 16 | u[(i + 1) & 3] << 16 : u[i];
+        w[0] = u;
     }
-    __device__ __forceinline__ void split(v4u *p)
+    __device__ __forceinline__ void split(v4u *p) const
     {
+        if constexpr (TYPE == ACH_BF16) {
+            p[0] = w[0];
+        } else {
+            float f[8];
+            if constexpr (TYPE == ACH_F32) {
+                __builtin_memcpy(f, w, sizeof(f));
+            } else {
+                _Float16 h[8];
+                __builtin_memcpy(h, w, sizeof(h));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float a = f[2 * i], b = f[2 * i + 1];
+                for (int i = 0; i < 8; ++i) f[i] = (float)h[i];
+            }
 #pragma unroll
-            for (int q = 0; q < Pieces<TYPE>::N; ++q) {
-                p[q][i] = upper_halves(a, b);
-                a = below(a), b = below(b);
+            for (int i = 0; i < 4; ++i) {
+                float a = f[2 * i], b = f[2 * i + 1];
+#pragma unroll
+                for (int q = 0; q < Pieces<TYPE>::N; ++q) {
+                    p[q][i] = upper_halves(a, b);
+                    a = below(a), b = below(b);
+                }
             }
         }
     }
 };
 
-// Eight columns of a tile in LDS as a lane's operand of a 16-row step: `p` is
-// the lane's own place in the first four rows.
-__device__ __forceinline__ v8bf fragment(const short *p)
+// A window of DEPTH rows on a matrix, moved from stage to stage; what lies behind
+// the last byte reads as 0.
+struct Window {
+    const char *p;
+    int64_t left, step;
+    __device__ __forceinline__ Window(const void *base, int64_t pitch, int64_t row_bytes, int r, int end)
+        : p((const char *)base + r * pitch), left((end - r) * pitch - (pitch - row_bytes)),
+          step(DEPTH * pitch)
+    {
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t next()
+    {
+        const __amdgpu_buffer_rsrc_t w =
+            make_rsrc(p, (unsigned)max(min(left, (int64_t)0x7fffffff), (int64_t)0));
+        p += step, left -= step;
+        return w;
+    }
+};
+
+// Eight columns' rows of a tile in LDS as a lane's operand of a 16-row step: `p`
+// is the lane's own place in the first four rows.
+template <int PITCH> __device__ __forceinline__ v8bf fragment(const short *p)
 {
     typedef __attribute__((address_space(3))) v4s *Lds;
     const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)p),
@@ -92,96 +121,141 @@ __device__ __forceinline__ v8bf fragment(const short *p)
     return __builtin_bit_cast(v8bf, v);
 }
 
-template <int TYPE>
-__global__ void __launch_bounds__(256, 2) k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
+enum { WHOLE, EARLY, SINGLE };
+template <int W> struct How {
+    static constexpr int value = W;
+};
+
+// WO x WI waves of 32 MO outputs x 64 inputs
+template <int TYPE, int WO, int WI, int MO> struct Tile {
+    static constexpr int THREADS = 64 * WO * WI;
+    static constexpr int O = 32 * MO * WO, I = 64 * WI;
+    static constexpr int OP = O + 32, IP = I + 32;  // 16-bit values of an LDS row
+    struct Stage {
+        short d[Pieces<TYPE>::N][DEPTH * OP], x[DEPTH * IP];
+    };
+    static constexpr size_t LDS = 2 * sizeof(Stage);
+};
+
+template <int TYPE, int WO, int WI, int MO, int LEAST>
+__global__ void __launch_bounds__(64 * WO * WI, LEAST)
+k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
 {
-    constexpr int P = Pieces<TYPE>::N;
-    __shared__ __align__(16) short sm[2][P + 1][DEPTH * PITCH];  // pieces of delta, then x
+    using S = Tile<TYPE, WO, WI, MO>;
+    constexpr int P = Pieces<TYPE>::N, SIZE = sizeof(typename Elem<TYPE>::T);
+    constexpr int XC = DEPTH * S::I / S::THREADS;        // codes of a thread's load: 8 or 16
+    constexpr int DN = DEPTH * S::O / S::THREADS / 8;    // chunks of 8 values of delta
+    constexpr int DR = S::THREADS / (S::O / 8);          // rows apart
+    extern __shared__ __align__(16) char smem[];
+    typename S::Stage *const stage = reinterpret_cast<typename S::Stage *>(smem);
     const int tid = (int)threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wo = wave & 1, wi = wave >> 1;
+    const int wo = wave % WO, wi = wave / WO;
     // each XCD, which takes every eighth workgroup, gets a contiguous range of
-    // tiles, in groups of 8 outputs' tiles: they share the operands in its L2
+    // tiles, in blocks of 8 outputs' tiles: they share the operands in its L2
     int id = blockIdx.x;
     {
         const int G = gridDim.x, g8 = G >> 3, r8 = G & 7, xcd = id & 7;
         id = xcd * g8 + min(xcd, r8) + (id >> 3);
     }
-    const int group = id / (8 * a.ti), in = id - group * 8 * a.ti;
-    const int high = min(8, a.to - group * 8);
-    const int o0 = (group * 8 + in % high) * TILE, i0 = in / high * TILE;
+    const int block = id / (8 * a.ti), in = id - block * 8 * a.ti;
+    const int high = min(8, a.to - block * 8);
+    const int o0 = (block * 8 + in % high) * S::O, i0 = in / high * S::I;
     const int r0 = (int)blockIdx.y * a.span, r1 = min((int64_t)a.rows, (int64_t)r0 + a.span);
 
-    // a thread's share of a stage: 16 codes of one row; 8 values of two rows
-    const int xr = tid >> 3, xc = (tid & 7) * 16, dr = tid >> 4, dc = (tid & 15) * 8;
-    const bool x_in = i0 + xc < a.k.width;
-    const int d_left = a.outputs - (o0 + dc);
-    v4u codes;
-    uint32_t step;
-    Eight<TYPE> d[2];
-    auto load = [&](int r) {
-        codes = 0;
-        step = 7;
-        if (r + xr < r1 && x_in) {
-            const size_t at = (size_t)(r + xr) * a.k.width + i0 + xc;
-            codes = *(const v4u *)(a.k.codes + at);
-            step = a.k.steps[at / KEPT_BLOCK];
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            d[h].load(delta + (r + dr + 16 * h) * a.stride + o0 + dc, r + dr + 16 * h < r1 ? d_left : 0);
+    // A thread's share of a stage.  What lies behind the last output or input is
+    // never stored, so any values will do there: loads that pass a row's end read
+    // the next row, or zeros behind the last one.  The range check is by dwords,
+    // so 16-bit values, which would lose the last one of an odd number, are
+    // loaded whole chunks inside a row instead, early and then shifted (EARLY),
+    // or one by one (SINGLE, under 8 outputs).
+    const int xr = tid / (S::I / XC), xc = tid % (S::I / XC) * XC;
+    const int dr = tid / (S::O / 8), dc = tid % (S::O / 8) * 8;
+    const int x_col = min(i0 + xc, a.k.width - XC);
+    const int x_at = xr * a.k.width + x_col, s_at = (xr * a.k.width + x_col) / KEPT_BLOCK;
+    const int64_t pitch = a.stride * SIZE;
+    struct Load {
+        uint32_t codes[XC / 4], step;
+        Eight<TYPE> d[DN];
     };
-    auto store = [&](int s) {
-        const float scale = kept_scale(step);
-        v4u w[2];
+    Window codes(a.k.codes, a.k.width, a.k.width, r0, r1),
+        steps(a.k.steps, a.k.width / KEPT_BLOCK, a.k.width / KEPT_BLOCK, r0, r1),
+        deltas(delta, pitch, (int64_t)a.outputs * SIZE, r0, r1);
+    auto load = [&](Load &g, const int *d_at, auto how) {
+        const __amdgpu_buffer_rsrc_t c = codes.next(), t = steps.next(), d = deltas.next();
+        if constexpr (XC == 16) {
+            const auto v = __builtin_amdgcn_raw_buffer_load_b128(c, x_at, 0, 0);
+            __builtin_memcpy(g.codes, &v, 16);
+        } else {
+            const auto v = __builtin_amdgcn_raw_buffer_load_b64(c, x_at, 0, 0);
+            __builtin_memcpy(g.codes, &v, 8);
+        }
+        g.step = __builtin_amdgcn_raw_buffer_load_b8(t, s_at, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int h = 0; h < DN; ++h) {
+            if constexpr (decltype(how)::value == SINGLE) {
+                uint16_t v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = __builtin_amdgcn_raw_buffer_load_b16(d, d_at[h] + 2 * i, 0, 0);
+                __builtin_memcpy(g.d[h].w, v, sizeof(v));
+            } else {
+#pragma unroll
+                for (int i = 0; i < Eight<TYPE>::N; ++i) {
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(d, d_at[h] + 16 * i, 0, 0);
+                    __builtin_memcpy(&g.d[h].w[i], &v, 16);
+                }
+            }
+        }
+    };
+    auto store = [&](Load &g, int s, int late, auto how) {
+        const float scale = kept_scale(g.step);
+        uint32_t w[XC / 2];
+#pragma unroll
+        for (int i = 0; i < XC / 4; ++i) {
             float f[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) f[b] = (float)(int8_t)(codes[i] >> (8 * b)) * scale;
-            w[i / 2][i % 2 * 2] = upper_halves(f[0], f[1]);
-            w[i / 2][i % 2 * 2 + 1] = upper_halves(f[2], f[3]);
+            for (int b = 0; b < 4; ++b) f[b] = (float)(int8_t)(g.codes[i] >> (8 * b)) * scale;
+            w[2 * i] = upper_halves(f[0], f[1]);
+            w[2 * i + 1] = upper_halves(f[2], f[3]);
         }
-        short *const to = &sm[s][P][xr * PITCH + xc];
-        *(v4u *)to = w[0];
-        *(v4u *)(to + 8) = w[1];
+        short *const to = &stage[s].x[xr * S::IP + xc];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int i = 0; i < XC / 8; ++i) *(v4u *)(to + 8 * i) = *(v4u *)(w + 4 * i);
+#pragma unroll
+        for (int h = 0; h < DN; ++h) {
             v4u p[P];
-            d[h].split(p);
+            if constexpr (decltype(how)::value == EARLY) g.d[h].shift(late);
+            g.d[h].split(p);
 #pragma unroll
-            for (int q = 0; q < P; ++q) *(v4u *)&sm[s][q][(dr + 16 * h) * PITCH + dc] = p[q];
+            for (int q = 0; q < P; ++q) *(v4u *)&stage[s].d[q][(dr + h * DR) * S::OP + dc] = p[q];
         }
     };
 
-    v16f hi[2][2], lo[2][2];
+    v16f hi[MO][2], lo[P > 1 ? MO : 1][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MO; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) hi[i][j][e] = lo[i][j][e] = 0.f;
+            for (int e = 0; e < 16; ++e) hi[i][j][e] = lo[P > 1 ? i : 0][j][e] = 0.f;
 
-    // a lane's place: rows 8 * (lane / 32) + lane % 16 / 4, columns 16 * (lane / 16 % 2) + 4 * (lane % 4)
-    const int place = (8 * (lane >> 5) + ((lane & 15) >> 2)) * PITCH + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-    load(r0);
-    store(0);
-    load(r0 + DEPTH);
-    __syncthreads();
-    int s = 0;
-    for (int r = r0; r < r1; r += DEPTH, s ^= 1) {
+    // a lane's place in a 16-row step: row 8 * (lane / 32) + lane % 16 / 4, column
+    // 16 * (lane / 16 % 2) + 4 * (lane % 4)
+    const int row = 8 * (lane >> 5) + ((lane & 15) >> 2), column = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+    const int d_place = row * S::OP + wo * 32 * MO + column, x_place = row * S::IP + wi * 64 + column;
+    auto multiply = [&](int s) {
 #pragma unroll
-        for (int step16 = 0; step16 < DEPTH / 16; ++step16) {
+        for (int step = 0; step < DEPTH; step += 16) {
             v8bf x[2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                x[j] = fragment(&sm[s][P][place + step16 * 16 * PITCH + wi * 64 + j * 32]);
+            for (int j = 0; j < 2; ++j) x[j] = fragment<S::IP>(&stage[s].x[x_place + step * S::IP + j * 32]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < MO; ++i) {
                 v8bf p[P];
 #pragma unroll
                 for (int q = 0; q < P; ++q)
-                    p[q] = fragment(&sm[s][q][place + step16 * 16 * PITCH + wo * 64 + i * 32]);
+                    p[q] = fragment<S::OP>(&stage[s].d[q][d_place + step * S::OP + i * 32]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     hi[i][j] = MFMA_BF(p[0], x[j], hi[i][j]);
@@ -190,24 +264,50 @@ __global__ void __launch_bounds__(256, 2) k_fc_wgrad(const typename Elem<TYPE>::
                 }
             }
         }
-        store(s ^ 1);  // (past the last stage: zeros, which nothing reads)
-        load(r + 2 * DEPTH);
+    };
+    auto all = [&](auto how) {
+        const int start = decltype(how)::value == EARLY ? min(o0 + dc, a.outputs - 8) : o0 + dc;
+        const int late = min(o0 + dc - start, 7);
+        int d_at[DN];
+#pragma unroll
+        for (int h = 0; h < DN; ++h) d_at[h] = (dr + h * DR) * (int)pitch + start * SIZE;
+        Load ring[RING];
+#pragma unroll
+        for (int u = 0; u < RING; ++u) load(ring[u], d_at, how);
+        store(ring[0], 0, late, how);
+        load(ring[0], d_at, how);
         __syncthreads();
-    }
+        // whole turns of the ring (stages behind the last row are zeros)
+        for (int r = r0; r < r1; r += RING * DEPTH) {
+#pragma unroll
+            for (int u = 1; u <= RING; ++u) {
+                __builtin_amdgcn_iglp_opt(0);  // operand loads among the matrix instructions
+                multiply((u + 1) % 2);
+                store(ring[u % RING], u % 2, late, how);
+                load(ring[u % RING], d_at, how);
+                __syncthreads();
+            }
+        }
+    };
+    if (SIZE == 4) all(How<WHOLE>());
+    else if (a.outputs < 8) all(How<SINGLE>());
+    else if (a.outputs % 8 && o0 + S::O > a.outputs) all(How<EARLY>());
+    else all(How<WHOLE>());
+
     float *const out = a.part ? a.part + (size_t)blockIdx.y * a.outputs * a.inputs : a.dw;
     const bool add = a.accumulate && !a.part;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MO; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int o = o0 + wo * 64 + i * 32 + 4 * (lane >> 5), c = i0 + wi * 64 + j * 32 + (lane & 31);
+            const int o = o0 + (wo * MO + i) * 32 + 4 * (lane >> 5), c = i0 + wi * 64 + j * 32 + (lane & 31);
             if (c >= a.inputs) continue;
             float *const p = out + (size_t)o * a.inputs + c;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int r = 8 * (e >> 2) + (e & 3);
                 if (o + r >= a.outputs) continue;
-                float v = hi[i][j][e] + lo[i][j][e];
+                float v = P > 1 ? hi[i][j][e] + lo[P > 1 ? i : 0][j][e] : hi[i][j][e];
                 if (add) v += p[(size_t)r * a.inputs];
                 p[(size_t)r * a.inputs] = v;
             }
@@ -226,37 +326,58 @@ k_fc_wgrad_join(const float *part, size_t n, int slices, float *dw, int accumula
 
 bool fc_desc(const ach_fc_desc *d, ach_fc_desc *out)
 {
-    if (!d || d->rows < 0 || d->inputs < 1 || d->inputs > KEPT_MOST || d->outputs < 1) return false;
-    if (d->rows > KEPT_MOST) return false;
+    if (!d || d->rows < 0 || d->inputs < 1 || d->outputs < 1) return false;
+    if (d->rows > KEPT_MOST || d->inputs > MOST_COLUMNS || d->outputs > MOST_COLUMNS) return false;
     if (!elem_type(d->type) || d->stride < 0) return false;
     *out = *d;
     if (out->stride == 0) out->stride = d->outputs;
-    return out->stride >= d->outputs;
+    return out->stride >= d->outputs && out->stride <= MOST_COLUMNS;
 }
 
-// Slices of the rows, so that two workgroups a compute unit run, of at least
-// four stages each.
 struct Plan {
+    bool high;  // tiles of 256 outputs x 128 inputs, else 128 x 256
     int ti, to, span, slices;
     size_t bytes;
 };
 
+int tiles_of(int n, int tile) { return (n + tile - 1) / tile; }
+
 Plan fc_plan(const ach_fc_desc &d)
 {
     Plan p;
-    p.ti = (int)(((int64_t)d.inputs + TILE - 1) / TILE);
-    p.to = (int)(((int64_t)d.outputs + TILE - 1) / TILE);
+    const int64_t high = (int64_t)tiles_of(d.outputs, 256) * tiles_of(d.inputs, 128),
+                  wide = (int64_t)tiles_of(d.outputs, 128) * tiles_of(d.inputs, 256);
+    p.high = high < wide || (high == wide && d.type == ACH_BF16);
+    p.to = tiles_of(d.outputs, p.high ? 256 : 128);
+    p.ti = tiles_of(d.inputs, p.high ? 128 : 256);
     const int64_t tiles = (int64_t)p.ti * p.to;
-    int slices = tiles < 512 ? (int)((511 + tiles) / tiles) : 1;
-    const int stages = d.rows / DEPTH + (d.rows % DEPTH != 0);
+    const int stages = tiles_of(d.rows, DEPTH);
+    const int full = d.type == ACH_BF16 && p.high ? 512 : 256;  // workgroups that run at once
+    int slices = tiles < full ? (int)(full / tiles) : 1;
     if (slices > stages / 4) slices = stages / 4;
     if (slices > MOST_SLICES) slices = MOST_SLICES;
     if (slices < 1) slices = 1;
-    const int each = (stages + slices - 1) / slices;
-    p.slices = each ? (stages + each - 1) / each : 1;
-    p.span = each < 0x7fffffff / DEPTH ? each * DEPTH : 0x7fffffff;
+    int each = tiles_of(stages, slices);
+    each += each % RING;  // whole turns
+    p.slices = each ? tiles_of(stages, each) : 1;
+    p.span = each * DEPTH;
     p.bytes = p.slices > 1 ? (size_t)p.slices * d.outputs * d.inputs * sizeof(float) : 0;
     return p;
+}
+
+template <int TYPE, int WO, int WI, int MO, int LEAST>
+int fc_go(const Plan &p, const void *delta, const Fc &a, hipStream_t st)
+{
+    using S = Tile<TYPE, WO, WI, MO>;
+    const auto kern = &k_fc_wgrad<TYPE, WO, WI, MO, LEAST>;
+    if (S::LDS > 64 * 1024) {
+        const int rc = check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::LDS));
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL(kern, dim3((unsigned)(p.ti * p.to), (unsigned)p.slices), dim3(S::THREADS),
+                       S::LDS, st, (const typename Elem<TYPE>::T *)delta, a);
+    return check_launch();
 }
 
 }  // namespace
@@ -282,17 +403,18 @@ int ach_fc_bwd_filter_checkpoint(const ach_fc_desc *desc, const void *checkpoint
     if (!aligned(checkpoint, 16) || !aligned(delta, elem_size(d.type)) || !aligned(dw, 4))
         return ACH_EINVAL;
     const Plan p = fc_plan(d);
-    if ((int64_t)p.ti * p.to > 0x7fffffff) return ACH_EUNSUPPORTED;
+    if ((int64_t)p.ti * p.to > 0x7fffffff) return ACH_EINVAL;
     if (p.bytes && (!ws || ws_bytes < p.bytes || !aligned(ws, 16))) return ACH_EWORKSPACE;
     const Fc a = {d.rows, d.inputs, d.outputs, d.stride, kept(checkpoint, d.rows, d.inputs), dw,
                   p.slices > 1 ? (float *)ws : nullptr, accumulate, p.span, p.ti, p.to};
     hipStream_t st = as_stream(s);
+    int rc;
 #define CALL(TYPE)                                                                                 \
-    hipLaunchKernelGGL((k_fc_wgrad<TYPE>), dim3((unsigned)(p.ti * p.to), (unsigned)p.slices),      \
-                       dim3(256), 0, st, (const Elem<TYPE>::T *)delta, a)
+    rc = !p.high ? fc_go<TYPE, 2, 4, 2, 2>(p, delta, a, st)                                        \
+         : TYPE == ACH_BF16 ? fc_go<TYPE, 2, 2, TYPE == ACH_BF16 ? 4 : 2, 2>(p, delta, a, st)      \
+                            : fc_go<TYPE, 4, 2, 2, 2>(p, delta, a, st)
     FOR_TYPE(d.type, CALL);
 #undef CALL
-    const int rc = check_launch();
     if (rc || p.slices == 1) return rc;
     const size_t n = (size_t)d.outputs * d.inputs;
     hipLaunchKernelGGL(k_fc_wgrad_join, dim3(grid_for(n, 256, 4096)), dim3(256), 0, st,

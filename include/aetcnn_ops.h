@@ -564,13 +564,13 @@ int ach_layernorm_bwd(const ach_layernorm_desc *d, const void *delta, int64_t de
 /* ---- a fully connected layer's weight gradient from its input's checkpoint --
  * ach_conv_bwd_filter of a fully connected geometry with the input kept in 8
  * bits: dw[o][i] (+)= sum_r delta[r][o]*x[r][i], dw float [outputs][inputs]
- * without gaps, x the checkpoint of rows x inputs (each at most 2^30), delta
- * rows of `outputs` values of `type`, `stride` elements apart (0: outputs), at
- * any element address.  accumulate as above (rows 0 and accumulate 0: zeros).
- * Every product is exact and the sums are in 32 bits: an fp32 delta is taken as
- * three bf16 pieces (fp16: two), of which parts below 2^-126 are lost.  What an
- * infinity or a NaN in delta, or a block of NaN in x, is summed into is not
- * finite; results do not depend on the run.                                */
+ * without gaps, x the checkpoint of rows x inputs, delta rows of `outputs` values
+ * of `type`, `stride` elements apart (0: outputs), at any element address; rows 0
+ * to 2^30, inputs, outputs and stride up to 2^23.  accumulate as above (rows 0 and
+ * accumulate 0: zeros).  Every product is exact and the sums are in 32 bits: an
+ * fp32 delta is taken as three bf16 pieces (fp16: two), of which parts below
+ * 2^-126 are lost.  What an infinity or a NaN in delta, or a block of NaN in x,
+ * is summed into is not finite; results do not depend on the run.           */
 typedef struct {
     int rows, inputs, outputs;
     int type;             /* of delta                                        */

@@ -164,7 +164,7 @@ class Weights:
 
 @pytest.mark.parametrize("kind", [F32, BF16, F16])
 @pytest.mark.parametrize("rows,inputs,outputs,pad,shift", [
-    (1, 1, 1, 0, 0), (1, 40, 3, 0, 1), (2, 33, 65, 1, 0), (15, 64, 64, 0, 0), (16, 100, 31, 0, 0),
+    (1, 1, 1, 0, 0), (1, 40, 3, 0, 1), (50, 300, 7, 1, 0), (70, 31, 8, 0, 1), (40, 65, 263, 0, 1), (2, 33, 65, 1, 0), (15, 64, 64, 0, 0), (16, 100, 31, 0, 0),
     (17, 129, 127, 3, 1), (33, 31, 200, 0, 0), (64, 256, 128, 0, 0), (100, 1003, 77, 5, 3),
     (128, 512, 300, 0, 0), (130, 257, 1000, 0, 0), (1531, 203, 177, 2, 1), (5000, 70, 9, 0, 0),
     (9000, 32, 16, 0, 0)])

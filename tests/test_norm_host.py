@@ -109,7 +109,8 @@ def test_checkpoint_refusals_and_sizes():
 @pytest.mark.parametrize("d", [
     FcDesc(-1, 10, 10, F32), FcDesc(2, 0, 10, F32), FcDesc(2, 10, 0, F32), FcDesc(2, 10, 10, 3),
     FcDesc(2, 10, 10, -1), FcDesc(2, 10, 10, F32, 9), FcDesc(2, 10, 10, F32, -10),
-    FcDesc(2, (1 << 30) + 1, 10, F32), FcDesc((1 << 30) + 1, 10, 10, F32), None])
+    FcDesc(2, (1 << 23) + 1, 10, F32), FcDesc((1 << 30) + 1, 10, 10, F32),
+    FcDesc(2, 10, (1 << 23) + 1, F32), FcDesc(2, 10, 10, F32, (1 << 23) + 1), None])
 def test_bad_fc_descriptors(d):
     ops = aetcnn.ops()
     assert fc(ops, d) == ACH_EINVAL
