@@ -1,5 +1,13 @@
 // Layer norm (include/aetcnn_ops.h): forward, and backward with the reduction of
 // the scales' and biases' gradients.
+//
+// Bound by memory.  A row of up to 8192 chunks of 16 bytes (backward: 4096 or
+// 2048) lies in the registers of the G threads that share it, I chunks each, so that
+// it is read once: its sums, then its values.  Short rows share a wave, rows of
+// more than a few thousand values take a workgroup of 256 or 1024 threads.
+// Workgroups run over rows and keep the parameters, and in the backward pass the
+// sums of the parameters' gradients, in registers; the next row is loaded while
+// one is worked on.  Longer rows are cut into parts, in two passes over memory.
 #include "checkpoint.hpp"
 
 #include <math.h>
@@ -7,200 +15,548 @@
 namespace ach {
 namespace {
 
-constexpr int NT = 256;
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
 
-// Sum over the workgroup; every thread gets it.  sh holds a V per wave and may
-// be used again at once.
-template <class V> __device__ __forceinline__ V block_sum(V v, V *sh)
+// ---- sums over the G threads of a row; every thread gets them -------------------
+template <int CTRL> __device__ __forceinline__ float moved(float v)
 {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    V r = sh[0];
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL> __device__ __forceinline__ double moved(double v)
+{
+    const uint64_t u = __double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xf, 0xf, true),
+                   hi = __builtin_amdgcn_mov_dpp((int)(u >> 32), CTRL, 0xf, 0xf, true);
+    return __longlong_as_double((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ float of_lane(float v, int lane) { return lane_value(v, lane); }
+__device__ __forceinline__ double of_lane(double v, int lane)
+{
+    const uint64_t u = __double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane),
+                   hi = __builtin_amdgcn_readlane((int)(u >> 32), lane);
+    return __longlong_as_double((uint64_t)hi << 32 | lo);
+}
+// Within 16 lanes by their mirror images, over a wave by its four sixteens, over a
+// workgroup through `sh`, which holds N values per wave and must not have been read
+// since the last barrier but one.
+template <int G, int N, class V> __device__ __forceinline__ void row_sums(V *v, V *sh)
+{
 #pragma unroll
-    for (int i = 1; i < NT / 64; ++i) r += sh[i];
-    return r;
+    for (int i = 0; i < N; ++i) {
+        v[i] += moved<0xb1>(v[i]);
+        v[i] += moved<0x4e>(v[i]);
+        v[i] += moved<0x141>(v[i]);
+        v[i] += moved<0x140>(v[i]);
+        if (G >= 64) v[i] = of_lane(v[i], 0) + of_lane(v[i], 16) + of_lane(v[i], 32) + of_lane(v[i], 48);
+    }
+    if (G <= 64) return;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) sh[wave * N + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = sh[i];
+#pragma unroll
+    for (int w = 1; w < G / 64; ++w)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += sh[w * N + i];
 }
 
-// The reciprocal standard deviation.  Squares that pass a float's range, of
-// differences from 1.8e19 on, are summed in 64 bits instead: `again` does that.
-template <class F> __device__ __forceinline__ float rstd_of(float squares, float n, float eps, F again)
+// ---- chunks ------------------------------------------------------------------------
+// 16 bytes as they lie in memory, of which `left` values are there (the others: fill).
+template <int TYPE>
+__device__ __forceinline__ v4u load_chunk(const typename Elem<TYPE>::T *p, int left, float fill)
 {
-    if (squares < INFINITY) return 1.f / sqrtf(squares / n + eps);
-    return (float)(1. / sqrt(again() / n + (double)eps));
+    constexpr int VEC = Row<TYPE>::VEC;
+    using T = typename Elem<TYPE>::T;
+    if (left >= VEC) {
+        const typename Row<TYPE>::Chunk c = Row<TYPE>::load(p);
+        return __builtin_bit_cast(v4u, c);
+    }
+    typename Row<TYPE>::Chunk c;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) c[i] = (T)fill;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+        if (i < left) c[i] = p[i];
+    return __builtin_bit_cast(v4u, c);
+}
+template <int TYPE> __device__ __forceinline__ void chunk_values(v4u c, float *v)
+{
+    const typename Row<TYPE>::Chunk t = __builtin_bit_cast(typename Row<TYPE>::Chunk, c);
+#pragma unroll
+    for (int i = 0; i < Row<TYPE>::VEC; ++i) v[i] = (float)t[i];
 }
 
+// Keeps the compiler from holding a chunk's values, twice the registers, from one
+// use of it to the next.
+__device__ __forceinline__ void forget(v4u &c)
+{
+    asm volatile("" : "+v"(c));
+}
+
+// ---- forward -------------------------------------------------------------------------
 struct Fwd {
     int rows, features, chunks;  // chunks of a row: with a checkpoint, of whole blocks
+    double inv;                  // 1 / features
     float eps;
     int64_t stride, y_stride;
     const float *scales, *biases;
     float *stats;
     Kept k;
+    double2 *part;   // of rows in parts: [rows][parts] sums,
+    float *first;    // [rows] first values
+    int parts, span; // chunks of a part
 };
 
-// A workgroup per row: sums relative to the row's first value (which keeps a
-// mean far above the deviations exact), squares about the mean, then the values.
-template <int TYPE, bool KEEP>
-__global__ void __launch_bounds__(NT)
-k_norm_fwd(const typename Elem<TYPE>::T *x, typename Elem<TYPE>::T *y, Fwd a)
+// From the sums of x - first and of their squares, in 64 bits: the subtraction of
+// the mean's square is exact enough for a mean 10^4 times above the deviations, and
+// relative to the row's first value it rarely is.  (The variance passes a float's
+// range where the values pass 1.8e19.)
+__device__ __forceinline__ float2 statistics(double s, double q, float first, double inv, float eps)
 {
-    constexpr int VEC = Row<TYPE>::VEC;
-    __shared__ float sh[NT / 64];
-    __shared__ double shd[NT / 64];
-    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const typename Elem<TYPE>::T *p = x + r * a.stride;
-        const float first = (float)p[0];
-        auto each = [&](auto f) {
-            for (int c = threadIdx.x; c < a.chunks; c += NT) {
-                float v[VEC];
-                load_values<TYPE>(p + c * VEC, a.features - c * VEC, v);
-                f(c * VEC, v);
-            }
-        };
-        float s = 0.f;
-        each([&](int col, const float *v) {
+    const double m = s * inv, var = fmax(q * inv - m * m, 0.) + (double)eps;
+    const float v = (float)var, mean = (float)((double)first + m);
+    float r;
+    if (v < 0x1p120f) {
+        r = __builtin_amdgcn_rsqf(v);
+        r = fmaf(.5f * r, fmaf(-v * r, r, 1.f), r);
+    } else {
+        r = (float)(1. / sqrt(var));
+    }
+    return make_float2(mean, q < (double)INFINITY ? r : NAN);
+}
+
+template <int VEC>
+__device__ __forceinline__ void add_values(const float *v, float first, double &s, double &q)
+{
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) s += col + i < a.features ? v[i] - first : 0.f;
-        });
-        const float mean = first + block_sum(s, sh) / (float)a.features;
-        float q = 0.f;
-        each([&](int col, const float *v) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float d = col + i < a.features ? v[i] - mean : 0.f;
-                q += d * d;
-            }
-        });
-        const float rstd = rstd_of(block_sum(q, sh), (float)a.features, a.eps, [&] {
-            double t = 0;
-            each([&](int col, const float *v) {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const double d = col + i < a.features ? v[i] - mean : 0.f;
-                    t += d * d;
-                }
-            });
-            return block_sum(t, shd);
-        });
-        if (a.stats && threadIdx.x == 0) a.stats[2 * (size_t)r] = mean, a.stats[2 * (size_t)r + 1] = rstd;
-        if (!y && !KEEP) continue;
-        __syncthreads();  // y may be x, whose first value the others may still read
-        each([&](int col, const float *v) {
-            float n[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) n[i] = col + i < a.features ? (v[i] - mean) * rstd : 0.f;
-            if (KEEP) keep_values<VEC>(a.k, (size_t)r * a.k.width + col, n);
-            if (!y) return;
-            float sc[VEC], b[VEC];
-            load_floats<VEC>(a.scales, col, a.features - col, 1.f, sc);
-            load_floats<VEC>(a.biases, col, a.features - col, 0.f, b);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) n[i] = n[i] * sc[i] + b[i];
-            store_values<TYPE>(y + r * a.y_stride + col, a.features - col, n);
-        });
+    for (int i = 0; i < VEC; ++i) {
+        const double d = (double)(v[i] - first);
+        s += d;
+        q = fma(d, d, q);
     }
 }
 
+// The values of a chunk: into the checkpoint and into y.
+template <int TYPE, bool KEEP>
+__device__ __forceinline__ void put_values(const Fwd &a, typename Elem<TYPE>::T *y, int r, int col,
+                                           v4u c, float2 st, const float *sc, const float *b)
+{
+    constexpr int VEC = Row<TYPE>::VEC;
+    const int left = a.features - col;
+    float n[VEC];
+    chunk_values<TYPE>(c, n);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) n[i] = (n[i] - st.x) * st.y;
+    if (KEEP) {
+        if (left < VEC) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) n[i] = i < left ? n[i] : 0.f;
+        }
+        keep_values<VEC>(a.k, (size_t)r * a.k.width + col, n);
+    }
+    if (!y) return;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) n[i] = n[i] * sc[i] + b[i];
+    store_values<TYPE>(y + r * a.y_stride + col, left, n);
+}
+
+template <int TYPE, int G, int I, bool KEEP>
+__global__ void __launch_bounds__(G < 256 ? 256 : G)
+k_norm_fwd(const typename Elem<TYPE>::T *x, typename Elem<TYPE>::T *y, Fwd a)
+{
+    constexpr int VEC = Row<TYPE>::VEC, NT = G < 256 ? 256 : G, AT_ONCE = NT / G;
+    constexpr bool HOLD = I <= 2, AHEAD = I <= 4;
+    using T = typename Elem<TYPE>::T;
+    __shared__ double sh[2][2 * NT / 64];
+    const int t = threadIdx.x % G, step = (int)gridDim.x * AT_ONCE;
+    int r = (int)blockIdx.x * AT_ONCE + threadIdx.x / G;
+    float sc[HOLD ? I * VEC : VEC], b[HOLD ? I * VEC : VEC];
+    auto parameters = [&](int c, float *s, float *o) {
+        load_floats<VEC>(a.scales, c * VEC, a.features - c * VEC, 1.f, s);
+        load_floats<VEC>(a.biases, c * VEC, a.features - c * VEC, 0.f, o);
+    };
+    if (HOLD && y) {
+#pragma unroll
+        for (int i = 0; i < I; ++i) parameters(t + i * G, sc + i * VEC, b + i * VEC);
+    }
+    v4u c[I], ahead[AHEAD ? I : 1];
+    float first, next_first;
+    auto load = [&](int row, v4u *to, float &f) {
+        const T *p = x + row * a.stride;
+        f = (float)p[0];
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const int col = (t + i * G) * VEC;
+            to[i] = load_chunk<TYPE>(p + col, a.features - col, f);
+        }
+    };
+    if (r < a.rows) load(r, c, first);
+    for (int turn = 0; r < a.rows; r += step, turn ^= 1) {
+        const bool more = r + step < a.rows;
+        if (AHEAD && more) load(r + step, ahead, next_first);
+        double sums[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            float v[VEC];
+            chunk_values<TYPE>(c[i], v);
+            add_values<VEC>(v, first, sums[0], sums[1]);
+        }
+        row_sums<G, 2>(sums, sh[turn]);
+        if (I > 2) {
+#pragma unroll
+            for (int i = 0; i < I; ++i) forget(c[i]);
+        }
+        const float2 st = statistics(sums[0], sums[1], first, a.inv, a.eps);
+        if (a.stats && t == 0) {
+            a.stats[2 * (size_t)r] = st.x;
+            a.stats[2 * (size_t)r + 1] = st.y;
+        }
+        if (y || KEEP) {
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                const int at = t + i * G;
+                if (at >= a.chunks) continue;
+                if (!HOLD && y) parameters(at, sc, b);
+                put_values<TYPE, KEEP>(a, y, r, at * VEC, c[i], st, sc + (HOLD ? i * VEC : 0),
+                                       b + (HOLD ? i * VEC : 0));
+            }
+        }
+        if (AHEAD) {
+#pragma unroll
+            for (int i = 0; i < I; ++i) c[i] = ahead[AHEAD ? i : 0];
+            first = next_first;
+        } else if (more) {
+            load(r + step, c, first);
+        }
+    }
+}
+
+// Rows in parts: the sums of each part, then, from all of a row's, its values.
+constexpr int PART_NT = 256;
+template <int TYPE>
+__global__ void __launch_bounds__(PART_NT) k_norm_fwd_sums(const typename Elem<TYPE>::T *x, Fwd a)
+{
+    constexpr int VEC = Row<TYPE>::VEC;
+    __shared__ double sh[2 * PART_NT / 64];
+    const int r = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const typename Elem<TYPE>::T *p = x + r * a.stride;
+    const float first = (float)p[0];
+    const int end = min((part + 1) * a.span, a.chunks);
+    double sums[2] = {0, 0};
+    for (int c = part * a.span + threadIdx.x; c < end; c += PART_NT) {
+        float v[VEC];
+        chunk_values<TYPE>(load_chunk<TYPE>(p + c * VEC, a.features - c * VEC, first), v);
+        add_values<VEC>(v, first, sums[0], sums[1]);
+    }
+    row_sums<PART_NT, 2>(sums, sh);
+    if (threadIdx.x == 0) {
+        a.part[blockIdx.x] = make_double2(sums[0], sums[1]);
+        if (part == 0) a.first[r] = first;  // (y may be x)
+    }
+}
+
+template <int TYPE, bool KEEP>
+__global__ void __launch_bounds__(PART_NT)
+k_norm_fwd_values(const typename Elem<TYPE>::T *x, typename Elem<TYPE>::T *y, Fwd a)
+{
+    constexpr int VEC = Row<TYPE>::VEC;
+    const int r = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const typename Elem<TYPE>::T *p = x + r * a.stride;
+    const float first = a.first[r];
+    double s = 0, q = 0;
+    for (int i = 0; i < a.parts; ++i) {
+        const double2 v = a.part[(size_t)r * a.parts + i];
+        s += v.x, q += v.y;
+    }
+    const float2 st = statistics(s, q, first, a.inv, a.eps);
+    if (a.stats && part == 0 && threadIdx.x == 0) {
+        a.stats[2 * (size_t)r] = st.x;
+        a.stats[2 * (size_t)r + 1] = st.y;
+    }
+    if (!y && !KEEP) return;
+    const int end = min((part + 1) * a.span, a.chunks);
+    for (int c = part * a.span + threadIdx.x; c < end; c += PART_NT) {
+        const int col = c * VEC, left = a.features - col;
+        float sc[VEC], b[VEC];
+        if (y) {
+            load_floats<VEC>(a.scales, col, left, 1.f, sc);
+            load_floats<VEC>(a.biases, col, left, 0.f, b);
+        }
+        put_values<TYPE, KEEP>(a, y, r, col, load_chunk<TYPE>(p + col, left, 0.f), st, sc, b);
+    }
+}
+
+// ---- backward -------------------------------------------------------------------------
 struct Bwd {
     int rows, features, chunks;
     int64_t stride, d_stride, dx_stride;
     const float *stats, *scales;
     Kept k;
-    float2 *sums;   // [rows] {sum g, sum g*x_norm} / n
-    float *part;    // [2][spans][features]
-    int span, spans;  // rows of a partial sum
+    float2 *sums;     // of rows in parts: [rows][parts] sums of g and of g*x_norm
+    int parts, span;  // chunks of a part
+    float *partial;   // [2][spans][features]: sums over rows, or null
+    int rows_of, spans;  // rows of one (rows in parts), their number
 };
 
-// x_norm of a chunk, from the rows or from their checkpoint
-template <int TYPE, bool KEPT>
-__device__ __forceinline__ void normal_values(const typename Elem<TYPE>::T *x, const Bwd &a, int r,
-                                              int col, float mean, float rstd, float *v)
-{
-    constexpr int VEC = Row<TYPE>::VEC;
-    if (KEPT) {
-        kept_values<VEC>(a.k, (size_t)r * a.k.width + col, v);
-        return;
+// What the sums and the values need of a row's chunk: delta and x as they lie in
+// memory (or x_norm's codes and step).
+template <int TYPE, bool KEPT> struct Pair {
+    static constexpr int VEC = Row<TYPE>::VEC;
+    using T = typename Elem<TYPE>::T;
+    v4u d;
+    uint32_t x[KEPT ? VEC / 4 : 4], step;
+    __device__ __forceinline__ void load(const T *delta, const T *xs, const Bwd &a, int r, int col)
+    {
+        const int left = a.features - col;
+        d = load_chunk<TYPE>(delta + r * a.d_stride + col, left, 0.f);
+        if (KEPT) {
+            // (codes behind the last value are 0, up to a whole block)
+            const size_t at = (size_t)r * a.k.width + min(col, a.k.width - VEC);
+            __builtin_memcpy(x, __builtin_assume_aligned(a.k.codes + at, VEC), VEC);
+            step = a.k.steps[at / KEPT_BLOCK];
+        } else {
+            const v4u c = load_chunk<TYPE>(xs + r * a.stride + col, left, 0.f);
+            __builtin_memcpy(x, &c, sizeof(c));
+        }
     }
-    load_values<TYPE>(x + r * a.stride + col, a.features - col, v);
+    __device__ __forceinline__ void forget_values()
+    {
+        forget(d);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = (v[i] - mean) * rstd;
+        for (auto &v : x) asm volatile("" : "+v"(v));
+    }
+    __device__ __forceinline__ void values(float2 st, float *dv, float *n) const
+    {
+        chunk_values<TYPE>(d, dv);
+        if constexpr (KEPT) {
+            const float scale = kept_scale(step);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) n[i] = (float)(int8_t)(x[i / 4] >> (8 * (i % 4))) * scale;
+        } else {
+            v4u c;
+            __builtin_memcpy(&c, x, sizeof(c));
+            chunk_values<TYPE>(c, n);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) n[i] = (n[i] - st.x) * st.y;
+        }
+    }
+};
+
+__device__ __forceinline__ float2 stats_of(const Bwd &a, int r)
+{
+    return make_float2(a.stats[2 * (size_t)r], a.stats[2 * (size_t)r + 1]);
 }
 
+template <int TYPE, int G, int I, bool KEPT>
+__global__ void __launch_bounds__(G < 256 ? 256 : G)
+k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
+           typename Elem<TYPE>::T *dx, Bwd a, float inv)
+{
+    constexpr int VEC = Row<TYPE>::VEC, NT = G < 256 ? 256 : G, AT_ONCE = NT / G;
+    constexpr bool HOLD = I * VEC <= 16, AHEAD = I * VEC <= 16;  // (registers)
+    using P = Pair<TYPE, KEPT>;
+    __shared__ float sh[2][2 * NT / 64];
+    __shared__ float join[AT_ONCE > 1 ? NT * I * VEC : 1];
+    const int t = threadIdx.x % G, step = (int)gridDim.x * AT_ONCE;
+    int r = (int)blockIdx.x * AT_ONCE + threadIdx.x / G;
+    float sc[HOLD ? I * VEC : VEC], ds[I * VEC], db[I * VEC];
+    if (HOLD) {
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+            load_floats<VEC>(a.scales, (t + i * G) * VEC, a.features - (t + i * G) * VEC, 1.f, sc + i * VEC);
+    }
+#pragma unroll
+    for (int i = 0; i < I * VEC; ++i) ds[i] = db[i] = 0.f;
+    P c[I], ahead[AHEAD ? I : 1];
+    float2 st, next;
+    auto load = [&](int row, P *to, float2 &s) {
+        s = stats_of(a, row);
+#pragma unroll
+        for (int i = 0; i < I; ++i) to[i].load(delta, x, a, row, (t + i * G) * VEC);
+    };
+    if (r < a.rows) load(r, c, st);
+    for (int turn = 0; r < a.rows; r += step, turn ^= 1) {
+        const bool more = r + step < a.rows;
+        if (AHEAD && more) load(r + step, ahead, next);
+        float sums[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            float d[VEC], n[VEC];
+            c[i].values(st, d, n);
+            if (!HOLD && dx) load_floats<VEC>(a.scales, (t + i * G) * VEC, a.features - (t + i * G) * VEC, 1.f, sc);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                // (deltas behind the last value are 0, x_norm is any number there)
+                const float g = d[e] * sc[(HOLD ? i * VEC : 0) + e];
+                sums[0] += g;
+                sums[1] = fmaf(g, n[e], sums[1]);
+                ds[i * VEC + e] = fmaf(d[e], n[e], ds[i * VEC + e]);
+                db[i * VEC + e] += d[e];
+            }
+        }
+        if (dx) {
+            row_sums<G, 2>(sums, sh[turn]);
+            if (I * VEC > 16) {
+#pragma unroll
+                for (int i = 0; i < I; ++i) c[i].forget_values();
+            }
+            const float m1 = sums[0] * inv, m2 = sums[1] * inv;
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                const int col = (t + i * G) * VEC;
+                if (col >= a.features) continue;
+                float d[VEC], n[VEC];
+                c[i].values(st, d, n);
+                if (!HOLD) load_floats<VEC>(a.scales, col, a.features - col, 1.f, sc);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    d[e] = st.y * (d[e] * sc[(HOLD ? i * VEC : 0) + e] - m1 - n[e] * m2);
+                store_values<TYPE>(dx + r * a.dx_stride + col, a.features - col, d);
+            }
+        }
+        if (AHEAD) {
+#pragma unroll
+            for (int i = 0; i < I; ++i) c[i] = ahead[AHEAD ? i : 0];
+            st = next;
+        } else if (more) {
+            load(r + step, c, st);
+        }
+    }
+    if (!a.partial) return;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float *const v = which ? db : ds;
+        float *const to = a.partial + ((size_t)which * a.spans + blockIdx.x) * a.features;
+        if (AT_ONCE > 1) {  // the workgroup's rows, in LDS as [value][row][thread]
+            if (which) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < I * VEC; ++i) join[i * NT + threadIdx.x] = v[i];
+            __syncthreads();
+            for (int j = threadIdx.x; j < G * I * VEC; j += NT) {
+                const int i = j / G, u = j % G;
+                const int col = (u + i / VEC * G) * VEC + i % VEC;
+                if (col >= a.features) continue;
+                float s = 0.f;
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k) s += join[i * NT + k * G + u];
+                to[col] = s;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+                const int col = (t + i * G) * VEC;
+#pragma unroll
+                for (int e = 0; e < VEC; e += 4)
+                    store_values<ACH_F32>(to + col + e, a.features - col - e, v + i * VEC + e);
+            }
+        }
+    }
+}
+
+// Rows in parts: the sums of each part, then tiles of columns over spans of rows.
 template <int TYPE, bool KEPT>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(PART_NT)
 k_norm_bwd_sums(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x, Bwd a)
 {
     constexpr int VEC = Row<TYPE>::VEC;
-    __shared__ float sh[NT / 64];
-    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const float mean = a.stats[2 * (size_t)r], rstd = a.stats[2 * (size_t)r + 1];
-        float s = 0.f, t = 0.f;
-        for (int c = threadIdx.x; c < a.chunks; c += NT) {
-            const int col = c * VEC, left = a.features - col;
-            float d[VEC], n[VEC], sc[VEC];
-            load_values<TYPE>(delta + r * a.d_stride + col, left, d);
-            normal_values<TYPE, KEPT>(x, a, r, col, mean, rstd, n);
-            load_floats<VEC>(a.scales, col, left, 1.f, sc);
+    __shared__ float sh[2 * PART_NT / 64];
+    const int r = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const float2 st = stats_of(a, r);
+    const int end = min((part + 1) * a.span, a.chunks);
+    float sums[2] = {0.f, 0.f};
+    for (int c = part * a.span + threadIdx.x; c < end; c += PART_NT) {
+        Pair<TYPE, KEPT> p;
+        float d[VEC], n[VEC], sc[VEC];
+        p.load(delta, x, a, r, c * VEC);
+        p.values(st, d, n);
+        load_floats<VEC>(a.scales, c * VEC, a.features - c * VEC, 1.f, sc);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float g = d[i] * sc[i];
-                if (i < left) s += g, t += g * n[i];
-            }
+        for (int e = 0; e < VEC; ++e) {
+            const float g = d[e] * sc[e];
+            sums[0] += g;
+            sums[1] = fmaf(g, n[e], sums[1]);
         }
-        s = block_sum(s, sh), t = block_sum(t, sh);
-        if (threadIdx.x == 0) a.sums[r] = make_float2(s / a.features, t / a.features);
     }
+    row_sums<PART_NT, 2>(sums, sh);
+    if (threadIdx.x == 0) a.sums[blockIdx.x] = make_float2(sums[0], sums[1]);
 }
 
-// A tile of NT chunks of columns and a span of rows
 template <int TYPE, bool KEPT>
-__global__ void __launch_bounds__(NT)
-k_norm_bwd_apply(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
-                 typename Elem<TYPE>::T *dx, Bwd a)
+__global__ void __launch_bounds__(PART_NT)
+k_norm_bwd_values(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
+                  typename Elem<TYPE>::T *dx, Bwd a, float inv)
 {
     constexpr int VEC = Row<TYPE>::VEC;
-    const int tiles = (a.chunks + NT - 1) / NT;
-    const int tile = blockIdx.x % tiles, part = blockIdx.x / tiles;
-    const int col = (tile * NT + threadIdx.x) * VEC, left = a.features - col;
+    const int tiles = (a.chunks + PART_NT - 1) / PART_NT;
+    const int tile = blockIdx.x % tiles, span = blockIdx.x / tiles;
+    const int col = (tile * PART_NT + threadIdx.x) * VEC, left = a.features - col;
     if (left <= 0) return;
     float sc[VEC], ds[VEC], db[VEC];
     load_floats<VEC>(a.scales, col, left, 1.f, sc);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) ds[i] = db[i] = 0.f;
-    const int end = min((int64_t)a.rows, (int64_t)(part + 1) * a.span);
-    for (int r = part * a.span; r < end; ++r) {
-        const float mean = a.stats[2 * (size_t)r], rstd = a.stats[2 * (size_t)r + 1];
+    for (int e = 0; e < VEC; ++e) ds[e] = db[e] = 0.f;
+    const int end = min((int64_t)a.rows, (int64_t)(span + 1) * a.rows_of);
+    for (int r = span * a.rows_of; r < end; ++r) {
+        const float2 st = stats_of(a, r);
+        Pair<TYPE, KEPT> p;
         float d[VEC], n[VEC];
-        load_values<TYPE>(delta + r * a.d_stride + col, left, d);
-        normal_values<TYPE, KEPT>(x, a, r, col, mean, rstd, n);
+        p.load(delta, x, a, r, col);
+        p.values(st, d, n);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) ds[i] += d[i] * n[i], db[i] += d[i];
+        for (int e = 0; e < VEC; ++e) ds[e] = fmaf(d[e], n[e], ds[e]), db[e] += d[e];
         if (!dx) continue;
-        const float2 m = a.sums[r];
+        float m1 = 0.f, m2 = 0.f;
+        for (int i = 0; i < a.parts; ++i) {
+            const float2 v = a.sums[(size_t)r * a.parts + i];
+            m1 += v.x, m2 += v.y;
+        }
+        m1 *= inv, m2 *= inv;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) d[i] = rstd * (d[i] * sc[i] - m.x - n[i] * m.y);
+        for (int e = 0; e < VEC; ++e) d[e] = st.y * (d[e] * sc[e] - m1 - n[e] * m2);
         store_values<TYPE>(dx + r * a.dx_stride + col, left, d);
     }
-    if (!a.part) return;
+    if (!a.partial) return;
+    float *const to = a.partial + (size_t)span * a.features + col;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i)
-        if (i < left) {
-            a.part[(size_t)part * a.features + col + i] = ds[i];
-            a.part[((size_t)a.spans + part) * a.features + col + i] = db[i];
-        }
+    for (int e = 0; e < VEC; e += 4) {
+        store_values<ACH_F32>(to + e, left - e, ds + e);
+        store_values<ACH_F32>(to + (size_t)a.spans * a.features + e, left - e, db + e);
+    }
 }
 
-__global__ void __launch_bounds__(NT)
-k_norm_bwd_join(const float *part, int spans, int features, float *scale_updates,
+// The partial sums of a column, an eighth of them by each of eight threads.
+__global__ void __launch_bounds__(256)
+k_norm_bwd_join(const float *partial, int spans, int features, float *scale_updates,
                 float *bias_updates, int accumulate)
 {
-    const int j = blockIdx.x * NT + threadIdx.x;
-    float *to = blockIdx.y ? bias_updates : scale_updates;
-    if (j >= features || !to) return;
+    __shared__ double sh[8][32];
+    float *const to = blockIdx.y ? bias_updates : scale_updates;
+    if (!to) return;
+    const int lane = threadIdx.x & 31, eighth = threadIdx.x >> 5;
+    const int j = blockIdx.x * 32 + lane;
     double s = 0;
-    for (int i = 0; i < spans; ++i) s += part[((size_t)blockIdx.y * spans + i) * features + j];
+    if (j < features) {
+        const float *p = partial + (size_t)blockIdx.y * spans * features + j;
+        int i = eighth;
+        for (; i + 24 < spans; i += 32) {  // four loads in flight
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = p[(size_t)(i + 8 * u) * features];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s += v[u];
+        }
+        for (; i < spans; i += 8) s += p[(size_t)i * features];
+    }
+    sh[eighth][lane] = s;
+    __syncthreads();
+    if (eighth || j >= features) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += sh[i][lane];
     to[j] = accumulate ? (float)(to[j] + s) : (float)s;
 }
 
@@ -220,29 +576,127 @@ bool row_stride(int64_t *stride, int features)
     return *stride >= features;
 }
 
-unsigned grid_of(size_t n) { return (unsigned)(n < (1u << 20) ? n : 1u << 20); }
-
 size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 
+// Chunks of a row, in whole blocks of a checkpoint.
+int chunks_of(const ach_layernorm_desc &d)
+{
+    const int vec = 16 / (int)elem_size(d.type);
+    return (int)(((int64_t)d.features + KEPT_BLOCK - 1) / KEPT_BLOCK * KEPT_BLOCK / vec);
+}
+
 struct Plan {
-    int tiles, span, spans;
-    size_t sums, bytes;  // of the workspace: the rows' sums, all
+    int grid;            // workgroups of rows in registers; 0: rows in parts
+    int parts, span;     // of a row: parts, chunks of each
+    int tiles, rows_of, spans;  // backward, rows in parts: tiles of columns, rows of a span, spans
+    size_t first, partial, bytes;  // of the workspace
 };
+
+// The threads that share a row and the chunks of each: the fewest threads that
+// hold it.
+template <int G_, int I_> struct Kind {
+    static constexpr int G = G_, I = I_, NT = G < 256 ? 256 : G;
+};
+template <class F> bool for_kind(int chunks, int most, F f)
+{
+    if (chunks > most) return false;
+    if (chunks <= 16) f(Kind<16, 1>());
+    else if (chunks <= 64) f(Kind<64, 1>());
+    else if (chunks <= 128) f(Kind<64, 2>());
+    else if (chunks <= 256) f(Kind<256, 1>());
+    else if (chunks <= 512) f(Kind<256, 2>());
+    else if (chunks <= 1024) f(Kind<256, 4>());
+    else if (chunks <= 2048) f(Kind<512, 4>());
+    else if (chunks <= 4096) f(Kind<512, 8>());
+    else f(Kind<512, 16>());
+    return true;
+}
+// A row's chunks that fit the registers: 16 of a thread's 512 in the forward pass;
+// in the backward pass 8 of 4 values or 4 of 8, for which it holds two sums each.
+constexpr int FWD_CHUNKS = 8192;
+constexpr int bwd_chunks(int type) { return type == ACH_F32 ? 4096 : 2048; }
+
+void in_parts(int chunks, int rows, Plan *p)
+{
+    // parts of 4 to 16 chunks a thread, so that there are 1024 workgroups where that can be
+    int64_t parts = rows ? 1024 / rows : 1;
+    const int64_t least = (chunks + 16 * PART_NT - 1) / (16 * PART_NT), most = chunks / (4 * PART_NT);
+    if (parts > most) parts = most;
+    if (parts < least) parts = least;
+    if (parts < 1) parts = 1;
+    p->span = (int)((chunks + parts - 1) / parts);
+    p->span = (p->span + PART_NT - 1) / PART_NT * PART_NT;
+    p->parts = (chunks + p->span - 1) / p->span;
+}
+
+Plan fwd_plan(const ach_layernorm_desc &d)
+{
+    Plan p = {};
+    const int chunks = chunks_of(d);
+    if (!for_kind(chunks, FWD_CHUNKS, [&](auto k) {
+            const int at_once = k.NT / k.G, all = (d.rows + at_once - 1) / at_once;
+            p.grid = min(all, k.NT == 512 ? 1024 : 2048);
+        })) {
+        in_parts(chunks, d.rows, &p);
+        p.first = (size_t)d.rows * p.parts * sizeof(double2);
+        p.bytes = p.first + (size_t)d.rows * sizeof(float);
+    }
+    return p;
+}
 
 Plan bwd_plan(const ach_layernorm_desc &d)
 {
-    Plan p;
-    const int vec = 16 / (int)elem_size(d.type);
-    p.tiles = ((d.features + vec - 1) / vec + NT - 1) / NT;
-    int spans = 1024 / p.tiles;
-    if (spans < d.rows / 256) spans = d.rows / 256;  // short chains of sums
-    if (spans > d.rows) spans = d.rows;
-    if (spans < 1) spans = 1;
-    p.span = d.rows ? (int)(((int64_t)d.rows + spans - 1) / spans) : 1;
-    p.spans = (int)(((int64_t)d.rows + p.span - 1) / p.span);
-    p.sums = round16((size_t)d.rows * sizeof(float2));
-    p.bytes = p.sums + (size_t)2 * p.spans * d.features * sizeof(float);
+    Plan p = {};
+    const int chunks = chunks_of(d);
+    if (!for_kind(chunks, bwd_chunks(d.type), [&](auto k) {
+            const int at_once = k.NT / k.G, all = (d.rows + at_once - 1) / at_once;
+            // at least so many that no chain of sums is longer than 256 rows
+            p.grid = p.spans = min(all, max(k.NT == 512 ? 256 : 512, (all + 255) / 256));
+        })) {
+        in_parts(chunks, d.rows, &p);
+        p.tiles = (chunks + PART_NT - 1) / PART_NT;
+        const int spans = max(min(max(1024 / p.tiles, d.rows / 256), d.rows), 1);
+        p.rows_of = d.rows ? (int)(((int64_t)d.rows + spans - 1) / spans) : 1;
+        p.spans = (int)(((int64_t)d.rows + p.rows_of - 1) / p.rows_of);
+        p.partial = round16((size_t)d.rows * p.parts * sizeof(float2));
+    }
+    p.bytes = p.partial + (size_t)2 * p.spans * d.features * sizeof(float);
     return p;
+}
+
+template <int TYPE, bool KEEP>
+int fwd_go(const Plan &p, const void *x, void *y, const Fwd &a, int chunks, hipStream_t st)
+{
+    using T = typename Elem<TYPE>::T;
+    if (!for_kind(chunks, FWD_CHUNKS, [&](auto k) {
+            hipLaunchKernelGGL((k_norm_fwd<TYPE, k.G, k.I, KEEP>), dim3(p.grid), dim3(k.NT), 0, st,
+                               (const T *)x, (T *)y, a);
+        })) {
+        const dim3 grid((unsigned)(a.rows * p.parts)), nt(PART_NT);
+        hipLaunchKernelGGL((k_norm_fwd_sums<TYPE>), grid, nt, 0, st, (const T *)x, a);
+        hipLaunchKernelGGL((k_norm_fwd_values<TYPE, KEEP>), grid, nt, 0, st, (const T *)x, (T *)y, a);
+    }
+    return check_launch();
+}
+
+template <int TYPE, bool KEPT>
+int bwd_go(const Plan &p, const void *delta, const void *x, void *dx, const Bwd &a, int chunks,
+           hipStream_t st)
+{
+    using T = typename Elem<TYPE>::T;
+    const float inv = (float)(1. / a.features);
+    if (!for_kind(chunks, bwd_chunks(TYPE), [&](auto k) {
+            if constexpr (k.G * k.I <= bwd_chunks(TYPE))
+                hipLaunchKernelGGL((k_norm_bwd<TYPE, k.G, k.I, KEPT>), dim3(p.grid), dim3(k.NT), 0, st,
+                                   (const T *)delta, (const T *)x, (T *)dx, a, inv);
+        })) {
+        if (dx)
+            hipLaunchKernelGGL((k_norm_bwd_sums<TYPE, KEPT>), dim3((unsigned)(a.rows * p.parts)),
+                               dim3(PART_NT), 0, st, (const T *)delta, (const T *)x, a);
+        hipLaunchKernelGGL((k_norm_bwd_values<TYPE, KEPT>), dim3((unsigned)(p.tiles * p.spans)),
+                           dim3(PART_NT), 0, st, (const T *)delta, (const T *)x, (T *)dx, a, inv);
+    }
+    return check_launch();
 }
 
 }  // namespace
@@ -252,14 +706,15 @@ using namespace ach;
 
 extern "C" {
 
-size_t ach_layernorm_fwd_workspace(const ach_layernorm_desc *)
+size_t ach_layernorm_fwd_workspace(const ach_layernorm_desc *desc)
 {
-    return 0;
+    ach_layernorm_desc d;
+    return layernorm_desc(desc, &d) ? fwd_plan(d).bytes : 0;
 }
 
 int ach_layernorm_fwd(const ach_layernorm_desc *desc, const void *x, const float *scales,
                       const float *biases, void *y, int64_t y_stride, float *stats,
-                      void *checkpoint, void *, size_t, ach_stream_t s)
+                      void *checkpoint, void *ws, size_t ws_bytes, ach_stream_t s)
 {
     ach_layernorm_desc d;
     if (!layernorm_desc(desc, &d) || !x || (!y && !stats && !checkpoint)) return ACH_EINVAL;
@@ -268,25 +723,21 @@ int ach_layernorm_fwd(const ach_layernorm_desc *desc, const void *x, const float
     if (!aligned(x, size) || !aligned(y, size) || !aligned(checkpoint, 16)) return ACH_EINVAL;
     if (!aligned(scales, 4) || !aligned(biases, 4) || !aligned(stats, 4)) return ACH_EINVAL;
     if (y == x && y_stride != d.stride) return ACH_EINVAL;
+    const Plan p = fwd_plan(d);
+    if (p.bytes && (!ws || ws_bytes < p.bytes || !aligned(ws, 16))) return ACH_EWORKSPACE;
     if (d.rows == 0) return ACH_OK;
-    Fwd a = {d.rows, d.features, 0, d.eps, d.stride, y_stride, scales, biases, stats, {}};
+    Fwd a = {d.rows, d.features, 0, 1. / d.features, d.eps, d.stride, y_stride, scales, biases,
+             stats, {}, (double2 *)ws, (float *)((char *)ws + p.first), p.parts, p.span};
     if (checkpoint) a.k = kept(checkpoint, d.rows, d.features);
     hipStream_t st = as_stream(s);
+    const int vec = 16 / (int)size;
+    a.chunks = checkpoint ? chunks_of(d) : (d.features + vec - 1) / vec;
+    if ((int64_t)d.rows * p.parts > 0x7fffffff) return ACH_EINVAL;
 #define CALL(TYPE)                                                                                 \
-    do {                                                                                           \
-        using T = Elem<TYPE>::T;                                                                   \
-        constexpr int VEC = Row<TYPE>::VEC;                                                        \
-        a.chunks = checkpoint ? a.k.width / VEC : (d.features + VEC - 1) / VEC;                    \
-        if (checkpoint)                                                                            \
-            hipLaunchKernelGGL((k_norm_fwd<TYPE, true>), dim3(grid_of(d.rows)), dim3(NT), 0, st,   \
-                               (const T *)x, (T *)y, a);                                           \
-        else                                                                                       \
-            hipLaunchKernelGGL((k_norm_fwd<TYPE, false>), dim3(grid_of(d.rows)), dim3(NT), 0, st,  \
-                               (const T *)x, (T *)y, a);                                           \
-    } while (0)
+    return checkpoint ? fwd_go<TYPE, true>(p, x, y, a, chunks_of(d), st)                           \
+                      : fwd_go<TYPE, false>(p, x, y, a, chunks_of(d), st)
     FOR_TYPE(d.type, CALL);
 #undef CALL
-    return check_launch();
 }
 
 size_t ach_layernorm_bwd_workspace(const ach_layernorm_desc *desc)
@@ -314,38 +765,28 @@ int ach_layernorm_bwd(const ach_layernorm_desc *desc, const void *delta, int64_t
     if (dx == delta && dx_stride != delta_stride) return ACH_EINVAL;
     const Plan p = bwd_plan(d);
     if (p.bytes && (!ws || ws_bytes < p.bytes || !aligned(ws, 16))) return ACH_EWORKSPACE;
+    if ((int64_t)d.rows * p.parts > 0x7fffffff || (int64_t)p.tiles * p.spans > 0x7fffffff) return ACH_EINVAL;
     hipStream_t st = as_stream(s);
     const bool updates = scale_updates || bias_updates;
+    float *const partial = (float *)((char *)ws + p.partial);
+    const int vec = 16 / (int)size;
     if (d.rows) {
-        Bwd a = {d.rows, d.features, 0, d.stride, delta_stride, dx_stride, stats, scales, {},
-                 (float2 *)ws, updates ? (float *)((char *)ws + p.sums) : nullptr, p.span, p.spans};
+        Bwd a = {d.rows, d.features, (d.features + vec - 1) / vec, d.stride, delta_stride, dx_stride,
+                 stats, scales, {}, (float2 *)ws, p.parts, p.span, updates ? partial : nullptr,
+                 p.rows_of, p.spans};
         if (checkpoint) a.k = kept(checkpoint, d.rows, d.features);
-#define GO(TYPE, KEPT)                                                                             \
-    do {                                                                                           \
-        using T = Elem<TYPE>::T;                                                                   \
-        constexpr int VEC = Row<TYPE>::VEC;                                                        \
-        a.chunks = (d.features + VEC - 1) / VEC;                                                   \
-        if (dx)                                                                                    \
-            hipLaunchKernelGGL((k_norm_bwd_sums<TYPE, KEPT>), dim3(grid_of(d.rows)), dim3(NT), 0,  \
-                               st, (const T *)delta, (const T *)x, a);                             \
-        hipLaunchKernelGGL((k_norm_bwd_apply<TYPE, KEPT>), dim3((unsigned)(p.tiles * p.spans)),    \
-                           dim3(NT), 0, st, (const T *)delta, (const T *)x, (T *)dx, a);           \
-    } while (0)
+        int rc;
 #define CALL(TYPE)                                                                                 \
-    do {                                                                                           \
-        if (checkpoint) GO(TYPE, true);                                                            \
-        else GO(TYPE, false);                                                                      \
-    } while (0)
+    rc = checkpoint ? bwd_go<TYPE, true>(p, delta, x, dx, a, chunks_of(d), st)                     \
+                    : bwd_go<TYPE, false>(p, delta, x, dx, a, chunks_of(d), st)
         FOR_TYPE(d.type, CALL);
 #undef CALL
-#undef GO
-        const int rc = check_launch();
         if (rc) return rc;
     }
     if (updates) {
-        hipLaunchKernelGGL(k_norm_bwd_join, dim3((unsigned)((d.features + NT - 1) / NT), 2), dim3(NT),
-                           0, st, (const float *)((char *)ws + p.sums), p.spans, d.features,
-                           scale_updates, bias_updates, accumulate);
+        hipLaunchKernelGGL(k_norm_bwd_join, dim3((unsigned)((d.features + 31) / 32), 2), dim3(256), 0,
+                           st, (const float *)partial, p.spans, d.features, scale_updates,
+                           bias_updates, accumulate);
         return check_launch();
     }
     return ACH_OK;
