@@ -1,9 +1,9 @@
 // Layer norm (include/aetcnn_ops.h): forward, and backward with the reduction of
 // the scales' and biases' gradients.
 //
-// Bound by memory.  A row of up to 8192 chunks of 16 bytes (backward: 4096 or
-// 2048) lies in the registers of the G threads that share it, I chunks each, so that
-// it is read once: its sums, then its values.  Short rows share a wave, rows of
+// Bound by memory.  A row of up to 4096 chunks of 16 bytes (backward, 16-bit
+// types: 2048) lies in the registers of the G threads that share it, I chunks each,
+// so that it is read once: its sums, then its values.  Short rows share a wave, rows of
 // more than a few thousand values take a workgroup of 256 or 1024 threads.
 // Workgroups run over rows and keep the parameters, and in the backward pass the
 // sums of the parameters' gradients, in registers; the next row is loaded while
@@ -65,6 +65,17 @@ template <int G, int N, class V> __device__ __forceinline__ void row_sums(V *v, 
         for (int i = 0; i < N; ++i) v[i] += sh[w * N + i];
 }
 
+// Values into y or dx.  What the L2 caches (8 of 4 MB) do not hold is stored past
+// the caches, where it would take the place of rows that are still to be read
+// (4096 x 8192 bf16 forward: 32 us, 23 past them; 128 x 186624 fp32, which is read
+// twice: 66 and 55).
+template <int TYPE>
+__device__ __forceinline__ void write_values(typename Elem<TYPE>::T *p, int left, const float *v, bool past)
+{
+    if (past) store_values<TYPE, true>(p, left, v);
+    else store_values<TYPE>(p, left, v);
+}
+
 // ---- chunks ------------------------------------------------------------------------
 // 16 bytes as they lie in memory, of which `left` values are there (the others: fill).
 template <int TYPE>
@@ -100,6 +111,7 @@ __device__ __forceinline__ void forget(v4u &c)
 
 // ---- forward -------------------------------------------------------------------------
 struct Fwd {
+    bool past;                   // y past the caches
     int rows, features, chunks;  // chunks of a row: with a checkpoint, of whole blocks
     double inv;                  // 1 / features
     float eps;
@@ -162,7 +174,7 @@ __device__ __forceinline__ void put_values(const Fwd &a, typename Elem<TYPE>::T 
     if (!y) return;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) n[i] = n[i] * sc[i] + b[i];
-    store_values<TYPE>(y + r * a.y_stride + col, left, n);
+    write_values<TYPE>(y + r * a.y_stride + col, left, n, a.past);
 }
 
 template <int TYPE, int G, int I, bool KEEP>
@@ -170,7 +182,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G)
 k_norm_fwd(const typename Elem<TYPE>::T *x, typename Elem<TYPE>::T *y, Fwd a)
 {
     constexpr int VEC = Row<TYPE>::VEC, NT = G < 256 ? 256 : G, AT_ONCE = NT / G;
-    constexpr bool HOLD = I <= 2, AHEAD = I <= 4;
+    constexpr bool HOLD = I <= 2, AHEAD = G < 1024 || !KEEP;  // (registers)
     using T = typename Elem<TYPE>::T;
     __shared__ double sh[2][2 * NT / 64];
     const int t = threadIdx.x % G, step = (int)gridDim.x * AT_ONCE;
@@ -293,6 +305,7 @@ k_norm_fwd_values(const typename Elem<TYPE>::T *x, typename Elem<TYPE>::T *y, Fw
 
 // ---- backward -------------------------------------------------------------------------
 struct Bwd {
+    bool past;  // dx past the caches
     int rows, features, chunks;
     int64_t stride, d_stride, dx_stride;
     const float *stats, *scales;
@@ -352,26 +365,51 @@ __device__ __forceinline__ float2 stats_of(const Bwd &a, int r)
     return make_float2(a.stats[2 * (size_t)r], a.stats[2 * (size_t)r + 1]);
 }
 
+// A workgroup of 1024 threads has 128 registers each: with four chunks a thread and
+// four ahead, the sums of the parameters' gradients lie in LDS.
+template <int G, int I> constexpr int bwd_lds()
+{
+    return G == 1024 && I == 4 ? 2 * 1024 * I * (int)sizeof(float4) : 0;
+}
+
 template <int TYPE, int G, int I, bool KEPT>
 __global__ void __launch_bounds__(G < 256 ? 256 : G)
 k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
            typename Elem<TYPE>::T *dx, Bwd a, float inv)
 {
     constexpr int VEC = Row<TYPE>::VEC, NT = G < 256 ? 256 : G, AT_ONCE = NT / G;
-    constexpr bool HOLD = I * VEC <= 16, AHEAD = I * VEC <= 16;  // (registers)
+    constexpr bool HOLD = I * VEC <= 16 && G < 1024, AHEAD = I * VEC <= 16;
+    constexpr bool IN_LDS = bwd_lds<G, I>() > 0;  // the gradients' sums: a float4 of each thread after the other
     using P = Pair<TYPE, KEPT>;
     __shared__ float sh[2][2 * NT / 64];
     __shared__ float join[AT_ONCE > 1 ? NT * I * VEC : 1];
     const int t = threadIdx.x % G, step = (int)gridDim.x * AT_ONCE;
     int r = (int)blockIdx.x * AT_ONCE + threadIdx.x / G;
-    float sc[HOLD ? I * VEC : VEC], ds[I * VEC], db[I * VEC];
+    extern __shared__ __align__(16) float4 in_lds[];
+    float sc[HOLD ? I * VEC : VEC], ds[IN_LDS ? VEC : I * VEC], db[IN_LDS ? VEC : I * VEC];
     if (HOLD) {
 #pragma unroll
         for (int i = 0; i < I; ++i)
             load_floats<VEC>(a.scales, (t + i * G) * VEC, a.features - (t + i * G) * VEC, 1.f, sc + i * VEC);
     }
+    if (IN_LDS) {
 #pragma unroll
-    for (int i = 0; i < I * VEC; ++i) ds[i] = db[i] = 0.f;
+        for (int i = 0; i < 2 * I; ++i) in_lds[i * G + t] = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < I * VEC; ++i) ds[i] = db[i] = 0.f;
+    }
+    // a chunk's share of these sums, in turn with those of the row
+    auto fetch = [&](int i) {
+        if (!IN_LDS) return;
+        __builtin_memcpy(ds, &in_lds[i * G + t], 16);
+        __builtin_memcpy(db, &in_lds[(I + i) * G + t], 16);
+    };
+    auto put = [&](int i) {
+        if (!IN_LDS) return;
+        __builtin_memcpy(&in_lds[i * G + t], ds, 16);
+        __builtin_memcpy(&in_lds[(I + i) * G + t], db, 16);
+    };
     P c[I], ahead[AHEAD ? I : 1];
     float2 st, next;
     auto load = [&](int row, P *to, float2 &s) {
@@ -389,15 +427,18 @@ k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
             float d[VEC], n[VEC];
             c[i].values(st, d, n);
             if (!HOLD && dx) load_floats<VEC>(a.scales, (t + i * G) * VEC, a.features - (t + i * G) * VEC, 1.f, sc);
+            const int at = IN_LDS ? 0 : i * VEC;
+            fetch(i);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 // (deltas behind the last value are 0, x_norm is any number there)
                 const float g = d[e] * sc[(HOLD ? i * VEC : 0) + e];
                 sums[0] += g;
                 sums[1] = fmaf(g, n[e], sums[1]);
-                ds[i * VEC + e] = fmaf(d[e], n[e], ds[i * VEC + e]);
-                db[i * VEC + e] += d[e];
+                ds[at + e] = fmaf(d[e], n[e], ds[at + e]);
+                db[at + e] += d[e];
             }
+            put(i);
         }
         if (dx) {
             row_sums<G, 2>(sums, sh[turn]);
@@ -416,7 +457,7 @@ k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
 #pragma unroll
                 for (int e = 0; e < VEC; ++e)
                     d[e] = st.y * (d[e] * sc[(HOLD ? i * VEC : 0) + e] - m1 - n[e] * m2);
-                store_values<TYPE>(dx + r * a.dx_stride + col, a.features - col, d);
+                write_values<TYPE>(dx + r * a.dx_stride + col, a.features - col, d, a.past);
             }
         }
         if (AHEAD) {
@@ -450,9 +491,10 @@ k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
 #pragma unroll
             for (int i = 0; i < I; ++i) {
                 const int col = (t + i * G) * VEC;
+                if (IN_LDS) __builtin_memcpy(v, &in_lds[(which * I + i) * G + t], 16);
 #pragma unroll
                 for (int e = 0; e < VEC; e += 4)
-                    store_values<ACH_F32>(to + col + e, a.features - col - e, v + i * VEC + e);
+                    store_values<ACH_F32>(to + col + e, a.features - col - e, v + (IN_LDS ? 0 : i * VEC) + e);
             }
         }
     }
@@ -518,7 +560,7 @@ k_norm_bwd_values(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>
         m1 *= inv, m2 *= inv;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) d[e] = st.y * (d[e] * sc[e] - m1 - n[e] * m2);
-        store_values<TYPE>(dx + r * a.dx_stride + col, left, d);
+        write_values<TYPE>(dx + r * a.dx_stride + col, left, d, a.past);
     }
     if (!a.partial) return;
     float *const to = a.partial + (size_t)span * a.features + col;
@@ -529,34 +571,37 @@ k_norm_bwd_values(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>
     }
 }
 
-// The partial sums of a column, an eighth of them by each of eight threads.
-__global__ void __launch_bounds__(256)
+// The partial sums of 32 columns, a 32nd of each by each of 32 threads.
+constexpr int JOIN = 32;
+__global__ void __launch_bounds__(JOIN * 32)
 k_norm_bwd_join(const float *partial, int spans, int features, float *scale_updates,
                 float *bias_updates, int accumulate)
 {
-    __shared__ double sh[8][32];
+    __shared__ double sh[JOIN][32];
     float *const to = blockIdx.y ? bias_updates : scale_updates;
     if (!to) return;
-    const int lane = threadIdx.x & 31, eighth = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
     const int j = blockIdx.x * 32 + lane;
     double s = 0;
     if (j < features) {
         const float *p = partial + (size_t)blockIdx.y * spans * features + j;
-        int i = eighth;
-        for (; i + 24 < spans; i += 32) {  // four loads in flight
+        int i = share;
+        for (; i + 3 * JOIN < spans; i += 4 * JOIN) {  // four loads in flight
             float v[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = p[(size_t)(i + 8 * u) * features];
+            for (int u = 0; u < 4; ++u) v[u] = p[(size_t)(i + u * JOIN) * features];
 #pragma unroll
             for (int u = 0; u < 4; ++u) s += v[u];
         }
-        for (; i < spans; i += 8) s += p[(size_t)i * features];
+        for (; i < spans; i += JOIN) s += p[(size_t)i * features];
     }
-    sh[eighth][lane] = s;
+    sh[share][lane] = s;
     __syncthreads();
-    if (eighth || j >= features) return;
-#pragma unroll
-    for (int i = 1; i < 8; ++i) s += sh[i][lane];
+    for (int n = JOIN / 2; n; n >>= 1) {
+        if (share < n) sh[share][lane] = s += sh[share + n][lane];
+        __syncthreads();
+    }
+    if (share || j >= features) return;
     to[j] = accumulate ? (float)(to[j] + s) : (float)s;
 }
 
@@ -577,6 +622,11 @@ bool row_stride(int64_t *stride, int features)
 }
 
 size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+bool past_caches(const ach_layernorm_desc &d)
+{
+    return (size_t)d.rows * d.features * elem_size(d.type) > (size_t)32 << 20;
+}
 
 // Chunks of a row, in whole blocks of a checkpoint.
 int chunks_of(const ach_layernorm_desc &d)
@@ -605,15 +655,29 @@ template <class F> bool for_kind(int chunks, int most, F f)
     else if (chunks <= 128) f(Kind<64, 2>());
     else if (chunks <= 256) f(Kind<256, 1>());
     else if (chunks <= 512) f(Kind<256, 2>());
-    else if (chunks <= 1024) f(Kind<256, 4>());
+    else if (chunks <= 1024) f(Kind<512, 2>());
     else if (chunks <= 2048) f(Kind<512, 4>());
-    else if (chunks <= 4096) f(Kind<512, 8>());
-    else f(Kind<512, 16>());
+    else f(Kind<1024, 4>());
     return true;
 }
-// A row's chunks that fit the registers: 16 of a thread's 512 in the forward pass;
-// in the backward pass 8 of 4 values or 4 of 8, for which it holds two sums each.
-constexpr int FWD_CHUNKS = 8192;
+template <class F> bool for_bwd_kind(int chunks, int most, F f)
+{
+    if (chunks > most) return false;
+    if (chunks <= 16) f(Kind<16, 1>());
+    else if (chunks <= 64) f(Kind<64, 1>());
+    else if (chunks <= 128) f(Kind<64, 2>());
+    else if (chunks <= 256) f(Kind<256, 1>());
+    else if (chunks <= 512) f(Kind<256, 2>());
+    else if (chunks <= 1024) f(Kind<256, 4>());
+    else if (chunks <= 2048) f(Kind<1024, 2>());
+    else f(Kind<1024, 4>());
+    return true;
+}
+// A row's chunks that fit the registers, four of each thread's, which a workgroup
+// of 1024 has 128 of; the backward pass holds two sums for each value, those of 8
+// values a chunk for two chunks.  (Twice as many in the forward pass, eight
+// chunks a thread: 1000 x 60000 bf16 91 us, in parts 78.)
+constexpr int FWD_CHUNKS = 4096;
 constexpr int bwd_chunks(int type) { return type == ACH_F32 ? 4096 : 2048; }
 
 void in_parts(int chunks, int rows, Plan *p)
@@ -635,7 +699,7 @@ Plan fwd_plan(const ach_layernorm_desc &d)
     const int chunks = chunks_of(d);
     if (!for_kind(chunks, FWD_CHUNKS, [&](auto k) {
             const int at_once = k.NT / k.G, all = (d.rows + at_once - 1) / at_once;
-            p.grid = min(all, k.NT == 512 ? 1024 : 2048);
+            p.grid = min(all, k.NT >= 512 ? 1024 : 2048);
         })) {
         in_parts(chunks, d.rows, &p);
         p.first = (size_t)d.rows * p.parts * sizeof(double2);
@@ -648,10 +712,10 @@ Plan bwd_plan(const ach_layernorm_desc &d)
 {
     Plan p = {};
     const int chunks = chunks_of(d);
-    if (!for_kind(chunks, bwd_chunks(d.type), [&](auto k) {
+    if (!for_bwd_kind(chunks, bwd_chunks(d.type), [&](auto k) {
             const int at_once = k.NT / k.G, all = (d.rows + at_once - 1) / at_once;
             // at least so many that no chain of sums is longer than 256 rows
-            p.grid = p.spans = min(all, max(k.NT == 512 ? 256 : 512, (all + 255) / 256));
+            p.grid = p.spans = min(all, max(k.NT == 1024 ? 256 : 512, (all + 255) / 256));
         })) {
         in_parts(chunks, d.rows, &p);
         p.tiles = (chunks + PART_NT - 1) / PART_NT;
@@ -685,10 +749,18 @@ int bwd_go(const Plan &p, const void *delta, const void *x, void *dx, const Bwd 
 {
     using T = typename Elem<TYPE>::T;
     const float inv = (float)(1. / a.features);
-    if (!for_kind(chunks, bwd_chunks(TYPE), [&](auto k) {
-            if constexpr (k.G * k.I <= bwd_chunks(TYPE))
-                hipLaunchKernelGGL((k_norm_bwd<TYPE, k.G, k.I, KEPT>), dim3(p.grid), dim3(k.NT), 0, st,
-                                   (const T *)delta, (const T *)x, (T *)dx, a, inv);
+    int rc = ACH_OK;
+    if (!for_bwd_kind(chunks, bwd_chunks(TYPE), [&](auto k) {
+            if constexpr (k.G * k.I <= bwd_chunks(TYPE)) {
+                constexpr int lds = bwd_lds<k.G, k.I>();
+                const auto kern = &k_norm_bwd<TYPE, k.G, k.I, KEPT>;
+                if (lds > 64 * 1024)
+                    rc = check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern),
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+                if (rc) return;
+                hipLaunchKernelGGL(kern, dim3(p.grid), dim3(k.NT), lds, st, (const T *)delta,
+                                   (const T *)x, (T *)dx, a, inv);
+            }
         })) {
         if (dx)
             hipLaunchKernelGGL((k_norm_bwd_sums<TYPE, KEPT>), dim3((unsigned)(a.rows * p.parts)),
@@ -696,7 +768,7 @@ int bwd_go(const Plan &p, const void *delta, const void *x, void *dx, const Bwd 
         hipLaunchKernelGGL((k_norm_bwd_values<TYPE, KEPT>), dim3((unsigned)(p.tiles * p.spans)),
                            dim3(PART_NT), 0, st, (const T *)delta, (const T *)x, (T *)dx, a, inv);
     }
-    return check_launch();
+    return rc ? rc : check_launch();
 }
 
 }  // namespace
@@ -726,7 +798,7 @@ int ach_layernorm_fwd(const ach_layernorm_desc *desc, const void *x, const float
     const Plan p = fwd_plan(d);
     if (p.bytes && (!ws || ws_bytes < p.bytes || !aligned(ws, 16))) return ACH_EWORKSPACE;
     if (d.rows == 0) return ACH_OK;
-    Fwd a = {d.rows, d.features, 0, 1. / d.features, d.eps, d.stride, y_stride, scales, biases,
+    Fwd a = {past_caches(d), d.rows, d.features, 0, 1. / d.features, d.eps, d.stride, y_stride, scales, biases,
              stats, {}, (double2 *)ws, (float *)((char *)ws + p.first), p.parts, p.span};
     if (checkpoint) a.k = kept(checkpoint, d.rows, d.features);
     hipStream_t st = as_stream(s);
@@ -771,7 +843,7 @@ int ach_layernorm_bwd(const ach_layernorm_desc *desc, const void *delta, int64_t
     float *const partial = (float *)((char *)ws + p.partial);
     const int vec = 16 / (int)size;
     if (d.rows) {
-        Bwd a = {d.rows, d.features, (d.features + vec - 1) / vec, d.stride, delta_stride, dx_stride,
+        Bwd a = {past_caches(d), d.rows, d.features, (d.features + vec - 1) / vec, d.stride, delta_stride, dx_stride,
                  stats, scales, {}, (float2 *)ws, p.parts, p.span, updates ? partial : nullptr,
                  p.rows_of, p.spans};
         if (checkpoint) a.k = kept(checkpoint, d.rows, d.features);
@@ -784,7 +856,8 @@ int ach_layernorm_bwd(const ach_layernorm_desc *desc, const void *delta, int64_t
         if (rc) return rc;
     }
     if (updates) {
-        hipLaunchKernelGGL(k_norm_bwd_join, dim3((unsigned)((d.features + 31) / 32), 2), dim3(256), 0,
+        hipLaunchKernelGGL(k_norm_bwd_join, dim3((unsigned)((d.features + 31) / 32), 2),
+                           dim3(JOIN * 32), 0,
                            st, (const float *)partial, p.spans, d.features, scale_updates,
                            bias_updates, accumulate);
         return check_launch();
