@@ -5,11 +5,22 @@
 // delta (its first 8 bits, the next 8, the last 8; one piece for bf16, two for
 // fp16, three for fp32): every product is exact and is summed in fp32.
 //
-// Eight waves of 64 outputs x 64 inputs each, as a tile of 256 x 128 or 128 x
-// 256.  A stage of 32 rows of both operands is loaded two stages ahead, turned
-// into bf16 and stored as it lies in memory, [row][column]; the matrix
+// Tiles of 256 outputs x 128 inputs or 128 x 256, a wave 64 x 64 (bf16 also 128 x
+// 64) of it.  A stage of 32 rows of both operands is loaded two stages ahead,
+// turned into bf16 and stored as it lies in memory, [row][column]; the matrix
 // instructions want 8 rows of a column in a lane, which the transposing LDS loads
-// give: 16 lanes read 4 rows x 16 columns, and each gets a column of it.
+// give: 16 lanes read 4 rows x 16 columns, and each gets a column of it.  Few tiles
+// share out the rows in slices, whose sums a second launch adds up in order.
+//
+// Bound by the matrix units on many rows: 8192 x 8192 -> 4096 (a matrix product of
+// the library at 8192^3 in bf16: 1250 TFLOP/s) bf16 527 us, 1043 TFLOP/s; fp32 1355
+// us, three passes of 405; 16384 x 4096 -> 1024 bf16 157 us, of which 15 are the
+// four slices' sums.  By the writing of dw on few: 128 x 9216 -> 4096 fp32 60 us
+// for 154 MB; its workgroups write in step, so that neither the loads nor the
+// products of a next tile lie behind it.  What it took on 16384 x 4096 -> 1024 bf16:
+// one stage ahead 399 us, two 233; offsets in the loads' windows instead of 64-bit
+// addresses and clamps (100 vector instructions for 8 of the matrix) 189; waves of
+// 128 x 64 162; the operands' loads among the matrix instructions 157.
 #include "checkpoint.hpp"
 #include "pieces.hpp"
 
@@ -35,7 +46,8 @@ struct Fc {
     float *dw, *part;  // part: [slices][outputs][inputs], or null
     int accumulate;
     int span;          // rows of a slice
-    int ti, to;        // tiles along the inputs and the outputs
+    int ti;            // tiles along the inputs
+    bool past;         // dw past the caches
 };
 
 // The upper halves of two floats: their first 8 bits of precision as bf16.
@@ -137,8 +149,8 @@ template <int TYPE, int WO, int WI, int MO> struct Tile {
     static constexpr size_t LDS = 2 * sizeof(Stage);
 };
 
-template <int TYPE, int WO, int WI, int MO, int LEAST>
-__global__ void __launch_bounds__(64 * WO * WI, LEAST)
+template <int TYPE, int WO, int WI, int MO>
+__global__ void __launch_bounds__(64 * WO * WI, 2)
 k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
 {
     using S = Tile<TYPE, WO, WI, MO>;
@@ -152,15 +164,13 @@ k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wo = wave % WO, wi = wave / WO;
     // each XCD, which takes every eighth workgroup, gets a contiguous range of
-    // tiles, in blocks of 8 outputs' tiles: they share the operands in its L2
+    // tiles, which share their operands in its L2
     int id = blockIdx.x;
     {
         const int G = gridDim.x, g8 = G >> 3, r8 = G & 7, xcd = id & 7;
         id = xcd * g8 + min(xcd, r8) + (id >> 3);
     }
-    const int block = id / (8 * a.ti), in = id - block * 8 * a.ti;
-    const int high = min(8, a.to - block * 8);
-    const int o0 = (block * 8 + in % high) * S::O, i0 = in / high * S::I;
+    const int o0 = id / a.ti * S::O, i0 = id % a.ti * S::I;
     const int r0 = (int)blockIdx.y * a.span, r1 = min((int64_t)a.rows, (int64_t)r0 + a.span);
 
     // A thread's share of a stage.  What lies behind the last output or input is
@@ -309,18 +319,30 @@ k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
                 if (o + r >= a.outputs) continue;
                 float v = P > 1 ? hi[i][j][e] + lo[P > 1 ? i : 0][j][e] : hi[i][j][e];
                 if (add) v += p[(size_t)r * a.inputs];
-                p[(size_t)r * a.inputs] = v;
+                if (a.past) __builtin_nontemporal_store(v, p + (size_t)r * a.inputs);
+                else p[(size_t)r * a.inputs] = v;
             }
         }
 }
 
+// dw (+)= the slices' sums, four values and four slices in flight a thread.
 __global__ void __launch_bounds__(256)
 k_fc_wgrad_join(const float *part, size_t n, int slices, float *dw, int accumulate)
 {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        float s = accumulate ? dw[i] : 0.f;
-        for (int k = 0; k < slices; ++k) s += part[k * n + i];
-        dw[i] = s;
+    for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (size_t)gridDim.x * 1024) {
+        const int left = (int)(n - i < 4 ? n - i : 4);
+        float s[4], v[4][4];
+        load_floats<4>(accumulate ? dw : nullptr, i, left, 0.f, s);
+        for (int k = 0; k < slices; k += 4) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                load_floats<4>(k + u < slices ? part : nullptr, (size_t)(k + u) * n + i, left, 0.f, v[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] += v[u][e];
+        }
+        store_values<ACH_F32>(dw + i, left, s);
     }
 }
 
@@ -345,15 +367,16 @@ int tiles_of(int n, int tile) { return (n + tile - 1) / tile; }
 Plan fc_plan(const ach_fc_desc &d)
 {
     Plan p;
+    const int stages = tiles_of(d.rows, DEPTH);
     const int64_t high = (int64_t)tiles_of(d.outputs, 256) * tiles_of(d.inputs, 128),
                   wide = (int64_t)tiles_of(d.outputs, 128) * tiles_of(d.inputs, 256);
     p.high = high < wide || (high == wide && d.type == ACH_BF16);
     p.to = tiles_of(d.outputs, p.high ? 256 : 128);
     p.ti = tiles_of(d.inputs, p.high ? 128 : 256);
     const int64_t tiles = (int64_t)p.ti * p.to;
-    const int stages = tiles_of(d.rows, DEPTH);
-    const int full = d.type == ACH_BF16 && p.high ? 512 : 256;  // workgroups that run at once
-    int slices = tiles < full ? (int)(full / tiles) : 1;
+    int slices = tiles < 256 ? (int)(256 / tiles) : 1;
+    if (d.type == ACH_BF16 && p.high && tiles < 512 && stages / slices >= 256)
+        slices = (int)(512 / tiles);
     if (slices > stages / 4) slices = stages / 4;
     if (slices > MOST_SLICES) slices = MOST_SLICES;
     if (slices < 1) slices = 1;
@@ -365,11 +388,11 @@ Plan fc_plan(const ach_fc_desc &d)
     return p;
 }
 
-template <int TYPE, int WO, int WI, int MO, int LEAST>
+template <int TYPE, int WO, int WI, int MO>
 int fc_go(const Plan &p, const void *delta, const Fc &a, hipStream_t st)
 {
     using S = Tile<TYPE, WO, WI, MO>;
-    const auto kern = &k_fc_wgrad<TYPE, WO, WI, MO, LEAST>;
+    const auto kern = &k_fc_wgrad<TYPE, WO, WI, MO>;
     if (S::LDS > 64 * 1024) {
         const int rc = check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::LDS));
@@ -378,6 +401,16 @@ int fc_go(const Plan &p, const void *delta, const Fc &a, hipStream_t st)
     hipLaunchKernelGGL(kern, dim3((unsigned)(p.ti * p.to), (unsigned)p.slices), dim3(S::THREADS),
                        S::LDS, st, (const typename Elem<TYPE>::T *)delta, a);
     return check_launch();
+}
+
+// bf16 deltas, whose tiles cost the matrix units a third of the others' time, need
+// fewer loads of operands from LDS: four waves of 128 x 64, two workgroups a
+// compute unit.
+template <int TYPE> int fc_tiles(const Plan &p, const void *delta, const Fc &a, hipStream_t st)
+{
+    if (!p.high) return fc_go<TYPE, 2, 4, 2>(p, delta, a, st);
+    if constexpr (TYPE == ACH_BF16) return fc_go<TYPE, 2, 2, 4>(p, delta, a, st);
+    else return fc_go<TYPE, 4, 2, 2>(p, delta, a, st);
 }
 
 }  // namespace
@@ -406,18 +439,16 @@ int ach_fc_bwd_filter_checkpoint(const ach_fc_desc *desc, const void *checkpoint
     if ((int64_t)p.ti * p.to > 0x7fffffff) return ACH_EINVAL;
     if (p.bytes && (!ws || ws_bytes < p.bytes || !aligned(ws, 16))) return ACH_EWORKSPACE;
     const Fc a = {d.rows, d.inputs, d.outputs, d.stride, kept(checkpoint, d.rows, d.inputs), dw,
-                  p.slices > 1 ? (float *)ws : nullptr, accumulate, p.span, p.ti, p.to};
+                  p.slices > 1 ? (float *)ws : nullptr, accumulate, p.span, p.ti,
+                  p.slices == 1 && (size_t)d.outputs * d.inputs * sizeof(float) > (size_t)32 << 20};
     hipStream_t st = as_stream(s);
     int rc;
-#define CALL(TYPE)                                                                                 \
-    rc = !p.high ? fc_go<TYPE, 2, 4, 2, 2>(p, delta, a, st)                                        \
-         : TYPE == ACH_BF16 ? fc_go<TYPE, 2, 2, TYPE == ACH_BF16 ? 4 : 2, 2>(p, delta, a, st)      \
-                            : fc_go<TYPE, 4, 2, 2, 2>(p, delta, a, st)
+#define CALL(TYPE) rc = fc_tiles<TYPE>(p, delta, a, st)
     FOR_TYPE(d.type, CALL);
 #undef CALL
     if (rc || p.slices == 1) return rc;
     const size_t n = (size_t)d.outputs * d.inputs;
-    hipLaunchKernelGGL(k_fc_wgrad_join, dim3(grid_for(n, 256, 4096)), dim3(256), 0, st,
+    hipLaunchKernelGGL(k_fc_wgrad_join, dim3(grid_for((n + 3) / 4, 256, 4096)), dim3(256), 0, st,
                        (const float *)ws, n, p.slices, dw, accumulate);
     return check_launch();
 }
