@@ -32,7 +32,7 @@ F32, BF16, F16 = 0, 1, 2  # element types of logits, layer norm rows and checkpo
 TOP_MAX = 128
 DISTILL_RENORM, DISTILL_TAIL = 0, 1
 
-AN_CONVOLUTIONAL, AN_MAXPOOL, AN_AVGPOOL, AN_DROPOUT, AN_SOFTMAX = 0, 1, 2, 3, 4
+AN_CONVOLUTIONAL, AN_MAXPOOL, AN_AVGPOOL, AN_DROPOUT, AN_SOFTMAX, AN_LAYERNORM = range(6)
 
 # an_policy (the reference's LearningRatePolicy order)
 (POLICY_CONSTANT, POLICY_STEP, POLICY_EXP, POLICY_POLY, POLICY_STEPS, POLICY_SIG,
@@ -231,6 +231,9 @@ _NET = {
     "an_add_avgpool": (_i, [_vp]),
     "an_add_dropout": (_i, [_vp, _f]),
     "an_add_softmax": (_i, [_vp, _i, _f]),
+    "an_add_layernorm": (_i, [_vp, _f]),
+    "an_set_checkpoints": (_i, [_vp, _i]),
+    "an_device_bytes": (_sz, [_vp]),
     "an_set_hyper": (None, [_vp, _f, _f, _f]),
     "an_set_dropout_seed": (None, [_vp, _u64]),
     "an_set_policy": (_i, [_vp, _i, _i, _f, _f, _f, _i, _i, _i, _vp, _vp]),
@@ -409,6 +412,9 @@ class DeviceArray:
             pass
 
 
+_BUFFER_TYPES = {14: np.int32, 17: np.uint8}  # of an_layer_buffer, else float32
+
+
 class Network:
     """Thin owner of an ``an_network*`` built layer by layer."""
 
@@ -484,6 +490,20 @@ class Network:
 
     def softmax(self, groups=1, temperature=1.0):
         return self.lib.an_add_softmax(self.h, groups, temperature)
+
+    def layernorm(self, eps=1e-5):
+        r = self.lib.an_add_layernorm(self.h, eps)
+        if r < 0:
+            raise ValueError(f"an_add_layernorm: {r}")
+        return r
+
+    def checkpoints(self, on=True):
+        """an_set_checkpoints (before finalize): batch-norm layers keep their
+        pre-norm tensor in 8 bits"""
+        check(self.lib.an_set_checkpoints(self.h, int(on)), "an_set_checkpoints")
+
+    def device_bytes(self) -> int:
+        return self.lib.an_device_bytes(self.h)
 
     def hyper(self, lr, momentum, decay):
         self.lib.an_set_hyper(self.h, lr, momentum, decay)
@@ -638,15 +658,14 @@ class Network:
         p = self.lib.an_layer_buffer(self.h, layer, which, C.byref(n))
         if not p or n.value == 0:
             return None
-        dt = np.int32 if which == 14 else np.float32
-        out = np.empty(n.value, dtype=dt)
+        out = np.empty(n.value, dtype=_BUFFER_TYPES.get(which, np.float32))
         check(ops().ach_memcpy_d2h(out.ctypes.data, p, out.nbytes, self.stream), "d2h")
         return out
 
     def set_buffer(self, layer: int, which: int, values: np.ndarray):
         n = _sz()
         p = self.lib.an_layer_buffer(self.h, layer, which, C.byref(n))
-        v = np.ascontiguousarray(values, dtype=np.int32 if which == 14 else np.float32).ravel()
+        v = np.ascontiguousarray(values, dtype=_BUFFER_TYPES.get(which, np.float32)).ravel()
         assert p and v.size == n.value, (layer, which, v.size, n.value)
         check(ops().ach_memcpy_h2d(p, v.ctypes.data, v.nbytes, self.stream), "h2d")
 

@@ -183,6 +183,7 @@ static const char *const NET_KEYS[] = {
     "contrastive_color", "unsupervised", "label_smooth_eps", "resize_step", "attention",
     "adversarial_lr", "max_chart_loss", "angle", "aspect", "saturation", "exposure", "hue",
     "power", "policy", "burn_in", "step", "scale", "steps", "scales", "seq_scales", "gamma",
+    "activation_checkpoints", /* this project's: an_set_checkpoints */
     NULL};
 static const char *const LAYER_KEYS[] = { /* createLayer + createNetwork, every layer */
     "truth", "onlyforward", "stopbackward", "dontsave", "dontload", "numload",
@@ -202,6 +203,7 @@ static const char *const DROPOUT_KEYS[] = {
     "probability", "dropblock", "dropblock_size_rel", "dropblock_size_abs", NULL};
 static const char *const SOFTMAX_KEYS[] = {
     "groups", "temperature", "spatial", "noloss", "tree", NULL};
+static const char *const LAYERNORM_KEYS[] = {"eps", NULL}; /* this project's */
 static const char *const NO_KEYS[] = {NULL};
 
 static int in_list(const char *const *l, const char *k)
@@ -364,6 +366,10 @@ an_network *an_parse_cfg_unfinalized(const char *path)
         an_set_hyper(net, getf(g, "learning_rate", .001f), getf(g, "momentum", .9f),
                      getf(g, "decay", .0001f));
         if (an_set_subdivisions(net, subdivs) || parse_policy(net, g)) goto fail;
+        if (an_set_checkpoints(net, geti(g, "activation_checkpoints", 0))) {
+            fprintf(stderr, "an_parse_cfg: [net] activation_checkpoints is 0 or 1\n");
+            goto fail;
+        }
     }
     for (int i = 1; i < ng; ++i) {
         const cfg_group *g = &gs[i];
@@ -419,6 +425,9 @@ an_network *an_parse_cfg_unfinalized(const char *path)
             report_unused(g, DROPOUT_KEYS, 1);
             if (unsupported(g, "dropblock", 0)) goto fail;
             rc = an_add_dropout(net, getf(g, "probability", .2f));
+        } else if (!strcmp(g->name, "layernorm")) {
+            report_unused(g, LAYERNORM_KEYS, 1);
+            rc = an_add_layernorm(net, getf(g, "eps", 1e-5f));
         } else if (!strcmp(g->name, "softmax") || !strcmp(g->name, "soft")) {
             report_unused(g, SOFTMAX_KEYS, 1);
             if (unsupported(g, "spatial", 0) || unsupported(g, "noloss", 0) ||

@@ -54,6 +54,8 @@ struct an_network {
     size_t nweights_total;
     float *bflat, *bvflat;         /* biases (+scales) / their updates       */
     size_t nbias_total;
+    int checkpoints;               /* an_set_checkpoints */
+    float *x_shared;               /* the batch-norm layers' x with it      */
     float *wtflat, *wftflat;       /* k-major / flipped k-major filters    */
     /* weight gradients run on a second stream, overlapping the input-gradient
      * chain: its own workspace, one "delta ready" event per layer and one
@@ -219,12 +221,16 @@ static int conv_forward(an_network *net, an_layer *l, an_state st)
         /* conv output goes straight into NormData.x; BN writes output */
         AN_CHECK(forward_sums(&d, st, l, NULL, ACH_LINEAR, l->x, s));
         const int act = fusable(l->activation) ? l->activation : ACH_LINEAR;
-        if (st.train)
+        if (st.train) {
             AN_CHECK(ach_bn_train_fwd_from_x(l->x, l->output, l->batch, l->n, spatial,
                                              l->scales, l->biases, l->mean, l->variance,
                                              l->rolling_mean, l->rolling_variance, act,
                                              st.workspace, st.workspace_bytes, s));
-        else /* forwardNormCPU test branch: normalizeByRoll (NormData.c:291-326) */
+            if (l->x_kept) {
+                const ach_checkpoint_desc k = {l->batch, l->outputs, ACH_F32, 0};
+                AN_CHECK(ach_checkpoint_pack(&k, l->x, l->x_kept, s));
+            }
+        } else /* forwardNormCPU test branch: normalizeByRoll (NormData.c:291-326) */
             AN_CHECK(ach_bn_infer(l->x, l->output, l->batch, l->n, spatial, l->scales,
                                   l->biases, l->rolling_mean, l->rolling_variance, act, s));
         if (!fusable(l->activation))
@@ -274,11 +280,15 @@ static int conv_backward(an_network *net, an_layer *l, an_state st)
     const size_t nout = (size_t)l->batch * l->outputs;
     if (l->batch_normalize) {
         int act = ACH_LINEAR;
-        if ((l->activation == ACH_LEAKY || l->activation == ACH_RELU) &&
+        if ((l->activation == ACH_LEAKY || l->activation == ACH_RELU) && !l->x_kept &&
             !output_masked_unreverted(net, l))
             act = l->activation; /* gradient fused into the BN passes */
-        else
+        else /* (rounded values of x may give a pre-activation another sign) */
             AN_CHECK(ach_gradient(l->output, nout, l->activation, l->delta, s));
+        if (l->x_kept) {
+            const ach_checkpoint_desc k = {l->batch, l->outputs, ACH_F32, 0};
+            AN_CHECK(ach_checkpoint_unpack(&k, l->x_kept, l->x, s));
+        }
         AN_CHECK(ach_bn_bwd(l->delta, l->batch, l->n, spatial, l->x, NULL, l->mean,
                             l->variance, l->scales, l->biases, l->scale_updates,
                             l->mean_delta, l->variance_delta, act, st.workspace,
@@ -645,6 +655,68 @@ int an_add_softmax(an_network *net, int groups, float temperature)
     return net->n++;
 }
 
+/* ======================================================================== */
+/* Layer norm: an image's inputs normalised among themselves.               */
+static ach_layernorm_desc layernorm_desc(const an_layer *l)
+{
+    const ach_layernorm_desc d = {l->batch, l->inputs, ACH_F32, l->eps, 0};
+    return d;
+}
+
+static int layernorm_forward(an_network *net, an_layer *l, an_state st)
+{
+    const ach_layernorm_desc d = layernorm_desc(l);
+    return ach_layernorm_fwd(&d, st.input, l->scales, l->biases, l->output, 0, l->stats, NULL,
+                             st.workspace, st.workspace_bytes, net->stream);
+}
+
+static int layernorm_backward(an_network *net, an_layer *l, an_state st)
+{
+    const ach_layernorm_desc d = layernorm_desc(l);
+    AN_CHECK(ach_layernorm_bwd(&d, l->delta, 0, st.input, NULL, l->stats, l->scales, st.delta, 0,
+                               l->scale_updates, l->bias_updates, 1, st.workspace,
+                               st.workspace_bytes, net->stream));
+    if (!net->early_update) return ACH_OK;
+    return conv_update(net, l, net->batch * net->subdivisions, net->early_rate, net->momentum,
+                       net->decay);
+}
+
+int an_add_layernorm(an_network *net, float eps)
+{
+    if (!net || !(eps >= 1e-12f && eps <= 1.f)) return ACH_EINVAL;
+    an_layer *l = push_layer(net);
+    if (!l) return ACH_EINVAL;
+    l->type = AN_LAYERNORM;
+    l->n = l->inputs;
+    l->eps = eps;
+    l->out_h = l->h;
+    l->out_w = l->w;
+    l->out_c = l->c;
+    l->outputs = l->inputs;
+    l->forward = layernorm_forward;
+    l->backward = layernorm_backward;
+    l->update = conv_update; /* without weights */
+    return net->n++;
+}
+
+/* layers with parameters, and with scales among them                       */
+static int has_parameters(const an_layer *l)
+{
+    return l->type == AN_CONVOLUTIONAL || l->type == AN_LAYERNORM;
+}
+
+static int has_scales(const an_layer *l)
+{
+    return l->type == AN_LAYERNORM || (l->type == AN_CONVOLUTIONAL && l->batch_normalize);
+}
+
+int an_set_checkpoints(an_network *net, int on)
+{
+    if (!net || net->finalized || (on != 0 && on != 1)) return ACH_EINVAL;
+    net->checkpoints = on;
+    return ACH_OK;
+}
+
 void an_set_hyper(an_network *net, float learning_rate, float momentum, float decay)
 {
     net->learning_rate = learning_rate;
@@ -765,6 +837,10 @@ static size_t layer_ws(const an_layer *l, int batch)
         ws = ws > n ? ws : n;
     } else if (l->type == AN_SOFTMAX) {
         ws = ach_softmax_workspace(batch, l->groups);
+    } else if (l->type == AN_LAYERNORM) {
+        const ach_layernorm_desc d = layernorm_desc(l);
+        const size_t f = ach_layernorm_fwd_workspace(&d), b = ach_layernorm_bwd_workspace(&d);
+        ws = f > b ? f : b;
     }
     return ws;
 }
@@ -783,6 +859,14 @@ static void layout(an_network *net, bump *b)
     net->zero_region = b->dry ? NULL : (float *)(b->base + zstart);
     net->zero_floats = (b->off - zstart) / sizeof(float);
     /* 2. per-layer tensors (flat parameters are carved by an_finalize) */
+    size_t shared = 0;
+    for (int i = 0; i < net->n; ++i) {
+        const an_layer *l = net->layers[i];
+        if (net->checkpoints && l->type == AN_CONVOLUTIONAL && l->batch_normalize &&
+            B * l->outputs > shared)
+            shared = B * l->outputs;
+    }
+    if (shared) net->x_shared = (float *)take(b, sizeof(float) * shared);
     for (int i = 0; i < net->n; ++i) {
         an_layer *l = net->layers[i];
         const size_t bo = B * l->outputs;
@@ -796,7 +880,12 @@ static void layout(an_network *net, bump *b)
         l->output = (float *)take(b, sizeof(float) * bo);
         if (!l->zero_delta) l->delta = (float *)take(b, sizeof(float) * bo);
         if (l->type == AN_CONVOLUTIONAL && l->batch_normalize) {
-            l->x = (float *)take(b, sizeof(float) * bo);
+            if (net->checkpoints) {
+                l->x = net->x_shared;
+                l->x_kept = take(b, ach_checkpoint_bytes(l->batch, l->outputs));
+            } else {
+                l->x = (float *)take(b, sizeof(float) * bo);
+            }
             l->mean = (float *)take(b, sizeof(float) * l->n);
             l->variance = (float *)take(b, sizeof(float) * l->n);
             l->rolling_mean = (float *)take(b, sizeof(float) * l->n);
@@ -807,6 +896,8 @@ static void layout(an_network *net, bump *b)
             l->indexes = (int32_t *)take(b, sizeof(int32_t) * bo);
         } else if (l->type == AN_CONVOLUTIONAL && l->out_h * l->out_w >= 128) {
             l->bias_planes = (double *)take(b, sizeof(double) * B * l->n);
+        } else if (l->type == AN_LAYERNORM) {
+            l->stats = (float *)take(b, sizeof(float) * 2 * B);
         } else if (l->type == AN_SOFTMAX) {
             l->loss = (float *)take(b, sizeof(float) * bo);
             l->cost = (float *)take(b, sizeof(float) * 4);
@@ -951,9 +1042,9 @@ int an_finalize(an_network *net)
     size_t nw = 0, nb = 0;
     for (int i = 0; i < net->n; ++i) {
         an_layer *l = net->layers[i];
-        if (l->type != AN_CONVOLUTIONAL) continue;
+        if (!has_parameters(l)) continue;
         nw += (size_t)((l->nweights + 63) & ~63);
-        nb += (size_t)((l->n + 63) & ~63) * (l->batch_normalize ? 2 : 1);
+        nb += (size_t)((l->n + 63) & ~63) * (has_scales(l) ? 2 : 1);
     }
     const size_t extra = al(sizeof(float) * nw) * 4 + al(sizeof(float) * nb) * 2;
     net->arena_bytes = dry.off + extra;
@@ -989,18 +1080,20 @@ int an_finalize(an_network *net)
     size_t ow = 0, ob = 0;
     for (int i = 0; i < net->n; ++i) {
         an_layer *l = net->layers[i];
-        if (l->type != AN_CONVOLUTIONAL) continue;
-        l->weights = net->wflat + ow;
-        l->weight_updates = net->vflat + ow;
-        /* fully connected geometry: the forward GEMM reads W itself */
-        const ach_conv_desc dl = conv_desc(l);
-        l->weights_kmajor = ach_conv_is_fully_connected(&dl) ? l->weights : net->wtflat + ow;
-        l->weights_flipped = net->wftflat + ow;
-        ow += (size_t)((l->nweights + 63) & ~63);
+        if (!has_parameters(l)) continue;
+        if (l->type == AN_CONVOLUTIONAL) {
+            l->weights = net->wflat + ow;
+            l->weight_updates = net->vflat + ow;
+            /* fully connected geometry: the forward GEMM reads W itself */
+            const ach_conv_desc dl = conv_desc(l);
+            l->weights_kmajor = ach_conv_is_fully_connected(&dl) ? l->weights : net->wtflat + ow;
+            l->weights_flipped = net->wftflat + ow;
+            ow += (size_t)((l->nweights + 63) & ~63);
+        }
         l->biases = net->bflat + ob;
         l->bias_updates = net->bvflat + ob;
         ob += (size_t)((l->n + 63) & ~63);
-        if (l->batch_normalize) {
+        if (has_scales(l)) {
             l->scales = net->bflat + ob;
             l->scale_updates = net->bvflat + ob;
             ob += (size_t)((l->n + 63) & ~63);
@@ -1028,12 +1121,13 @@ int an_finalize(an_network *net)
     AN_CHECK(ach_fill((float *)net->arena, net->arena_bytes / sizeof(float), 0.f, net->stream));
     for (int i = 0; i < net->n; ++i) {
         an_layer *l = net->layers[i];
-        if (l->type != AN_CONVOLUTIONAL) continue;
-        AN_CHECK(ach_memcpy_h2d(l->weights, net->init_w[i], sizeof(float) * l->nweights,
-                                net->stream));
-        free(net->init_w[i]);
-        net->init_w[i] = NULL;
-        if (l->batch_normalize) /* ScaleData.init(1.0) */
+        if (l->type == AN_CONVOLUTIONAL) {
+            AN_CHECK(ach_memcpy_h2d(l->weights, net->init_w[i], sizeof(float) * l->nweights,
+                                    net->stream));
+            free(net->init_w[i]);
+            net->init_w[i] = NULL;
+        }
+        if (has_scales(l)) /* ScaleData.init(1.0) */
             AN_CHECK(ach_fill(l->scales, (size_t)l->n, 1.f, net->stream));
     }
     AN_CHECK(ach_stream_sync(net->stream));
@@ -1213,7 +1307,7 @@ static int update_at_rate(an_network *net, float rate)
          * (updateCPU NNetwork.c:667-680; ConvolutionalLayer.c:959-960) */
         for (int i = 0; i < net->n; ++i) {
             an_layer *l = net->layers[i];
-            if (l->type != AN_CONVOLUTIONAL || !l->train) continue;
+            if (!has_parameters(l) || !l->train) continue;
             AN_CHECK(conv_update(net, l, batch, rate * l->learning_rate_scale, net->momentum,
                                  net->decay));
         }
@@ -1516,14 +1610,18 @@ void *an_layer_buffer(an_network *net, int li, int which, size_t *count)
     case 9: p = l->rolling_variance; n = (size_t)l->n; break;
     case 10: p = l->mean; n = (size_t)l->n; break;
     case 11: p = l->variance; n = (size_t)l->n; break;
-    case 12: p = l->x; n = bo; break;
+    case 12: p = l->x_kept ? NULL : l->x; n = bo; break;
     case 14: p = l->indexes; n = bo; break;
     case 15: p = l->loss; n = bo; break;
+    case 16: p = l->stats; n = 2 * (size_t)l->batch; break;
+    case 17: p = l->x_kept; n = ach_checkpoint_bytes(l->batch, l->outputs); break;
     default: break;
     }
     if (p) *count = n;
     return p;
 }
+
+size_t an_device_bytes(const an_network *net) { return net ? net->arena_bytes : 0; }
 
 double an_step_conv_gflop(const an_network *net)
 {
@@ -1546,14 +1644,20 @@ double an_step_conv_gflop(const an_network *net)
  *   for each convolutional layer in order:
  *     biases[n], (batch_normalize: scales[n], rolling_mean[n],
  *     rolling_variance[n]), weights[nweights]  (float32 each)
+ * and, of this project's own, for each layer norm: biases[n], scales[n].
  * Save writes seen = cur_iteration * batch * subdivisions and, as the
  * reference does (NNetwork.c:125), makes that the network's seen; load
  * sets cur_iteration = seen / (batch * subdivisions) (NNetwork.c:88).     */
 
-/* one conv layer's parameter arrays in file order */
-static int conv_param_arrays(an_layer *l, float **ptr, size_t *cnt)
+/* one layer's parameter arrays in file order */
+static int param_arrays(an_layer *l, float **ptr, size_t *cnt)
 {
     int k = 0;
+    if (l->type == AN_LAYERNORM) {
+        ptr[k] = l->biases; cnt[k++] = (size_t)l->n;
+        ptr[k] = l->scales; cnt[k++] = (size_t)l->n;
+        return k;
+    }
     if (l->connected) {
         /* darknet's connected-layer order: biases, weights, then BN arrays */
         ptr[k] = l->biases; cnt[k++] = (size_t)l->n;
@@ -1594,10 +1698,10 @@ int an_save_weights(an_network *net, const char *path)
     size_t host_cap = 0;
     for (int i = 0; i < net->n && rc == ACH_OK; ++i) {
         an_layer *l = net->layers[i];
-        if (l->type != AN_CONVOLUTIONAL) continue;
+        if (!has_parameters(l)) continue;
         float *ptr[5];
         size_t cnt[5];
-        const int na = conv_param_arrays(l, ptr, cnt);
+        const int na = param_arrays(l, ptr, cnt);
         for (int a = 0; a < na && rc == ACH_OK; ++a) {
             if (cnt[a] > host_cap) {
                 float *nh = (float *)realloc(host, cnt[a] * sizeof(float));
@@ -1666,10 +1770,10 @@ int an_load_weights(an_network *net, const char *path)
     size_t host_cap = 0;
     for (int i = 0; i < net->n && rc == ACH_OK && !feof(fp); ++i) {
         an_layer *l = net->layers[i];
-        if (l->type != AN_CONVOLUTIONAL || l->dontload) continue;
+        if (!has_parameters(l) || l->dontload) continue;
         float *ptr[5];
         size_t cnt[5];
-        const int na = conv_param_arrays(l, ptr, cnt);
+        const int na = param_arrays(l, ptr, cnt);
         for (int a = 0; a < na && rc == ACH_OK; ++a) {
             const int is_w = ptr[a] == l->weights;
             const int is_bn = ptr[a] == l->scales || ptr[a] == l->rolling_mean ||

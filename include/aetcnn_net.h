@@ -38,7 +38,8 @@ typedef enum {
     AN_MAXPOOL = 1,
     AN_AVGPOOL = 2,
     AN_DROPOUT = 3,
-    AN_SOFTMAX = 4
+    AN_SOFTMAX = 4,
+    AN_LAYERNORM = 5
 } an_layer_type;
 
 typedef struct an_network an_network;
@@ -70,7 +71,9 @@ struct an_layer {
     float *scales, *scale_updates;
     float *mean, *variance, *rolling_mean, *rolling_variance;
     float *mean_delta, *variance_delta;
-    float *x;               /* pre-BN conv output (NormData.x)              */
+    float *x;               /* pre-BN conv output (NormData.x); with
+                               an_set_checkpoints one buffer of all layers  */
+    void *x_kept;           /* its checkpoint in 8 bits, or NULL            */
     float *weights_kmajor;  /* filter layouts the conv GEMMs read, refreshed */
     float *weights_flipped; /* from weights at every forward pass            */
     /* maxpool */
@@ -78,6 +81,9 @@ struct an_layer {
     /* dropout */
     float probability;
     int shares_prev;        /* output/delta alias the previous layer's    */
+    /* layer norm (biases and scales above, one each per feature)            */
+    float eps;
+    float *stats;           /* [batch][2] mean and rstd of each image        */
     /* softmax */
     int groups;
     float temperature;
@@ -135,6 +141,11 @@ int an_add_maxpool_xy(an_network *net, int size, int stride_x, int stride_y, int
 int an_add_avgpool(an_network *net);
 int an_add_dropout(an_network *net, float probability);
 int an_add_softmax(an_network *net, int groups, float temperature);
+/* Layer norm: every image's values normalised among themselves, with a scale
+ * and a bias per value (ach_layernorm_fwd / _bwd; eps from 1e-12 to 1).  No
+ * counterpart in the reference.  Scales start at 1, biases at 0; both are
+ * updated as the other layers' biases are (no decay).                      */
+int an_add_layernorm(an_network *net, float eps);
 void an_set_hyper(an_network *net, float learning_rate, float momentum, float decay);
 void an_set_dropout_seed(an_network *net, uint64_t seed);
 
@@ -166,6 +177,14 @@ float an_current_rate(an_network *net);
  * runs one minibatch and updates after every subdivisions-th, with update
  * batch = batch * subdivisions (NNetwork.c:667-680, 762-805).           */
 int an_set_subdivisions(an_network *net, int subdivisions);
+/* Batch-norm layers keep their pre-norm tensor, which only their backward
+ * reads, in 8 bits instead of 32 (on = 1; ach_checkpoint_pack): 0.26 of its
+ * memory, the tensor itself lying in one buffer that these layers share.  The
+ * forward pass and the activations' gradients are the same bit for bit;
+ * what the batch-norm backward makes of the rounded values differs by their
+ * rounding, at most a 127th of the largest of 32 neighbours each.  No
+ * counterpart in the reference.  Before an_finalize (ACH_EINVAL after).    */
+int an_set_checkpoints(an_network *net, int on);
 /* The per-layer cfg options the reference's CPU path acts on (NLayer.h:
  * 115-125, read by NetworkFactory.createLayer / createNetwork,
  * NetworkFactory.c:656-663, 926-935):
@@ -199,6 +218,8 @@ void an_free(an_network *net);
  * step/scale/steps/scales/gamma/max_batches; [convolutional] filters/size/stride/
  * stride_x/stride_y/pad/padding/activation/batch_normalize; [connected]
  * output/activation/batch_normalize (darknet's keys, an_add_connected);
+ * [layernorm] eps (1e-5; an_add_layernorm), [net] activation_checkpoints
+ * (an_set_checkpoints), neither of them darknet's;
  * [maxpool] size/stride/stride_x/stride_y/padding; [avgpool]; [dropout]
  * probability; [softmax] groups/temperature; in every layer section the
  * options of an_layer_options (stopbackward, onlyforward, dontload,
@@ -222,7 +243,8 @@ an_network *an_parse_cfg_unfinalized(const char *path);
  * header int32 {0, 2, 5} + uint64 seen, then per convolutional layer:
  * biases, [scales, rolling_mean, rolling_variance if batch_normalize],
  * weights (float32); per connected layer darknet's order: biases, weights,
- * [scales, rolling_mean, rolling_variance].  Load accepts older headers without seen and stops
+ * [scales, rolling_mean, rolling_variance]; per layer norm, which darknet does
+ * not have: biases, scales.  Load accepts older headers without seen and stops
  * quietly at end of file, as the reference does; it sets seen and the
  * iteration.  It honours the layer options dontload, dontloadscales and
  * flipped as NNetwork.loadWeights / ConvolutionalLayer.loadWeights do, and
@@ -445,8 +467,11 @@ int an_iteration(const an_network *net);
 /* device buffer of a layer: which = 0 output, 1 delta, 2 weights,
  * 3 weight_updates, 4 biases, 5 bias_updates, 6 scales, 7 scale_updates,
  * 8 rolling_mean, 9 rolling_variance, 10 mean, 11 variance, 12 x (pre-BN),
- * 14 indexes (int32), 15 loss; *count = elements (0 if absent)              */
+ * (NULL with an_set_checkpoints), 14 indexes (int32), 15 loss, 16 stats of a
+ * layer norm, 17 x's checkpoint (bytes); *count = elements (0 if absent)    */
 void *an_layer_buffer(an_network *net, int layer, int which, size_t *count);
+/* bytes of device memory that an_finalize took for the layers               */
+size_t an_device_bytes(const an_network *net);
 /* total GFLOP of one training step's conv GEMMs (fwd + wgrad + dgrad where
  * the layer has an input gradient)                                          */
 double an_step_conv_gflop(const an_network *net);

@@ -172,3 +172,32 @@ def test_checkpoint_form():
     edge = np.array([[127.0, 127.49, 127.5, 128.0]]).T  # alone in their blocks
     codes, steps = ref.pack(edge)
     assert list(steps[:, 0]) == [133, 133, 134, 134] and list(codes[:, 0]) == [127, 127, 64, 64]
+
+
+# ---- in a network, before it is finalized ------------------------------------------
+def test_network_refusals(tmp_path, capfd):
+    lib = aetcnn.net_lib()
+    h = lib.an_network_create(2, 4, 4, 3)
+    for eps in (0.0, -1.0, 1e-13, 2.0, NAN, INF):
+        assert lib.an_add_layernorm(h, eps) == ACH_EINVAL
+    assert lib.an_add_layernorm(None, 1e-5) == ACH_EINVAL
+    assert lib.an_add_layernorm(h, 1e-5) == 0
+    assert lib.an_set_checkpoints(None, 1) == lib.an_set_checkpoints(h, 2) == ACH_EINVAL
+    assert lib.an_set_checkpoints(h, 1) == lib.an_set_checkpoints(h, 0) == 0
+    lib.an_free(h)
+    cfg = tmp_path / "n.cfg"
+    text = ("[net]\nbatch=4\nheight=6\nwidth=5\nchannels=3\nactivation_checkpoints={}\n"
+            "[convolutional]\nfilters=8\nsize=3\npad=1\nbatch_normalize=1\nactivation=leaky\n"
+            "[layernorm]\neps={}\nlearning_rate=2\n[connected]\noutput=7\nactivation=linear\n[layernorm]\n"
+            "[softmax]\n")
+    cfg.write_text(text.format(1, 0.001))
+    net = aetcnn.Network.from_cfg(str(cfg), finalize=False)
+    assert "unused" not in capfd.readouterr().err
+    assert [net.shape(i)[:4] for i in range(5)] == [[0, 8, 6, 5], [5, 8, 6, 5], [0, 7, 1, 1],
+                                                    [5, 7, 1, 1], [4, 7, 1, 1]]
+    assert net.layer_options(1)["learning_rate_scale"] == 2.0
+    net.close()
+    for bad in (text.format(2, 0.001), text.format(0, 0)):
+        cfg.write_text(bad)
+        with pytest.raises(ValueError):
+            aetcnn.Network.from_cfg(str(cfg), finalize=False)
