@@ -436,7 +436,7 @@ int ach_fc_bwd_filter_checkpoint(const ach_fc_desc *desc, const void *checkpoint
     if (!aligned(checkpoint, 16) || !aligned(delta, elem_size(d.type)) || !aligned(dw, 4))
         return ACH_EINVAL;
     const Plan p = fc_plan(d);
-    if ((int64_t)p.ti * p.to > 0x7fffffff) return ACH_EINVAL;
+    if ((int64_t)p.ti * p.to >= 1 << 23) return ACH_EINVAL;  // more of dw than a card holds
     if (p.bytes && (!ws || ws_bytes < p.bytes || !aligned(ws, 16))) return ACH_EWORKSPACE;
     const Fc a = {d.rows, d.inputs, d.outputs, d.stride, kept(checkpoint, d.rows, d.inputs), dw,
                   p.slices > 1 ? (float *)ws : nullptr, accumulate, p.span, p.ti,

@@ -124,10 +124,10 @@ struct Fwd {
     int parts, span; // chunks of a part
 };
 
-// From the sums of x - first and of their squares, in 64 bits: the subtraction of
-// the mean's square is exact enough for a mean 10^4 times above the deviations, and
-// relative to the row's first value it rarely is.  (The variance passes a float's
-// range where the values pass 1.8e19.)
+// From the sums of x - first and of their squares, in 64 bits.  As the row's first
+// value is one of its n, the mean is at most sqrt(n) deviations from it, and the
+// subtraction of its square loses log2 n of the 53 bits at most.  (The variance
+// passes a float's range where the values pass 1.8e19.)
 __device__ __forceinline__ float2 statistics(double s, double q, float first, double inv, float eps)
 {
     const double m = s * inv, var = fmax(q * inv - m * m, 0.) + (double)eps;
@@ -250,6 +250,7 @@ k_norm_fwd(const typename Elem<TYPE>::T *x, typename Elem<TYPE>::T *y, Fwd a)
 
 // Rows in parts: the sums of each part, then, from all of a row's, its values.
 constexpr int PART_NT = 256;
+constexpr int MOST_GROUPS = (1 << 24) - 1;  // workgroups of a launch: for more values than a card holds
 template <int TYPE>
 __global__ void __launch_bounds__(PART_NT) k_norm_fwd_sums(const typename Elem<TYPE>::T *x, Fwd a)
 {
@@ -333,7 +334,11 @@ template <int TYPE, bool KEPT> struct Pair {
             __builtin_memcpy(x, __builtin_assume_aligned(a.k.codes + at, VEC), VEC);
             step = a.k.steps[at / KEPT_BLOCK];
         } else {
-            const v4u c = load_chunk<TYPE>(xs + r * a.stride + col, left, 0.f);
+            // (behind the last value delta is 0 and x one of the row's values: any
+            // other's x_norm might be too large for a float)
+            float fill = 0.f;
+            if (left < VEC) fill = (float)xs[r * a.stride];
+            const v4u c = load_chunk<TYPE>(xs + r * a.stride + col, left, fill);
             __builtin_memcpy(x, &c, sizeof(c));
         }
     }
@@ -431,7 +436,6 @@ k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
             fetch(i);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                // (deltas behind the last value are 0, x_norm is any number there)
                 const float g = d[e] * sc[(HOLD ? i * VEC : 0) + e];
                 sums[0] += g;
                 sums[1] = fmaf(g, n[e], sums[1]);
@@ -552,12 +556,12 @@ k_norm_bwd_values(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>
 #pragma unroll
         for (int e = 0; e < VEC; ++e) ds[e] = fmaf(d[e], n[e], ds[e]), db[e] += d[e];
         if (!dx) continue;
-        float m1 = 0.f, m2 = 0.f;
+        double s1 = 0, s2 = 0;  // (thousands of parts, where rows are that long)
         for (int i = 0; i < a.parts; ++i) {
             const float2 v = a.sums[(size_t)r * a.parts + i];
-            m1 += v.x, m2 += v.y;
+            s1 += v.x, s2 += v.y;
         }
-        m1 *= inv, m2 *= inv;
+        const float m1 = (float)s1 * inv, m2 = (float)s2 * inv;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) d[e] = st.y * (d[e] * sc[e] - m1 - n[e] * m2);
         write_values<TYPE>(dx + r * a.dx_stride + col, left, d, a.past);
@@ -571,7 +575,7 @@ k_norm_bwd_values(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>
     }
 }
 
-// The partial sums of 32 columns, a 32nd of each by each of 32 threads.
+// The partial sums of 32 columns at a time, a 32nd of each by each of 32 threads.
 constexpr int JOIN = 32;
 __global__ void __launch_bounds__(JOIN * 32)
 k_norm_bwd_join(const float *partial, int spans, int features, float *scale_updates,
@@ -581,28 +585,29 @@ k_norm_bwd_join(const float *partial, int spans, int features, float *scale_upda
     float *const to = blockIdx.y ? bias_updates : scale_updates;
     if (!to) return;
     const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
-    const int j = blockIdx.x * 32 + lane;
-    double s = 0;
-    if (j < features) {
-        const float *p = partial + (size_t)blockIdx.y * spans * features + j;
-        int i = share;
-        for (; i + 3 * JOIN < spans; i += 4 * JOIN) {  // four loads in flight
-            float v[4];
+    for (int first = blockIdx.x * 32; first < features; first += (int)gridDim.x * 32) {
+        const int j = first + lane;
+        double s = 0;
+        if (j < features) {
+            const float *p = partial + (size_t)blockIdx.y * spans * features + j;
+            int i = share;
+            for (; i + 3 * JOIN < spans; i += 4 * JOIN) {  // four loads in flight
+                float v[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = p[(size_t)(i + u * JOIN) * features];
+                for (int u = 0; u < 4; ++u) v[u] = p[(size_t)(i + u * JOIN) * features];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) s += v[u];
+                for (int u = 0; u < 4; ++u) s += v[u];
+            }
+            for (; i < spans; i += JOIN) s += p[(size_t)i * features];
         }
-        for (; i < spans; i += JOIN) s += p[(size_t)i * features];
-    }
-    sh[share][lane] = s;
-    __syncthreads();
-    for (int n = JOIN / 2; n; n >>= 1) {
-        if (share < n) sh[share][lane] = s += sh[share + n][lane];
+        sh[share][lane] = s;
         __syncthreads();
+        for (int n = JOIN / 2; n; n >>= 1) {
+            if (share < n) sh[share][lane] = s += sh[share + n][lane];
+            __syncthreads();
+        }
+        if (share == 0 && j < features) to[j] = accumulate ? (float)(to[j] + s) : (float)s;
     }
-    if (share || j >= features) return;
-    to[j] = accumulate ? (float)(to[j] + s) : (float)s;
 }
 
 // ---- plans ---------------------------------------------------------------------------
@@ -804,7 +809,7 @@ int ach_layernorm_fwd(const ach_layernorm_desc *desc, const void *x, const float
     hipStream_t st = as_stream(s);
     const int vec = 16 / (int)size;
     a.chunks = checkpoint ? chunks_of(d) : (d.features + vec - 1) / vec;
-    if ((int64_t)d.rows * p.parts > 0x7fffffff) return ACH_EINVAL;
+    if ((int64_t)d.rows * p.parts > MOST_GROUPS) return ACH_EINVAL;
 #define CALL(TYPE)                                                                                 \
     return checkpoint ? fwd_go<TYPE, true>(p, x, y, a, chunks_of(d), st)                           \
                       : fwd_go<TYPE, false>(p, x, y, a, chunks_of(d), st)
@@ -837,7 +842,8 @@ int ach_layernorm_bwd(const ach_layernorm_desc *desc, const void *delta, int64_t
     if (dx == delta && dx_stride != delta_stride) return ACH_EINVAL;
     const Plan p = bwd_plan(d);
     if (p.bytes && (!ws || ws_bytes < p.bytes || !aligned(ws, 16))) return ACH_EWORKSPACE;
-    if ((int64_t)d.rows * p.parts > 0x7fffffff || (int64_t)p.tiles * p.spans > 0x7fffffff) return ACH_EINVAL;
+    if ((int64_t)d.rows * p.parts > MOST_GROUPS || (int64_t)p.tiles * p.spans > MOST_GROUPS)
+        return ACH_EINVAL;
     hipStream_t st = as_stream(s);
     const bool updates = scale_updates || bias_updates;
     float *const partial = (float *)((char *)ws + p.partial);
@@ -856,7 +862,8 @@ int ach_layernorm_bwd(const ach_layernorm_desc *desc, const void *delta, int64_t
         if (rc) return rc;
     }
     if (updates) {
-        hipLaunchKernelGGL(k_norm_bwd_join, dim3((unsigned)((d.features + 31) / 32), 2),
+        const int tiles = (d.features + 31) / 32;
+        hipLaunchKernelGGL(k_norm_bwd_join, dim3((unsigned)min(tiles, 1 << 20), 2),
                            dim3(JOIN * 32), 0,
                            st, (const float *)partial, p.spans, d.features, scale_updates,
                            bias_updates, accumulate);

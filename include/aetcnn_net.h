@@ -73,7 +73,6 @@ struct an_layer {
     float *mean_delta, *variance_delta;
     float *x;               /* pre-BN conv output (NormData.x); with
                                an_set_checkpoints one buffer of all layers  */
-    void *x_kept;           /* its checkpoint in 8 bits, or NULL            */
     float *weights_kmajor;  /* filter layouts the conv GEMMs read, refreshed */
     float *weights_flipped; /* from weights at every forward pass            */
     /* maxpool */
@@ -81,9 +80,6 @@ struct an_layer {
     /* dropout */
     float probability;
     int shares_prev;        /* output/delta alias the previous layer's    */
-    /* layer norm (biases and scales above, one each per feature)            */
-    float eps;
-    float *stats;           /* [batch][2] mean and rstd of each image        */
     /* softmax */
     int groups;
     float temperature;
@@ -110,6 +106,10 @@ struct an_layer {
     int (*backward)(an_network *net, an_layer *l, an_state st);
     int (*update)(an_network *net, an_layer *l, int batch, float lr, float momentum,
                   float decay);
+    void *x_kept;           /* x's checkpoint in 8 bits (an_set_checkpoints), or NULL */
+    /* layer norm (biases and scales above, one each per feature)            */
+    float eps;
+    float *stats;           /* [batch][2] mean and rstd of each image        */
 };
 
 /* ---- construction ------------------------------------------------------- */

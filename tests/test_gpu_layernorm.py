@@ -253,6 +253,24 @@ def test_values_at_the_ends(gpu, n, eps):
     f.check()
 
 
+@pytest.mark.parametrize("n", [3, 101, 1001, 5003, 30001, 70001])
+def test_large_constant_rows(gpu, n):
+    """x_norm is 0 there; what stands behind a row's last value must not count,
+    though 0 in its place would be infinitely many deviations away"""
+    x = Rows(np.full((3, n), 1e35), F32)
+    rng = np.random.default_rng(n)
+    s, b = parameters(rng, n)
+    f = Forward(gpu, x, s, b, 1e-12, keep=True)
+    f.call()
+    f.check()
+    g = Backward(gpu, Rows(rng.standard_normal((3, n)) * 1e-8, F32), (x, 1e-12), s)
+    stats = np.stack([np.full(3, x.x[0, 0]), np.full(3, 1e6)], 1).astype(np.float32)
+    g.stats.upload(stats)
+    g.want = ref.backward(g.delta.x, np.zeros((3, n)), 0.0, stats[:, 1].astype(np.float64), s, F32)
+    g.call()
+    g.check()
+
+
 @pytest.mark.parametrize("kind", [F32, BF16, F16])
 @pytest.mark.parametrize("n", [3, 100, 3000, 20000, 140000])
 def test_rows_that_are_not_finite(gpu, n, kind):
@@ -323,6 +341,47 @@ def test_offsets_past_32_bits(gpu):
                                   k.ptr, None))
     assert np.array_equal(k.read()[0], ref.pack(x.x)[0])
     check(gpu.ach_free(big))
+
+
+def test_a_row_of_many_values(gpu):
+    """over 2^27: more columns than one launch's threads"""
+    n = (1 << 27) + 77
+    rng = np.random.default_rng(1)
+    block = rng.standard_normal(1 << 16).astype(np.float32)
+    raw = np.resize(block, n).view(np.uint32)
+    bits16 = (raw >> 16).astype(np.uint16)  # bf16, cut off
+    v = (bits16.astype(np.uint32) << 16).view(np.float32)
+    x, out = D.from_numpy(bits16), D((n,), np.uint16)
+    up = [D((n,)), D((n,))]
+    st = D((1, 2))
+    d = aetcnn.LayernormDesc(1, n, BF16, 1e-5)
+    fb, bb = (q(C.byref(d)) for q in (gpu.ach_layernorm_fwd_workspace, gpu.ach_layernorm_bwd_workspace))
+    ws = D((max(fb, bb) // 4 + 4,), np.int32)
+    check(gpu.ach_layernorm_fwd(C.byref(d), x.ptr, None, None, out.ptr, 0, st.ptr, None, ws.ptr, fb, None))
+    mean, var = v.mean(dtype=np.float64), v.var(dtype=np.float64)
+    got = st.numpy()[0].astype(np.float64)
+    assert abs(got[0] - mean) <= 1e-6 and abs(got[1] * np.sqrt(var + 1e-5) - 1) <= 1e-6
+    y = (out.numpy().astype(np.uint32) << 16).view(np.float32)
+    want = (v - np.float32(got[0])) * np.float32(got[1])
+    assert (np.abs(y - want) <= 2.0 ** -8 * np.abs(want) + 1e-30).all()
+    # the row itself as its delta
+    check(gpu.ach_layernorm_bwd(C.byref(d), x.ptr, 0, x.ptr, None, st.ptr, None, out.ptr, 0, up[0].ptr,
+                                up[1].ptr, 0, ws.ptr, bb, None))
+    assert np.array_equal(up[1].numpy(), v)
+    ds = up[0].numpy()
+    assert (np.abs(ds - v * want) <= 4 * ref.U * np.abs(v * want)).all()
+    # the row is nearly its own x_norm, so dx is what cancellation leaves.  Its
+    # terms are off by 5 u of their sizes (norm_ref.backward); the two means by that of
+    # chains of at most 16 chunks of 8 values a thread and what joins 256 threads
+    # (10), the parts' sums in 64 bits: 138 additions, a product, a division: 142 u
+    # of the mean of the terms' magnitudes
+    m1, m2 = mean, (v * want).mean(dtype=np.float64)
+    e1, e2 = (142 * ref.U * np.abs(q).mean(dtype=np.float64) for q in (v, v * want))
+    size = np.abs(v) + abs(m1) + np.abs(want * m2)
+    bound = got[1] * (5 * ref.U * size + e1 + np.abs(want) * (e2 + 3 * ref.U * abs(m2)))
+    y = (out.numpy().astype(np.uint32) << 16).view(np.float32)
+    want = got[1] * (v - m1 - want * m2)
+    assert (np.abs(y - want) <= bound + 2.0 ** -8 * (np.abs(want) + bound)).all()
 
 
 def bits(f, g):
