@@ -12,15 +12,17 @@
 // give: 16 lanes read 4 rows x 16 columns, and each gets a column of it.  Few tiles
 // share out the rows in slices, whose sums a second launch adds up in order.
 //
-// Bound by the matrix units on many rows: 8192 x 8192 -> 4096 (a matrix product of
-// the library at 8192^3 in bf16: 1250 TFLOP/s) bf16 527 us, 1043 TFLOP/s; fp32 1355
-// us, three passes of 405; 16384 x 4096 -> 1024 bf16 157 us, of which 15 are the
-// four slices' sums.  By the writing of dw on few: 128 x 9216 -> 4096 fp32 60 us
-// for 154 MB; its workgroups write in step, so that neither the loads nor the
-// products of a next tile lie behind it.  What it took on 16384 x 4096 -> 1024 bf16:
-// one stage ahead 399 us, two 233; offsets in the loads' windows instead of 64-bit
-// addresses and clamps (100 vector instructions for 8 of the matrix) 189; waves of
-// 128 x 64 162; the operands' loads among the matrix instructions 157.
+// Bound by the matrix units on many rows: 8192 x 8192 -> 4096 bf16 516 us, 1066
+// TFLOP/s (a matrix product of the library at 8192^3 in bf16: 1250); fp32 1357 us,
+// three passes of 405; 16384 x 4096 -> 1024 bf16 153 us, of which 15 are the four
+// slices' sums.  On few rows by a tile's start, its four stages and the writing
+// of dw, one after the other: 128 x 9216 -> 4096 fp32 56 us for 154 MB (without the
+// writing 50, only that 30).  What it took on 16384 x 4096 -> 1024 bf16: one stage ahead 399
+// us, two 233; offsets in the loads' windows instead of 64-bit addresses and clamps
+// (100 vector instructions for 8 of the matrix) 189; waves of 128 x 64 162; the
+// operands' loads among the matrix instructions 155; a last turn that loads nothing
+// 153.  Several tiles a workgroup, the next one's loads before the writing, gained
+// 2 us on few rows and lost 10% on many, where it spoils the loop's order.
 #include "checkpoint.hpp"
 #include "pieces.hpp"
 
@@ -28,7 +30,7 @@ namespace ach {
 namespace {
 
 constexpr int DEPTH = 32;  // rows of a stage
-constexpr int RING = 2;    // stages in flight, an even number
+constexpr int RING = 2;    // stages in flight (the loops are written for two)
 constexpr int MOST_SLICES = 64;
 constexpr int MOST_COLUMNS = 1 << 23;  // inputs, outputs, stride: a stage's offsets fit 31 bits
 
@@ -133,10 +135,13 @@ template <int PITCH> __device__ __forceinline__ v8bf fragment(const short *p)
     return __builtin_bit_cast(v8bf, v);
 }
 
+// How a chunk of delta is loaded.  What lies behind the last output or input is
+// never stored, so any values will do there: loads that pass a row's end read the
+// next row, or zeros behind the last one (WHOLE).  The range check is by dwords, so
+// 16-bit values, which would lose the last one of an odd number, are loaded whole
+// chunks inside a row instead, early and then shifted (EARLY), or one by one
+// (SINGLE, under 8 outputs).
 enum { WHOLE, EARLY, SINGLE };
-template <int W> struct How {
-    static constexpr int value = W;
-};
 
 // WO x WI waves of 32 MO outputs x 64 inputs
 template <int TYPE, int WO, int WI, int MO> struct Tile {
@@ -149,7 +154,7 @@ template <int TYPE, int WO, int WI, int MO> struct Tile {
     static constexpr size_t LDS = 2 * sizeof(Stage);
 };
 
-template <int TYPE, int WO, int WI, int MO>
+template <int TYPE, int WO, int WI, int MO, int HOW>
 __global__ void __launch_bounds__(64 * WO * WI, 2)
 k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
 {
@@ -165,33 +170,30 @@ k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
     const int wo = wave % WO, wi = wave / WO;
     // each XCD, which takes every eighth workgroup, gets a contiguous range of
     // tiles, which share their operands in its L2
-    int id = blockIdx.x;
-    {
-        const int G = gridDim.x, g8 = G >> 3, r8 = G & 7, xcd = id & 7;
-        id = xcd * g8 + min(xcd, r8) + (id >> 3);
-    }
-    const int o0 = id / a.ti * S::O, i0 = id % a.ti * S::I;
+    const int xcd = blockIdx.x & 7, tiles = gridDim.x;
+    const int tile = xcd * (tiles >> 3) + min(xcd, tiles & 7) + (int)(blockIdx.x >> 3);
+    const int o0 = tile / a.ti * S::O, i0 = tile % a.ti * S::I;
     const int r0 = (int)blockIdx.y * a.span, r1 = min((int64_t)a.rows, (int64_t)r0 + a.span);
 
-    // A thread's share of a stage.  What lies behind the last output or input is
-    // never stored, so any values will do there: loads that pass a row's end read
-    // the next row, or zeros behind the last one.  The range check is by dwords,
-    // so 16-bit values, which would lose the last one of an odd number, are
-    // loaded whole chunks inside a row instead, early and then shifted (EARLY),
-    // or one by one (SINGLE, under 8 outputs).
+    // a thread's share of a stage
     const int xr = tid / (S::I / XC), xc = tid % (S::I / XC) * XC;
     const int dr = tid / (S::O / 8), dc = tid % (S::O / 8) * 8;
-    const int x_col = min(i0 + xc, a.k.width - XC);
-    const int x_at = xr * a.k.width + x_col, s_at = (xr * a.k.width + x_col) / KEPT_BLOCK;
     const int64_t pitch = a.stride * SIZE;
     struct Load {
         uint32_t codes[XC / 4], step;
         Eight<TYPE> d[DN];
     };
+    const int x_col = min(i0 + xc, a.k.width - XC);
+    const int x_at = xr * a.k.width + x_col, s_at = x_at / KEPT_BLOCK;
+    const int d_col = HOW == EARLY ? min(o0 + dc, a.outputs - 8) : o0 + dc;
+    const int late = min(o0 + dc - d_col, 7);
+    int d_at[DN];
+#pragma unroll
+    for (int h = 0; h < DN; ++h) d_at[h] = (dr + h * DR) * (int)pitch + d_col * SIZE;
     Window codes(a.k.codes, a.k.width, a.k.width, r0, r1),
         steps(a.k.steps, a.k.width / KEPT_BLOCK, a.k.width / KEPT_BLOCK, r0, r1),
         deltas(delta, pitch, (int64_t)a.outputs * SIZE, r0, r1);
-    auto load = [&](Load &g, const int *d_at, auto how) {
+    auto load = [&](Load &g) {
         const __amdgpu_buffer_rsrc_t c = codes.next(), t = steps.next(), d = deltas.next();
         if constexpr (XC == 16) {
             const auto v = __builtin_amdgcn_raw_buffer_load_b128(c, x_at, 0, 0);
@@ -203,7 +205,7 @@ k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
         g.step = __builtin_amdgcn_raw_buffer_load_b8(t, s_at, 0, 0);
 #pragma unroll
         for (int h = 0; h < DN; ++h) {
-            if constexpr (decltype(how)::value == SINGLE) {
+            if constexpr (HOW == SINGLE) {
                 uint16_t v[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -218,7 +220,7 @@ k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
             }
         }
     };
-    auto store = [&](Load &g, int s, int late, auto how) {
+    auto store = [&](Load &g, int s) {
         const float scale = kept_scale(g.step);
         uint32_t w[XC / 2];
 #pragma unroll
@@ -235,13 +237,12 @@ k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
 #pragma unroll
         for (int h = 0; h < DN; ++h) {
             v4u p[P];
-            if constexpr (decltype(how)::value == EARLY) g.d[h].shift(late);
+            if constexpr (HOW == EARLY) g.d[h].shift(late);
             g.d[h].split(p);
 #pragma unroll
             for (int q = 0; q < P; ++q) *(v4u *)&stage[s].d[q][(dr + h * DR) * S::OP + dc] = p[q];
         }
     };
-
     v16f hi[MO][2], lo[P > 1 ? MO : 1][2];
 #pragma unroll
     for (int i = 0; i < MO; ++i)
@@ -255,6 +256,7 @@ k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
     const int row = 8 * (lane >> 5) + ((lane & 15) >> 2), column = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
     const int d_place = row * S::OP + wo * 32 * MO + column, x_place = row * S::IP + wi * 64 + column;
     auto multiply = [&](int s) {
+        __builtin_amdgcn_iglp_opt(0);  // operand loads among the matrix instructions
 #pragma unroll
         for (int step = 0; step < DEPTH; step += 16) {
             v8bf x[2];
@@ -275,34 +277,25 @@ k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
             }
         }
     };
-    auto all = [&](auto how) {
-        const int start = decltype(how)::value == EARLY ? min(o0 + dc, a.outputs - 8) : o0 + dc;
-        const int late = min(o0 + dc - start, 7);
-        int d_at[DN];
+    Load ring[RING];
 #pragma unroll
-        for (int h = 0; h < DN; ++h) d_at[h] = (dr + h * DR) * (int)pitch + start * SIZE;
-        Load ring[RING];
+    for (int u = 0; u < RING; ++u) load(ring[u]);
+    store(ring[0], 0);
+    load(ring[0]);
+    __syncthreads();
+    for (int r = r0; r + RING * DEPTH < r1; r += RING * DEPTH) {
 #pragma unroll
-        for (int u = 0; u < RING; ++u) load(ring[u], d_at, how);
-        store(ring[0], 0, late, how);
-        load(ring[0], d_at, how);
-        __syncthreads();
-        // whole turns of the ring (stages behind the last row are zeros)
-        for (int r = r0; r < r1; r += RING * DEPTH) {
-#pragma unroll
-            for (int u = 1; u <= RING; ++u) {
-                __builtin_amdgcn_iglp_opt(0);  // operand loads among the matrix instructions
-                multiply((u + 1) % 2);
-                store(ring[u % RING], u % 2, late, how);
-                load(ring[u % RING], d_at, how);
-                __syncthreads();
-            }
+        for (int u = 1; u <= RING; ++u) {
+            multiply((u + 1) % 2);
+            store(ring[u % RING], u % 2);
+            load(ring[u % RING]);
+            __syncthreads();
         }
-    };
-    if (SIZE == 4) all(How<WHOLE>());
-    else if (a.outputs < 8) all(How<SINGLE>());
-    else if (a.outputs % 8 && o0 + S::O > a.outputs) all(How<EARLY>());
-    else all(How<WHOLE>());
+    }
+    multiply(0);  // the last turn, with nothing left to load (a stage behind the last row is zeros)
+    store(ring[1], 1);
+    __syncthreads();
+    multiply(1);
 
     float *const out = a.part ? a.part + (size_t)blockIdx.y * a.outputs * a.inputs : a.dw;
     const bool add = a.accumulate && !a.part;
@@ -388,11 +381,11 @@ Plan fc_plan(const ach_fc_desc &d)
     return p;
 }
 
-template <int TYPE, int WO, int WI, int MO>
-int fc_go(const Plan &p, const void *delta, const Fc &a, hipStream_t st)
+template <int TYPE, int WO, int WI, int MO, int HOW>
+int fc_launch(const Plan &p, const void *delta, const Fc &a, hipStream_t st)
 {
     using S = Tile<TYPE, WO, WI, MO>;
-    const auto kern = &k_fc_wgrad<TYPE, WO, WI, MO>;
+    const auto kern = &k_fc_wgrad<TYPE, WO, WI, MO, HOW>;
     if (S::LDS > 64 * 1024) {
         const int rc = check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::LDS));
@@ -401,6 +394,16 @@ int fc_go(const Plan &p, const void *delta, const Fc &a, hipStream_t st)
     hipLaunchKernelGGL(kern, dim3((unsigned)(p.ti * p.to), (unsigned)p.slices), dim3(S::THREADS),
                        S::LDS, st, (const typename Elem<TYPE>::T *)delta, a);
     return check_launch();
+}
+
+template <int TYPE, int WO, int WI, int MO>
+int fc_go(const Plan &p, const void *delta, const Fc &a, hipStream_t st)
+{
+    if constexpr (TYPE != ACH_F32) {
+        if (a.outputs < 8) return fc_launch<TYPE, WO, WI, MO, SINGLE>(p, delta, a, st);
+        if (a.outputs % 8) return fc_launch<TYPE, WO, WI, MO, EARLY>(p, delta, a, st);
+    }
+    return fc_launch<TYPE, WO, WI, MO, WHOLE>(p, delta, a, st);
 }
 
 // bf16 deltas, whose tiles cost the matrix units a third of the others' time, need
