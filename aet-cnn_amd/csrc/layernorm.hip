@@ -575,28 +575,29 @@ k_norm_bwd_values(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>
     }
 }
 
-// The partial sums of 32 columns at a time, a 32nd of each by each of 32 threads.
-constexpr int JOIN = 32;
-__global__ void __launch_bounds__(JOIN * 32)
+// The partial sums of 64 columns at a time, a 16th of each by each of 16 waves.
+constexpr int JOIN = 16;
+__global__ void __launch_bounds__(JOIN * 64)
 k_norm_bwd_join(const float *partial, int spans, int features, float *scale_updates,
                 float *bias_updates, int accumulate)
 {
-    __shared__ double sh[JOIN][32];
+    constexpr int U = 8;  // loads in flight
+    __shared__ double sh[JOIN][64];
     float *const to = blockIdx.y ? bias_updates : scale_updates;
     if (!to) return;
-    const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
-    for (int first = blockIdx.x * 32; first < features; first += (int)gridDim.x * 32) {
+    const int lane = threadIdx.x & 63, share = threadIdx.x >> 6;
+    for (int first = blockIdx.x * 64; first < features; first += (int)gridDim.x * 64) {
         const int j = first + lane;
         double s = 0;
         if (j < features) {
             const float *p = partial + (size_t)blockIdx.y * spans * features + j;
             int i = share;
-            for (; i + 3 * JOIN < spans; i += 4 * JOIN) {  // four loads in flight
-                float v[4];
+            for (; i + (U - 1) * JOIN < spans; i += U * JOIN) {
+                float v[U];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = p[(size_t)(i + u * JOIN) * features];
+                for (int u = 0; u < U; ++u) v[u] = p[(size_t)(i + u * JOIN) * features];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) s += v[u];
+                for (int u = 0; u < U; ++u) s += v[u];
             }
             for (; i < spans; i += JOIN) s += p[(size_t)i * features];
         }
@@ -862,9 +863,9 @@ int ach_layernorm_bwd(const ach_layernorm_desc *desc, const void *delta, int64_t
         if (rc) return rc;
     }
     if (updates) {
-        const int tiles = (d.features + 31) / 32;
+        const int tiles = (d.features + 63) / 64;
         hipLaunchKernelGGL(k_norm_bwd_join, dim3((unsigned)min(tiles, 1 << 20), 2),
-                           dim3(JOIN * 32), 0,
+                           dim3(JOIN * 64), 0,
                            st, (const float *)partial, p.spans, d.features, scale_updates,
                            bias_updates, accumulate);
         return check_launch();
