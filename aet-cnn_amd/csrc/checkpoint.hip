@@ -60,8 +60,8 @@ int go(const ach_checkpoint_desc &d, void *x, const void *checkpoint, hipStream_
     // values of more than the L2 caches hold go past them (128 x 290400 fp32, both
     // ways: 73 us, 64 past them)
     const bool past = (size_t)d.rows * d.features * sizeof(T) > (size_t)32 << 20;
-    // launches of as many rows as have fewer than 2^31 chunks
-    const int most = per < 0x40000000 ? 0x7fffffff / per : 1;
+    // launches of as many rows as have fewer than 2^31 chunks (a row: 2^28 at most)
+    const int most = 0x7fffffff / per;
     for (int r = 0; r < d.rows; r += most) {
         const int rows = d.rows - r < most ? d.rows - r : most;
         const int n = rows * per;
@@ -72,7 +72,6 @@ int go(const ach_checkpoint_desc &d, void *x, const void *checkpoint, hipStream_
         if (rc) return rc;
         k.codes += (size_t)rows * k.width;
         k.steps += (size_t)rows * (k.width / KEPT_BLOCK);
-        if (d.rows - r <= most) break;
     }
     return ACH_OK;
 }

@@ -249,7 +249,12 @@ k_norm_fwd(const typename Elem<TYPE>::T *x, typename Elem<TYPE>::T *y, Fwd a)
 }
 
 // Rows in parts: the sums of each part, then, from all of a row's, its values.
-constexpr int PART_NT = 256;
+// A thread has FWD_U chunks (backward: BWD_U of delta and x) in flight, as the
+// stores of one hold back the loads of the next (128 x 186624 fp32 forward 57 us with
+// one, 53 with two, 51 with four; backward 128 and 92; 300 x 32768 bf16 backward 28 with
+// two, 30 with four).
+constexpr int PART_NT = 256, FWD_U = 4, BWD_U = 2;
+constexpr int MOST_SPAN = 256;             // rows whose gradients' sums are one chain of additions
 constexpr int MOST_GROUPS = (1 << 24) - 1;  // workgroups of a launch: for more values than a card holds
 template <int TYPE>
 __global__ void __launch_bounds__(PART_NT) k_norm_fwd_sums(const typename Elem<TYPE>::T *x, Fwd a)
@@ -261,10 +266,19 @@ __global__ void __launch_bounds__(PART_NT) k_norm_fwd_sums(const typename Elem<T
     const float first = (float)p[0];
     const int end = min((part + 1) * a.span, a.chunks);
     double sums[2] = {0, 0};
-    for (int c = part * a.span + threadIdx.x; c < end; c += PART_NT) {
-        float v[VEC];
-        chunk_values<TYPE>(load_chunk<TYPE>(p + c * VEC, a.features - c * VEC, first), v);
-        add_values<VEC>(v, first, sums[0], sums[1]);
+    for (int c = part * a.span + threadIdx.x; c < end; c += FWD_U * PART_NT) {
+        v4u w[FWD_U];
+#pragma unroll
+        for (int u = 0; u < FWD_U; ++u) {
+            const int at = min(c + u * PART_NT, end) * VEC;  // (behind the part: nothing but fill)
+            w[u] = load_chunk<TYPE>(p + at, c + u * PART_NT < end ? a.features - at : 0, first);
+        }
+#pragma unroll
+        for (int u = 0; u < FWD_U; ++u) {
+            float v[VEC];
+            chunk_values<TYPE>(w[u], v);
+            add_values<VEC>(v, first, sums[0], sums[1]);
+        }
     }
     row_sums<PART_NT, 2>(sums, sh);
     if (threadIdx.x == 0) {
@@ -278,29 +292,40 @@ __global__ void __launch_bounds__(PART_NT)
 k_norm_fwd_values(const typename Elem<TYPE>::T *x, typename Elem<TYPE>::T *y, Fwd a)
 {
     constexpr int VEC = Row<TYPE>::VEC;
+    __shared__ double sh[2 * PART_NT / 64];
     const int r = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
     const typename Elem<TYPE>::T *p = x + r * a.stride;
     const float first = a.first[r];
-    double s = 0, q = 0;
-    for (int i = 0; i < a.parts; ++i) {
+    double sums[2] = {0, 0};
+    for (int i = threadIdx.x; i < a.parts; i += PART_NT) {
         const double2 v = a.part[(size_t)r * a.parts + i];
-        s += v.x, q += v.y;
+        sums[0] += v.x, sums[1] += v.y;
     }
-    const float2 st = statistics(s, q, first, a.inv, a.eps);
+    row_sums<PART_NT, 2>(sums, sh);
+    const float2 st = statistics(sums[0], sums[1], first, a.inv, a.eps);
     if (a.stats && part == 0 && threadIdx.x == 0) {
         a.stats[2 * (size_t)r] = st.x;
         a.stats[2 * (size_t)r + 1] = st.y;
     }
     if (!y && !KEEP) return;
     const int end = min((part + 1) * a.span, a.chunks);
-    for (int c = part * a.span + threadIdx.x; c < end; c += PART_NT) {
-        const int col = c * VEC, left = a.features - col;
-        float sc[VEC], b[VEC];
-        if (y) {
-            load_floats<VEC>(a.scales, col, left, 1.f, sc);
-            load_floats<VEC>(a.biases, col, left, 0.f, b);
+    for (int c = part * a.span + threadIdx.x; c < end; c += FWD_U * PART_NT) {
+        v4u w[FWD_U];
+        float sc[FWD_U][VEC], b[FWD_U][VEC];
+#pragma unroll
+        for (int u = 0; u < FWD_U; ++u) {
+            const int col = (c + u * PART_NT) * VEC, left = c + u * PART_NT < end ? a.features - col : 0;
+            w[u] = load_chunk<TYPE>(p + col, left, 0.f);
+            if (y) {
+                load_floats<VEC>(a.scales, col, left, 1.f, sc[u]);
+                load_floats<VEC>(a.biases, col, left, 0.f, b[u]);
+            }
         }
-        put_values<TYPE, KEEP>(a, y, r, col, load_chunk<TYPE>(p + col, left, 0.f), st, sc, b);
+#pragma unroll
+        for (int u = 0; u < FWD_U; ++u) {
+            const int at = c + u * PART_NT;
+            if (at < end) put_values<TYPE, KEEP>(a, y, r, at * VEC, w[u], st, sc[u], b[u]);
+        }
     }
 }
 
@@ -515,17 +540,27 @@ k_norm_bwd_sums(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::
     const float2 st = stats_of(a, r);
     const int end = min((part + 1) * a.span, a.chunks);
     float sums[2] = {0.f, 0.f};
-    for (int c = part * a.span + threadIdx.x; c < end; c += PART_NT) {
-        Pair<TYPE, KEPT> p;
-        float d[VEC], n[VEC], sc[VEC];
-        p.load(delta, x, a, r, c * VEC);
-        p.values(st, d, n);
-        load_floats<VEC>(a.scales, c * VEC, a.features - c * VEC, 1.f, sc);
+    for (int c = part * a.span + threadIdx.x; c < end; c += BWD_U * PART_NT) {
+        Pair<TYPE, KEPT> p[BWD_U];
+        float sc[BWD_U][VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float g = d[e] * sc[e];
-            sums[0] += g;
-            sums[1] = fmaf(g, n[e], sums[1]);
+        for (int u = 0; u < BWD_U; ++u) {
+            // (behind the part: nothing of delta, so that it adds nothing)
+            const bool in = c + u * PART_NT < end;
+            const int col = (in ? c + u * PART_NT : a.chunks) * VEC;
+            p[u].load(delta, x, a, r, col);
+            load_floats<VEC>(a.scales, col, a.features - col, 1.f, sc[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < BWD_U; ++u) {
+            float d[VEC], n[VEC];
+            p[u].values(st, d, n);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float g = d[e] * sc[u][e];
+                sums[0] += g;
+                sums[1] = fmaf(g, n[e], sums[1]);
+            }
         }
     }
     row_sums<PART_NT, 2>(sums, sh);
@@ -541,30 +576,48 @@ k_norm_bwd_values(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>
     const int tiles = (a.chunks + PART_NT - 1) / PART_NT;
     const int tile = blockIdx.x % tiles, span = blockIdx.x / tiles;
     const int col = (tile * PART_NT + threadIdx.x) * VEC, left = a.features - col;
+    const int r0 = span * a.rows_of, end = min((int64_t)a.rows, (int64_t)r0 + a.rows_of);
+    __shared__ float2 means[MOST_SPAN];  // of g and of g*x_norm
+    if (dx) {
+        const int lane = threadIdx.x & 63;
+        for (int r = r0 + (threadIdx.x >> 6); r < end; r += PART_NT / 64) {
+            double s1 = 0, s2 = 0;
+            for (int i = lane; i < a.parts; i += 64) {
+                const float2 v = a.sums[(size_t)r * a.parts + i];
+                s1 += v.x, s2 += v.y;
+            }
+            s1 = wave_total(s1), s2 = wave_total(s2);
+            if (lane == 63) means[r - r0] = make_float2((float)s1 * inv, (float)s2 * inv);
+        }
+        __syncthreads();
+    }
     if (left <= 0) return;
     float sc[VEC], ds[VEC], db[VEC];
     load_floats<VEC>(a.scales, col, left, 1.f, sc);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) ds[e] = db[e] = 0.f;
-    const int end = min((int64_t)a.rows, (int64_t)(span + 1) * a.rows_of);
-    for (int r = span * a.rows_of; r < end; ++r) {
-        const float2 st = stats_of(a, r);
-        Pair<TYPE, KEPT> p;
-        float d[VEC], n[VEC];
-        p.load(delta, x, a, r, col);
-        p.values(st, d, n);
+    for (int r = r0; r < end; r += BWD_U) {
+        Pair<TYPE, KEPT> p[BWD_U];
+        float2 st[BWD_U];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) ds[e] = fmaf(d[e], n[e], ds[e]), db[e] += d[e];
-        if (!dx) continue;
-        double s1 = 0, s2 = 0;  // (thousands of parts, where rows are that long)
-        for (int i = 0; i < a.parts; ++i) {
-            const float2 v = a.sums[(size_t)r * a.parts + i];
-            s1 += v.x, s2 += v.y;
+        for (int u = 0; u < BWD_U; ++u)
+            if (r + u < end) {
+                st[u] = stats_of(a, r + u);
+                p[u].load(delta, x, a, r + u, col);
+            }
+#pragma unroll
+        for (int u = 0; u < BWD_U; ++u) {
+            if (r + u >= end) break;
+            float d[VEC], n[VEC];
+            p[u].values(st[u], d, n);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) ds[e] = fmaf(d[e], n[e], ds[e]), db[e] += d[e];
+            if (!dx) continue;
+            const float2 m = means[r + u - r0];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) d[e] = st[u].y * (d[e] * sc[e] - m.x - n[e] * m.y);
+            write_values<TYPE>(dx + (r + u) * a.dx_stride + col, left, d, a.past);
         }
-        const float m1 = (float)s1 * inv, m2 = (float)s2 * inv;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) d[e] = st.y * (d[e] * sc[e] - m1 - n[e] * m2);
-        write_values<TYPE>(dx + r * a.dx_stride + col, left, d, a.past);
     }
     if (!a.partial) return;
     float *const to = a.partial + (size_t)span * a.features + col;
@@ -575,37 +628,39 @@ k_norm_bwd_values(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>
     }
 }
 
-// The partial sums of 64 columns at a time, a 16th of each by each of 16 waves.
-constexpr int JOIN = 16;
-__global__ void __launch_bounds__(JOIN * 64)
+// The partial sums of a column: few by one thread, more by a thread in each of 16 waves.
+template <int SHARES>
+__global__ void __launch_bounds__(SHARES == 1 ? 256 : SHARES * 64)
 k_norm_bwd_join(const float *partial, int spans, int features, float *scale_updates,
                 float *bias_updates, int accumulate)
 {
-    constexpr int U = 8;  // loads in flight
-    __shared__ double sh[JOIN][64];
+    constexpr int U = 8, COLS = SHARES == 1 ? 256 : 64;  // loads in flight, columns of a workgroup
+    __shared__ double sh[SHARES][SHARES == 1 ? 1 : COLS];
     float *const to = blockIdx.y ? bias_updates : scale_updates;
     if (!to) return;
-    const int lane = threadIdx.x & 63, share = threadIdx.x >> 6;
-    for (int first = blockIdx.x * 64; first < features; first += (int)gridDim.x * 64) {
+    const int lane = threadIdx.x % COLS, share = threadIdx.x / COLS;
+    for (int first = blockIdx.x * COLS; first < features; first += (int)gridDim.x * COLS) {
         const int j = first + lane;
         double s = 0;
         if (j < features) {
             const float *p = partial + (size_t)blockIdx.y * spans * features + j;
             int i = share;
-            for (; i + (U - 1) * JOIN < spans; i += U * JOIN) {
+            for (; i + (U - 1) * SHARES < spans; i += U * SHARES) {
                 float v[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) v[u] = p[(size_t)(i + u * JOIN) * features];
+                for (int u = 0; u < U; ++u) v[u] = p[(size_t)(i + u * SHARES) * features];
 #pragma unroll
                 for (int u = 0; u < U; ++u) s += v[u];
             }
-            for (; i < spans; i += JOIN) s += p[(size_t)i * features];
+            for (; i < spans; i += SHARES) s += p[(size_t)i * features];
         }
-        sh[share][lane] = s;
-        __syncthreads();
-        for (int n = JOIN / 2; n; n >>= 1) {
-            if (share < n) sh[share][lane] = s += sh[share + n][lane];
+        if (SHARES > 1) {
+            sh[share][lane] = s;
             __syncthreads();
+            for (int n = SHARES / 2; n; n >>= 1) {
+                if (share < n) sh[share][lane] = s += sh[share + n][lane];
+                __syncthreads();
+            }
         }
         if (share == 0 && j < features) to[j] = accumulate ? (float)(to[j] + s) : (float)s;
     }
@@ -627,6 +682,7 @@ bool row_stride(int64_t *stride, int features)
     return *stride >= features;
 }
 
+int tiles_of(int n, int tile) { return (n + tile - 1) / tile; }
 size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 bool past_caches(const ach_layernorm_desc &d)
@@ -688,9 +744,9 @@ constexpr int bwd_chunks(int type) { return type == ACH_F32 ? 4096 : 2048; }
 
 void in_parts(int chunks, int rows, Plan *p)
 {
-    // parts of 4 to 16 chunks a thread, so that there are 1024 workgroups where that can be
+    // parts of 2 to 16 chunks a thread, so that there are 1024 workgroups where that can be
     int64_t parts = rows ? 1024 / rows : 1;
-    const int64_t least = (chunks + 16 * PART_NT - 1) / (16 * PART_NT), most = chunks / (4 * PART_NT);
+    const int64_t least = (chunks + 16 * PART_NT - 1) / (16 * PART_NT), most = chunks / (2 * PART_NT);
     if (parts > most) parts = most;
     if (parts < least) parts = least;
     if (parts < 1) parts = 1;
@@ -721,11 +777,15 @@ Plan bwd_plan(const ach_layernorm_desc &d)
     if (!for_bwd_kind(chunks, bwd_chunks(d.type), [&](auto k) {
             const int at_once = k.NT / k.G, all = (d.rows + at_once - 1) / at_once;
             // at least so many that no chain of sums is longer than 256 rows
-            p.grid = p.spans = min(all, max(k.NT == 1024 ? 256 : 512, (all + 255) / 256));
+            p.grid = min(all, max(k.NT == 1024 ? 256 : 512, (all + 255) / 256));
+            // (1024 threads, one a compute unit: no more of them than take equally many turns;
+            // 1027 x 13001 with 206 instead of 256, 43 -> 40 us)
+            if (k.NT == 1024 && p.grid) p.grid = tiles_of(all, tiles_of(all, p.grid));
+            p.spans = p.grid;
         })) {
         in_parts(chunks, d.rows, &p);
         p.tiles = (chunks + PART_NT - 1) / PART_NT;
-        const int spans = max(min(max(1024 / p.tiles, d.rows / 256), d.rows), 1);
+        const int spans = max(min(max(1024 / p.tiles, tiles_of(d.rows, MOST_SPAN)), d.rows), 1);
         p.rows_of = d.rows ? (int)(((int64_t)d.rows + spans - 1) / spans) : 1;
         p.spans = (int)(((int64_t)d.rows + p.rows_of - 1) / p.rows_of);
         p.partial = round16((size_t)d.rows * p.parts * sizeof(float2));
@@ -863,11 +923,13 @@ int ach_layernorm_bwd(const ach_layernorm_desc *desc, const void *delta, int64_t
         if (rc) return rc;
     }
     if (updates) {
-        const int tiles = (d.features + 63) / 64;
-        hipLaunchKernelGGL(k_norm_bwd_join, dim3((unsigned)min(tiles, 1 << 20), 2),
-                           dim3(JOIN * 64), 0,
-                           st, (const float *)partial, p.spans, d.features, scale_updates,
-                           bias_updates, accumulate);
+        // few of them are one thread's (4 x 1000000 fp32 by 16 waves each: 84 us in all, 26 so)
+        const bool few = p.spans <= 32;
+        const int tiles = tiles_of(d.features, few ? 256 : 64);
+        hipLaunchKernelGGL(few ? &k_norm_bwd_join<1> : &k_norm_bwd_join<16>,
+                           dim3((unsigned)min(tiles, 1 << 20), 2), dim3(few ? 256 : 1024), 0, st,
+                           (const float *)partial, p.spans, d.features, scale_updates, bias_updates,
+                           accumulate);
         return check_launch();
     }
     return ACH_OK;

@@ -193,6 +193,23 @@ def test_many_rows(gpu, rows, n, kind):
         g.check()
 
 
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,n", [(515, 9001), (333, 16500), (70, 60001)])
+def test_many_long_rows(gpu, rows, n, kind):
+    """rows of 1024 threads in turns, spans of rows in parts"""
+    rng = np.random.default_rng(n)
+    x = Rows(rng.standard_normal((rows, n)) + rng.standard_normal((rows, 1)), kind)
+    s, b = parameters(rng, n)
+    f = Forward(gpu, x, s, b, keep=True)
+    f.call()
+    f.check()
+    d = Rows(rng.standard_normal((rows, n)) + 0.1, kind)
+    for from_kept in (False, True):
+        g = Backward(gpu, d, (x, 1e-5), s, from_kept, accumulate=int(from_kept))
+        g.call()
+        g.check()
+
+
 @pytest.mark.parametrize("n", [5, 300, 2500, 20000, 140000])
 def test_optional_arguments(gpu, n):
     """no scales, no biases, each output alone"""
