@@ -5,8 +5,8 @@
 // delta (its first 8 bits, the next 8, the last 8; one piece for bf16, two for
 // fp16, three for fp32): every product is exact and is summed in fp32.
 //
-// Tiles of 256 outputs x 128 inputs or 128 x 256, a wave 64 x 64 (bf16 also 128 x
-// 64) of it.  A stage of 32 rows of both operands is loaded two stages ahead,
+// Tiles of 256 outputs x 128 inputs or 128 x 256, on few rows 128 x 128, a wave 64 x
+// 64 (bf16 also 128 x 64) of it.  A stage of 32 rows of both operands is loaded two stages ahead,
 // turned into bf16 and stored as it lies in memory, [row][column]; the matrix
 // instructions want 8 rows of a column in a lane, which the transposing LDS loads
 // give: 16 lanes read 4 rows x 16 columns, and each gets a column of it.  Few tiles
@@ -370,7 +370,7 @@ bool fc_desc(const ach_fc_desc *d, ach_fc_desc *out)
 }
 
 struct Plan {
-    bool high;  // tiles of 256 outputs x 128 inputs, else 128 x 256
+    int o, i;  // outputs and inputs of a tile: 128 x 128, 256 x 128 or 128 x 256
     int ti, to, span, slices;
     size_t bytes;
 };
@@ -382,11 +382,21 @@ Plan fc_plan(const ach_fc_desc &d)
 {
     Plan p;
     const int stages = tiles_of(d.rows, DEPTH);
-    const int64_t high = (int64_t)tiles_of(d.outputs, 256) * tiles_of(d.inputs, 128),
+    // Small tiles, of which two workgroups run on a compute unit, one writing while the
+    // other multiplies: on few rows (128 x 9216 -> 4096 fp32 45 us, 51 in large ones, bf16
+    // 31 and 34; 256 rows fp32 69 and 73; 400 rows 105 and 107, bf16 54 and 52; 1000 x 4096
+    // -> 4096 fp32 99 and 91), and on some more where they keep more of the compute units
+    // busy without slices (600 x 2000 -> 1500 fp32 24 and 28, 1000 rows 34 and 32).
+    const int64_t small = (int64_t)tiles_of(d.outputs, 128) * tiles_of(d.inputs, 128),
+                  high = (int64_t)tiles_of(d.outputs, 256) * tiles_of(d.inputs, 128),
                   wide = (int64_t)tiles_of(d.outputs, 128) * tiles_of(d.inputs, 256);
-    p.high = high < wide || (high == wide && d.type == ACH_BF16);
-    p.to = tiles_of(d.outputs, p.high ? 256 : 128);
-    p.ti = tiles_of(d.inputs, p.high ? 128 : 256);
+    p.o = p.i = 128;
+    if (stages > (small <= 256 ? 20 : 8)) {
+        if (high < wide || (high == wide && d.type == ACH_BF16)) p.o = 256;
+        else p.i = 256;
+    }
+    p.to = tiles_of(d.outputs, p.o);
+    p.ti = tiles_of(d.inputs, p.i);
     const int64_t tiles = (int64_t)p.ti * p.to;
     // Up to 256 workgroups (long bf16 deltas, two a compute unit: 512), each of four
     // stages or more; as many as cost least, a stage 0.85 us and the sums of the slices
@@ -396,7 +406,7 @@ Plan fc_plan(const ach_fc_desc &d)
     const size_t bytes = (size_t)d.outputs * d.inputs * sizeof(float);
     const int one_round = tiles < 256 ? (int)(256 / tiles) : 1;
     int each = whole_turns(stages), slices = one_round;
-    if (d.type == ACH_BF16 && p.high && tiles < 512 && stages / one_round >= 256) {
+    if (d.type == ACH_BF16 && p.o == 256 && tiles < 512 && stages / one_round >= 256) {
         slices = min((int)(512 / tiles), MOST_SLICES);
         each = whole_turns(tiles_of(stages, slices));
     } else {
@@ -444,7 +454,8 @@ int fc_go(const Plan &p, const void *delta, const Fc &a, hipStream_t st)
 // compute unit.
 template <int TYPE> int fc_tiles(const Plan &p, const void *delta, const Fc &a, hipStream_t st)
 {
-    if (!p.high) return fc_go<TYPE, 2, 4, 2>(p, delta, a, st);
+    if (p.i == 256) return fc_go<TYPE, 2, 4, 2>(p, delta, a, st);
+    if (p.o == 128) return fc_go<TYPE, 2, 2, 2>(p, delta, a, st);
     if constexpr (TYPE == ACH_BF16) return fc_go<TYPE, 2, 2, 4>(p, delta, a, st);
     else return fc_go<TYPE, 4, 2, 2>(p, delta, a, st);
 }
