@@ -340,7 +340,28 @@ struct Bwd {
     int parts, span;  // chunks of a part
     float *partial;   // [2][spans][features]: sums over rows, or null
     int rows_of, spans;  // rows of one (rows in parts), their number
+    float *updates[2];   // of a single span, whose sums go there themselves; either may be null
+    bool updating, accumulate;
 };
+
+// Where a span's sums over rows go: `which` 0 the scales', 1 the biases'.
+__device__ __forceinline__ float *sums_of(const Bwd &a, int which, int span)
+{
+    if (!a.partial) return which ? a.updates[1] : a.updates[0];
+    return a.partial + ((size_t)which * a.spans + span) * a.features;
+}
+template <int VEC>
+__device__ __forceinline__ void store_sums(const Bwd &a, float *to, int left, float *v)
+{
+    if (a.accumulate) {
+        float old[VEC];
+        load_floats<VEC>(to, 0, left, 0.f, old);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] += old[i];
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) store_values<ACH_F32>(to + i, left - i, v + i);
+}
 
 // What the sums and the values need of a row's chunk: delta and x as they lie in
 // memory (or x_norm's codes and step).
@@ -497,11 +518,12 @@ k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
             load(r + step, c, st);
         }
     }
-    if (!a.partial) return;
+    if (!a.updating) return;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float *const v = which ? db : ds;
-        float *const to = a.partial + ((size_t)which * a.spans + blockIdx.x) * a.features;
+        float *const to = sums_of(a, which, blockIdx.x);
+        if (!to) continue;
         if (AT_ONCE > 1) {  // the workgroup's rows, in LDS as [value][row][thread]
             if (which) __syncthreads();
 #pragma unroll
@@ -514,16 +536,14 @@ k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
                 float s = 0.f;
 #pragma unroll
                 for (int k = 0; k < AT_ONCE; ++k) s += join[i * NT + k * G + u];
-                to[col] = s;
+                to[col] = a.accumulate ? to[col] + s : s;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < I; ++i) {
                 const int col = (t + i * G) * VEC;
                 if (IN_LDS) __builtin_memcpy(v, &in_lds[(which * I + i) * G + t], 16);
-#pragma unroll
-                for (int e = 0; e < VEC; e += 4)
-                    store_values<ACH_F32>(to + col + e, a.features - col - e, v + (IN_LDS ? 0 : i * VEC) + e);
+                store_sums<VEC>(a, to + col, a.features - col, v + (IN_LDS ? 0 : i * VEC));
             }
         }
     }
@@ -619,13 +639,10 @@ k_norm_bwd_values(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>
             write_values<TYPE>(dx + (r + u) * a.dx_stride + col, left, d, a.past);
         }
     }
-    if (!a.partial) return;
-    float *const to = a.partial + (size_t)span * a.features + col;
-#pragma unroll
-    for (int e = 0; e < VEC; e += 4) {
-        store_values<ACH_F32>(to + e, left - e, ds + e);
-        store_values<ACH_F32>(to + (size_t)a.spans * a.features + e, left - e, db + e);
-    }
+    if (!a.updating) return;
+    float *const to = sums_of(a, 0, span), *const to_b = sums_of(a, 1, span);
+    if (to) store_sums<VEC>(a, to + col, left, ds);
+    if (to_b) store_sums<VEC>(a, to_b + col, left, db);
 }
 
 // The partial sums of a column: few by one thread, more by a thread in each of 16 waves.
@@ -781,16 +798,19 @@ Plan bwd_plan(const ach_layernorm_desc &d)
             // (1024 threads, one a compute unit: no more of them than take equally many turns;
             // 1027 x 13001 with 206 instead of 256, 43 -> 40 us)
             if (k.NT == 1024 && p.grid) p.grid = tiles_of(all, tiles_of(all, p.grid));
+            // a second launch costs more than a second turn (2 x 4096 fp32 7.4 us, in two
+            // workgroups 9.9), but for the largest (2 x 16000 fp32 10.5 and 9.7)
+            if (k.NT < 1024 && all == 2) p.grid = 1;
             p.spans = p.grid;
         })) {
         in_parts(chunks, d.rows, &p);
         p.tiles = (chunks + PART_NT - 1) / PART_NT;
-        const int spans = max(min(max(1024 / p.tiles, tiles_of(d.rows, MOST_SPAN)), d.rows), 1);
+        const int spans = d.rows <= 4 ? 1 : min(max(1024 / p.tiles, tiles_of(d.rows, MOST_SPAN)), d.rows);
         p.rows_of = d.rows ? (int)(((int64_t)d.rows + spans - 1) / spans) : 1;
         p.spans = (int)(((int64_t)d.rows + p.rows_of - 1) / p.rows_of);
         p.partial = round16((size_t)d.rows * p.parts * sizeof(float2));
     }
-    p.bytes = p.partial + (size_t)2 * p.spans * d.features * sizeof(float);
+    p.bytes = p.partial + (size_t)2 * p.spans * d.features * sizeof(float);  // (a single span's: unused)
     return p;
 }
 
@@ -906,13 +926,13 @@ int ach_layernorm_bwd(const ach_layernorm_desc *desc, const void *delta, int64_t
     if ((int64_t)d.rows * p.parts > MOST_GROUPS || (int64_t)p.tiles * p.spans > MOST_GROUPS)
         return ACH_EINVAL;
     hipStream_t st = as_stream(s);
-    const bool updates = scale_updates || bias_updates;
-    float *const partial = (float *)((char *)ws + p.partial);
+    const bool updating = scale_updates || bias_updates, joined = updating && p.spans != 1;
+    float *const partial = joined ? (float *)((char *)ws + p.partial) : nullptr;
     const int vec = 16 / (int)size;
     if (d.rows) {
         Bwd a = {past_caches(d), d.rows, d.features, (d.features + vec - 1) / vec, d.stride, delta_stride, dx_stride,
-                 stats, scales, {}, (float2 *)ws, p.parts, p.span, updates ? partial : nullptr,
-                 p.rows_of, p.spans};
+                 stats, scales, {}, (float2 *)ws, p.parts, p.span, partial, p.rows_of, p.spans,
+                 {scale_updates, bias_updates}, updating, accumulate && !joined};
         if (checkpoint) a.k = kept(checkpoint, d.rows, d.features);
         int rc;
 #define CALL(TYPE)                                                                                 \
@@ -922,7 +942,7 @@ int ach_layernorm_bwd(const ach_layernorm_desc *desc, const void *delta, int64_t
 #undef CALL
         if (rc) return rc;
     }
-    if (updates) {
+    if (joined) {
         // few of them are one thread's (4 x 1000000 fp32 by 16 waves each: 84 us in all, 26 so)
         const bool few = p.spans <= 32;
         const int tiles = tiles_of(d.features, few ? 256 : 64);
