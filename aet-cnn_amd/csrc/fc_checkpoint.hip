@@ -6,23 +6,23 @@
 // fp16, three for fp32): every product is exact and is summed in fp32.
 //
 // Tiles of 256 outputs x 128 inputs or 128 x 256, on few rows 128 x 128, a wave 64 x
-// 64 (bf16 also 128 x 64) of it.  A stage of 32 rows of both operands is loaded two stages ahead,
-// turned into bf16 and stored as it lies in memory, [row][column]; the matrix
-// instructions want 8 rows of a column in a lane, which the transposing LDS loads
-// give: 16 lanes read 4 rows x 16 columns, and each gets a column of it.  Few tiles
-// share out the rows in slices, whose sums a second launch adds up in order.
+// 64 (bf16 also 128 x 64) of it.  A stage of 32 rows of both operands is loaded two
+// stages ahead, turned into bf16 and stored as it lies in memory, [row][column]; the
+// matrix instructions want 8 rows of a column in a lane, which the transposing LDS
+// loads give: 16 lanes read 4 rows x 16 columns, and each gets a column of it.  Few
+// tiles share out the rows in slices, whose sums a second launch adds up in order.
 //
-// Bound by the matrix units on many rows: 8192 x 8192 -> 4096 bf16 516 us, 1066
-// TFLOP/s (a matrix product of the library at 8192^3 in bf16: 1250); fp32 1357 us,
-// three passes of 405; 16384 x 4096 -> 1024 bf16 153 us, of which 15 are the four
-// slices' sums.  On few rows by a tile's start, its four stages and the writing
-// of dw, one after the other: 128 x 9216 -> 4096 fp32 56 us for 154 MB (without the
-// writing 50, only that 30).  What it took on 16384 x 4096 -> 1024 bf16: one stage ahead 399
-// us, two 233; offsets in the loads' windows instead of 64-bit addresses and clamps
+// Bound by the matrix units on many rows: 8192 x 8192 -> 4096 bf16 503 us, 1090
+// TFLOP/s (a matrix product of the library at 8192^3 in bf16: 1250); fp32 1326 us,
+// three passes of 415; 16384 x 4096 -> 1024 bf16 151 us, of which 14 are the four
+// slices' sums.  On few rows by the writing of dw, which two workgroups a compute unit
+// overlap in part with a tile's start and its stages: 128 x 9216 -> 4096 fp32 45 us for
+// 154 MB, fp16 37, bf16 31.  What it took on 16384 x 4096 -> 1024 bf16: one stage ahead
+// 399 us, two 233; offsets in the loads' windows instead of 64-bit addresses and clamps
 // (100 vector instructions for 8 of the matrix) 189; waves of 128 x 64 162; the
 // operands' loads among the matrix instructions 155; a last turn that loads nothing
-// 153.  Several tiles a workgroup, the next one's loads before the writing, gained
-// 2 us on few rows and lost 10% on many, where it spoils the loop's order.
+// 153.  Several tiles a workgroup, the next one's loads before the writing, lost 10% on
+// many rows, where it spoils the loop's order.
 #include "checkpoint.hpp"
 #include "pieces.hpp"
 

@@ -755,7 +755,7 @@ template <class F> bool for_bwd_kind(int chunks, int most, F f)
 // A row's chunks that fit the registers, four of each thread's, which a workgroup
 // of 1024 has 128 of; the backward pass holds two sums for each value, those of 8
 // values a chunk for two chunks.  (Twice as many in the forward pass, eight
-// chunks a thread: 1000 x 60000 bf16 91 us, in parts 78.)
+// chunks a thread: 1000 x 60000 bf16 91 us, in parts 73.)
 constexpr int FWD_CHUNKS = 4096;
 constexpr int bwd_chunks(int type) { return type == ACH_F32 ? 4096 : 2048; }
 
