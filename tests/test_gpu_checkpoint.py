@@ -178,6 +178,19 @@ def test_weight_gradient(gpu, rows, inputs, outputs, pad, shift, kind):
 
 
 @pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,inputs,outputs,pad,shift", [
+    (30, 4128, 2100, 0, 0), (30, 4101, 2101, 0, 0), (300, 4128, 2048, 0, 0), (270, 4128, 2101, 1, 1),
+    (300, 90, 6, 0, 1), (2000, 300, 5, 1, 0), (700, 1003, 301, 0, 0), (1200, 2050, 520, 3, 0)])
+def test_weight_gradient_by_tiles(gpu, rows, inputs, outputs, pad, shift, kind):
+    """tiles of every kind, in slices and not, and dw of more than the caches"""
+    rng = np.random.default_rng(rows + inputs)
+    d = Rows(rng.standard_normal((rows, outputs)) / rows * 64, kind, pad, shift)
+    w = Weights(gpu, d, activations(rng, rows, inputs), int(rows % 20 == 0))
+    w.call()
+    w.check()
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
 def test_weight_gradient_of_far_magnitudes(gpu, kind):
     """deltas and activations from near the smallest to near the largest: each
     output's own size decides its error"""
