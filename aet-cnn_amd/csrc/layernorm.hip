@@ -4,7 +4,7 @@
 // Bound by memory.  A row of up to 4096 chunks of 16 bytes (backward, 16-bit
 // types: 2048) lies in the registers of the G threads that share it, I chunks each,
 // so that it is read once: its sums, then its values.  Short rows share a wave, rows of
-// more than a few thousand values take a workgroup of 256 or 1024 threads.
+// more than a few thousand values take a workgroup of 256 to 1024 threads.
 // Workgroups run over rows and keep the parameters, and in the backward pass the
 // sums of the parameters' gradients, in registers; the next row is loaded while
 // one is worked on.  Longer rows are cut into parts, in two passes over memory.
@@ -388,12 +388,6 @@ template <int TYPE, bool KEPT> struct Pair {
             __builtin_memcpy(x, &c, sizeof(c));
         }
     }
-    __device__ __forceinline__ void forget_values()
-    {
-        forget(d);
-#pragma unroll
-        for (auto &v : x) asm volatile("" : "+v"(v));
-    }
     __device__ __forceinline__ void values(float2 st, float *dv, float *n) const
     {
         chunk_values<TYPE>(d, dv);
@@ -429,7 +423,7 @@ k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
            typename Elem<TYPE>::T *dx, Bwd a, float inv)
 {
     constexpr int VEC = Row<TYPE>::VEC, NT = G < 256 ? 256 : G, AT_ONCE = NT / G;
-    constexpr bool HOLD = I * VEC <= 16 && G < 1024, AHEAD = I * VEC <= 16;
+    constexpr bool HOLD = G < 1024;  // (registers)
     constexpr bool IN_LDS = bwd_lds<G, I>() > 0;  // the gradients' sums: a float4 of each thread after the other
     using P = Pair<TYPE, KEPT>;
     __shared__ float sh[2][2 * NT / 64];
@@ -461,7 +455,7 @@ k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
         __builtin_memcpy(&in_lds[i * G + t], ds, 16);
         __builtin_memcpy(&in_lds[(I + i) * G + t], db, 16);
     };
-    P c[I], ahead[AHEAD ? I : 1];
+    P c[I], ahead[I];
     float2 st, next;
     auto load = [&](int row, P *to, float2 &s) {
         s = stats_of(a, row);
@@ -470,8 +464,7 @@ k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
     };
     if (r < a.rows) load(r, c, st);
     for (int turn = 0; r < a.rows; r += step, turn ^= 1) {
-        const bool more = r + step < a.rows;
-        if (AHEAD && more) load(r + step, ahead, next);
+        if (r + step < a.rows) load(r + step, ahead, next);
         float sums[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < I; ++i) {
@@ -492,10 +485,6 @@ k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
         }
         if (dx) {
             row_sums<G, 2>(sums, sh[turn]);
-            if (I * VEC > 16) {
-#pragma unroll
-                for (int i = 0; i < I; ++i) c[i].forget_values();
-            }
             const float m1 = sums[0] * inv, m2 = sums[1] * inv;
 #pragma unroll
             for (int i = 0; i < I; ++i) {
@@ -510,13 +499,9 @@ k_norm_bwd(const typename Elem<TYPE>::T *delta, const typename Elem<TYPE>::T *x,
                 write_values<TYPE>(dx + r * a.dx_stride + col, a.features - col, d, a.past);
             }
         }
-        if (AHEAD) {
 #pragma unroll
-            for (int i = 0; i < I; ++i) c[i] = ahead[AHEAD ? i : 0];
-            st = next;
-        } else if (more) {
-            load(r + step, c, st);
-        }
+        for (int i = 0; i < I; ++i) c[i] = ahead[i];
+        st = next;
     }
     if (!a.updating) return;
 #pragma unroll
@@ -747,7 +732,8 @@ template <class F> bool for_bwd_kind(int chunks, int most, F f)
     else if (chunks <= 128) f(Kind<64, 2>());
     else if (chunks <= 256) f(Kind<256, 1>());
     else if (chunks <= 512) f(Kind<256, 2>());
-    else if (chunks <= 1024) f(Kind<256, 4>());
+    else if (chunks <= 1024) f(Kind<512, 2>());
+    else if (chunks <= 1536) f(Kind<768, 2>());
     else if (chunks <= 2048) f(Kind<1024, 2>());
     else f(Kind<1024, 4>());
     return true;
@@ -796,9 +782,14 @@ Plan bwd_plan(const ach_layernorm_desc &d)
     if (!for_bwd_kind(chunks, bwd_chunks(d.type), [&](auto k) {
             const int at_once = k.NT / k.G, all = (d.rows + at_once - 1) / at_once;
             // at least so many that no chain of sums is longer than 256 rows
-            p.grid = min(all, max(k.NT == 1024 ? 256 : 512, (all + 255) / 256));
-            // (1024 threads, one a compute unit: no more of them than take equally many turns;
-            // 1027 x 13001 with 206 instead of 256, 43 -> 40 us)
+            // two a compute unit, of large ones that fill its registers one (300 x 8000 fp16 14 us,
+            // with two 17, four chunks of each of 256 threads 18), and of those of 512 threads
+            // that share it also where the partial sums are a large part of the work (700 x
+            // 3000 fp32 12 and 13, 10000 rows 91 and 71)
+            const bool one = k.NT > 512 || (k.NT == 512 && (d.type != ACH_F32 || d.rows <= 1024));
+            p.grid = min(all, max(one ? 256 : 512, (all + 255) / 256));
+            // of 1024 threads no more than take equally many turns (1027 x 13001 with 206
+            // instead of 256, 43 -> 40 us; 700 x 3000 fp32 with 234 12 -> 13)
             if (k.NT == 1024 && p.grid) p.grid = tiles_of(all, tiles_of(all, p.grid));
             // a second launch costs more than a second turn (2 x 4096 fp32 7.4 us, in two
             // workgroups 9.9), but for the largest (2 x 16000 fp32 10.5 and 9.7)
