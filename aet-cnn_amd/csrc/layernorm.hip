@@ -65,10 +65,11 @@ template <int G, int N, class V> __device__ __forceinline__ void row_sums(V *v, 
         for (int i = 0; i < N; ++i) v[i] += sh[w * N + i];
 }
 
-// Values into y or dx.  What the L2 caches (8 of 4 MB) do not hold is stored past
-// the caches, where it would take the place of rows that are still to be read
-// (4096 x 8192 bf16 forward: 32 us, 23 past them; 128 x 186624 fp32, which is read
-// twice: 66 and 55).
+// Values into y or dx.  What the L2 caches (8 of 4 MB) do not hold beside the rows that
+// are read, as much again, is stored past the caches, where it would take the place of
+// rows that are still to be read (4096 x 8192 bf16 forward: 32 us, 23 past them; 128 x
+// 186624 fp32, which is read twice: 66 and 55; backward 2048 x 4000 fp32, 33 MB, 29 and
+// 23, 1100 x 4000, 18 MB, 16.6 and 16.4, forward 9.1 and 7.9).
 template <int TYPE>
 __device__ __forceinline__ void write_values(typename Elem<TYPE>::T *p, int left, const float *v, bool past)
 {
@@ -689,7 +690,7 @@ size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 bool past_caches(const ach_layernorm_desc &d)
 {
-    return (size_t)d.rows * d.features * elem_size(d.type) > (size_t)32 << 20;
+    return (size_t)d.rows * d.features * elem_size(d.type) > (size_t)16 << 20;
 }
 
 // Chunks of a row, in whole blocks of a checkpoint.
