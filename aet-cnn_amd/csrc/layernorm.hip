@@ -125,10 +125,12 @@ struct Fwd {
     int parts, span; // chunks of a part
 };
 
-// From the sums of x - first and of their squares, in 64 bits.  As the row's first
-// value is one of its n, the mean is at most sqrt(n) deviations from it, and the
-// subtraction of its square loses log2 n of the 53 bits at most.  (The variance
-// passes a float's range where the values pass 1.8e19.)
+// From the sums of x - first and of their squares, differences and sums in 64 bits:
+// where the first value is far from the others, these differences would all round
+// alike in 32, and the mean move by as much (186624 values of 0.3 behind one of 1000:
+// by 4e-5 of itself).  As the row's first value is one of its n, the mean is at most
+// sqrt(n) deviations from it, and the subtraction of its square loses log2 n of the 53
+// bits at most.  (The variance passes a float's range where the values pass 1.8e19.)
 __device__ __forceinline__ float2 statistics(double s, double q, float first, double inv, float eps)
 {
     const double m = s * inv, var = fmax(q * inv - m * m, 0.) + (double)eps;
@@ -148,7 +150,7 @@ __device__ __forceinline__ void add_values(const float *v, float first, double &
 {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-        const double d = (double)(v[i] - first);
+        const double d = (double)v[i] - (double)first;
         s += d;
         q = fma(d, d, q);
     }

@@ -1,0 +1,51 @@
+"""Layer norm's statistics against bounds of 64-bit sums (norm_bounds.py), where
+a row's first value is far from the others."""
+import numpy as np
+import pytest
+
+import norm_bounds
+from aetcnn import BF16, F16, F32
+from test_gpu_layernorm import Forward, parameters
+from test_gpu_logits import Rows
+
+pytestmark = pytest.mark.gpu
+
+
+def check_forward(gpu, x, s, b, eps=1e-5, keep=True):
+    f = Forward(gpu, x, s, b, eps, keep=keep)
+    f.want = norm_bounds.forward(x.x, s, b, eps, x.kind)
+    f.call()
+    f.check()
+    return f
+
+
+# rows of a part of a wave, a wave, workgroups of every size, and in parts
+LENGTHS = [8, 40, 300, 1000, 4096, 9000, 16384, 17001, 186624]
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("n", LENGTHS)
+def test_a_first_value_far_from_the_others(gpu, n, kind):
+    """a constant background, whose differences from the first value all round
+    alike, and one that is not; the same values in the other order"""
+    rng = np.random.default_rng(n)
+    s, b = parameters(rng, n)
+    far = np.array([1000.0, -1000.0, 3e4, 0.3])
+    for spread in (0.0, 0.01):
+        x = 0.3 + spread * rng.standard_normal((4, n))
+        x[:, 0] = far
+        seen = []
+        for order in (slice(None), slice(None, None, -1)):
+            f = check_forward(gpu, Rows(x[:, order], kind), s, b)
+            seen.append(f.stats.numpy()[:, 0].astype(np.float64))
+        # the order of the values is of no consequence for their mean
+        assert (np.abs(seen[0] - seen[1]) <= 2.0 ** -22 * np.abs(seen[1]) + 2.0 ** -30).all()
+
+
+@pytest.mark.parametrize("n", LENGTHS)
+def test_a_first_value_far_above_all(gpu, n):
+    rng = np.random.default_rng(n + 1)
+    s, b = parameters(rng, n)
+    x = rng.standard_normal((5, n))
+    x[:, 0] = 1e3, 1e6, -1e9, 1e15, 3e37
+    check_forward(gpu, Rows(x, F32), s, b)
