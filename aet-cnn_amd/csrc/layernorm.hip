@@ -145,6 +145,13 @@ __device__ __forceinline__ float2 statistics(double s, double q, float first, do
     return make_float2(mean, q < (double)INFINITY ? r : NAN);
 }
 
+// x_norm from a row's mean and rstd, in halves: x - mean may pass a float's range
+// where neither does (both factors are exact, so the result is that of the whole)
+__device__ __forceinline__ float normalised(float x, float2 st)
+{
+    return fmaf(x, .5f, -.5f * st.x) * (st.y + st.y);
+}
+
 template <int VEC>
 __device__ __forceinline__ void add_values(const float *v, float first, double &s, double &q)
 {
@@ -166,7 +173,7 @@ __device__ __forceinline__ void put_values(const Fwd &a, typename Elem<TYPE>::T 
     float n[VEC];
     chunk_values<TYPE>(c, n);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) n[i] = (n[i] - st.x) * st.y;
+    for (int i = 0; i < VEC; ++i) n[i] = normalised(n[i], st);
     if (KEEP) {
         if (left < VEC) {
 #pragma unroll
@@ -403,7 +410,7 @@ template <int TYPE, bool KEPT> struct Pair {
             __builtin_memcpy(&c, x, sizeof(c));
             chunk_values<TYPE>(c, n);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) n[i] = (n[i] - st.x) * st.y;
+            for (int i = 0; i < VEC; ++i) n[i] = normalised(n[i], st);
         }
     }
 };

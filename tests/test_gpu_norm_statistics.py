@@ -5,7 +5,7 @@ import pytest
 
 import norm_bounds
 from aetcnn import BF16, F16, F32
-from test_gpu_layernorm import Forward, parameters
+from test_gpu_layernorm import Backward, Forward, parameters
 from test_gpu_logits import Rows
 
 pytestmark = pytest.mark.gpu
@@ -49,3 +49,26 @@ def test_a_first_value_far_above_all(gpu, n):
     x = rng.standard_normal((5, n))
     x[:, 0] = 1e3, 1e6, -1e9, 1e15, 3e37
     check_forward(gpu, Rows(x, F32), s, b)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("n", [3, 33, 300, 1000, 4096, 9000, 17001])
+def test_values_further_apart_than_the_largest(gpu, n, kind):
+    """differences pass a float's range, from the first value or from the mean;
+    statistics and outputs do not, whatever the order"""
+    rng = np.random.default_rng(n)
+    s, b = parameters(rng, n)
+    x = np.full((6, n), 3e38)
+    x[0, 0], x[0, -1] = 0, -3e38         # behind a small first value
+    x[1, 0] = -3e38                      # all far from the first
+    x[2, n // 2] = -3e38
+    x[3, ::2] = -3e38
+    x[4] = rng.uniform(-3.3e38, 3.3e38, n)
+    x[5] = -3e38 * (np.arange(n) == n - 1) + 1e38
+    f = check_forward(gpu, Rows(x, kind), s, b)
+    st = f.stats.numpy().astype(np.float64)
+    with np.errstate(over="raise"):
+        assert np.isfinite(st).all() and (np.abs(st[:, 1] / f.want["rstd"][0] - 1) < 2.0 ** -20).all()
+    g = Backward(gpu, Rows(rng.standard_normal((6, n)), kind), (f.x, 1e-5), s)
+    g.call()
+    g.check()
