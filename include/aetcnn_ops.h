@@ -525,10 +525,11 @@ int ach_checkpoint_unpack(const ach_checkpoint_desc *d, const void *checkpoint, 
  * among themselves.  eps from 1e-12 to 1.  Everything is computed in 32 bits
  * or more and rounded once where an output has fewer; results do not depend
  * on the run (no float atomics).  A row that holds a NaN or an infinity gives
- * NaN in all its outputs, statistics that are not finite, and NaN in the
- * updates; other rows are not touched by it.  Workspaces are aligned to 16
- * bytes and belong to one call at a time.  Outputs overlap neither one another
- * nor the inputs, but for what is said below.                              */
+ * NaN in all its outputs, statistics that are not finite, and NaN in
+ * scale_updates (bias_updates are sums of delta alone); other rows are not
+ * touched by it.  Workspaces are aligned to 16 bytes and belong to one call at
+ * a time.  Outputs overlap neither one another nor the inputs, but for what is
+ * said below.                                                              */
 typedef struct {
     int rows, features;
     int type;             /* of x, y, delta and dx                           */
