@@ -5,7 +5,8 @@ import pytest
 
 import norm_bounds
 from aetcnn import BF16, F16, F32
-from test_gpu_layernorm import Backward, Forward, parameters
+from test_gpu_checkpoint import activations
+from test_gpu_layernorm import SIZES, Backward, Forward, parameters
 from test_gpu_logits import Rows
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +73,30 @@ def test_values_further_apart_than_the_largest(gpu, n, kind):
     g = Backward(gpu, Rows(rng.standard_normal((6, n)), kind), (f.x, 1e-5), s)
     g.call()
     g.check()
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,n,pad,shift", SIZES + [(1500, 600, 0, 0), (700, 3000, 0, 0), (70, 60001, 0, 0)])
+def test_ordinary_rows(gpu, rows, n, pad, shift, kind):
+    """each with a level of its own, up to far above its deviations"""
+    rng = np.random.default_rng(rows * 3 + n)
+    x = activations(rng, rows, n) + rng.standard_normal((rows, 1)) * 10.0 ** rng.integers(-2, 4, (rows, 1))
+    s, b = parameters(rng, n)
+    check_forward(gpu, Rows(x, kind, pad, shift), s, b)
+
+
+@pytest.mark.parametrize("n", [20, 1000, 5000, 40000])
+@pytest.mark.parametrize("eps", [1e-12, 1e-5, 1.0])
+def test_values_at_the_ends(gpu, n, eps):
+    rng = np.random.default_rng(n)
+    x = activations(rng, 8, n)
+    x[0] = 3.25
+    x[1] = 1e4 + rng.standard_normal(n) * 0.01
+    x[2] = 1e4 + np.arange(n) % 2 * 2.0 ** -10        # one step apart
+    x[3, 0] = 1e6
+    x[4] *= 1e-30
+    x[5] *= 1e15
+    x[6] = np.where(np.arange(n) % 2, 1e25, -1e25)
+    x[7] = 0
+    s, b = parameters(rng, n)
+    check_forward(gpu, Rows(x, F32), s, b, eps)
