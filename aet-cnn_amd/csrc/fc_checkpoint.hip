@@ -3,7 +3,10 @@
 //
 // A code times its power of two is a bf16 number, and so is each piece of a
 // delta (its first 8 bits, the next 8, the last 8; one piece for bf16, two for
-// fp16, three for fp32): every product is exact and is summed in fp32.
+// fp16, three for fp32): every product is exact and is summed in fp32.  The last two
+// pieces of fp32 are scaled by kPieceUp, as those of values under 2^-110 would lie below
+// bf16's smallest number (a relative error of 1e-6 at 2^-115, 1e-4 at 2^-122).  Sums that
+// are not finite so, near deltas or sums of 2^111, are done again in fp32.
 //
 // Tiles of 256 outputs x 128 inputs or 128 x 256, on few rows 128 x 128, a wave 64 x
 // 64 (bf16 also 128 x 64) of it.  A stage of 32 rows of both operands is loaded two
@@ -25,6 +28,8 @@
 // many rows, where it spoils the loop's order.
 #include "checkpoint.hpp"
 #include "pieces.hpp"
+
+#include <math.h>
 
 namespace ach {
 namespace {
@@ -99,6 +104,7 @@ template <int TYPE> struct Eight {
                 for (int q = 0; q < Pieces<TYPE>::N; ++q) {
                     p[q][i] = upper_halves(a, b);
                     a = below(a), b = below(b);
+                    if (TYPE == ACH_F32 && q == 0) a *= kPieceUp, b *= kPieceUp;
                 }
             }
         }
@@ -142,6 +148,29 @@ template <int PITCH> __device__ __forceinline__ v8bf fragment(const short *p)
 // chunks inside a row instead, early and then shifted (EARLY), or one by one
 // (SINGLE, under 8 outputs).
 enum { WHOLE, EARLY, SINGLE };
+
+// The sums of a lane's outputs o .. o + 3, o + 8 .. in fp32, for inputs i and i + 32.
+template <int TYPE>
+__device__ __forceinline__ void plain_sums(const typename Elem<TYPE>::T *delta, const Fc &a, int r0, int r1,
+                                           int o, int i, float (*v)[16])
+{
+    // (what lies behind the last output or input is not written)
+    const int first = min(i, a.k.width - 1), second = min(i + 32, a.k.width - 1);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[0][e] = v[1][e] = 0.f;
+    for (int r = r0; r < r1; ++r) {
+        const int8_t *const codes = a.k.codes + (size_t)r * a.k.width;
+        const uint8_t *const steps = a.k.steps + (size_t)r * (a.k.width / KEPT_BLOCK);
+        const float x0 = (float)codes[first] * kept_scale(steps[first / KEPT_BLOCK]),
+                    x1 = (float)codes[second] * kept_scale(steps[second / KEPT_BLOCK]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float d = (float)delta[r * a.stride + min(o + 8 * (e >> 2) + (e & 3), a.outputs - 1)];
+            v[0][e] = fmaf(d, x0, v[0][e]);
+            v[1][e] = fmaf(d, x1, v[1][e]);
+        }
+    }
+}
 
 // WO x WI waves of 32 MO outputs x 64 inputs
 template <int TYPE, int WO, int WI, int MO> struct Tile {
@@ -309,13 +338,38 @@ k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
     const int col = i0 + tid % CHUNKS * 4, left = a.inputs - col;
 #pragma unroll
     for (int i = 0; i < MO; ++i) {
+        float v[2][16];
+        if constexpr (TYPE == ACH_F32) {
+            float all = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    v[j][e] = fmaf(lo[i][j][e], 1 / kPieceUp, hi[i][j][e]);
+                    all = __builtin_elementwise_maximum(all, fabsf(v[j][e]));
+                }
+            if (__builtin_expect(__any(!(all < INFINITY)), 0)) {
+                float plain[2][16];
+                plain_sums<TYPE>(delta, a, r0, r1, o0 + (wo * MO + i) * 32 + 4 * (lane >> 5),
+                                 i0 + wi * 64 + (lane & 31), plain);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[j][e] = fabsf(v[j][e]) < INFINITY ? v[j][e] : plain[j][e];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[j][e] = P > 1 ? hi[i][j][e] + lo[P > 1 ? i : 0][j][e] : hi[i][j][e];
+        }
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 turned[(wo * 32 + 4 * (lane >> 5) + 8 * (e >> 2) + (e & 3)) * S::TP + wi * 64 + j * 32 +
-                       (lane & 31)] = P > 1 ? hi[i][j][e] + lo[P > 1 ? i : 0][j][e] : hi[i][j][e];
+                       (lane & 31)] = v[j][e];
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 32 * WO / ROWS; ++k) {

@@ -568,9 +568,11 @@ int ach_layernorm_bwd(const ach_layernorm_desc *d, const void *delta, int64_t de
  * of `type`, `stride` elements apart (0: outputs), at any element address; rows 0
  * to 2^30, inputs, outputs and stride up to 2^23.  accumulate as above (rows 0 and
  * accumulate 0: zeros).  Every product is exact and the sums are in 32 bits: an
- * fp32 delta is taken as three bf16 pieces (fp16: two), of which parts below
- * 2^-126 are lost.  What an infinity or a NaN in delta, or a block of NaN in x,
- * is summed into is not finite; results do not depend on the run.           */
+ * fp32 delta is taken as three bf16 pieces (fp16: two), down to the last bit of
+ * the smallest.  What an infinity or a NaN in delta, or a block of NaN in x, is
+ * summed into is not finite; results do not depend on the run.  fp32 deltas or
+ * sums near 2^111 and above, infinities and NaN cost time: what they are summed
+ * into is done again without the matrix instructions.                      */
 typedef struct {
     int rows, inputs, outputs;
     int type;             /* of delta                                        */
