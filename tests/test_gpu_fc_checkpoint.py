@@ -75,3 +75,24 @@ def test_large_deltas_in_one_slice(gpu):
     w.call()
     want, size = w.delta.x.T @ w.k.values + w.old, np.abs(w.delta.x).T @ np.abs(w.k.values) + np.abs(w.old)
     assert (np.abs(w.read() - want) <= 2 * (4096 + 16) * U * size).all()
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+@pytest.mark.parametrize("sign", [1, 0])
+def test_one_long_chain(gpu, kind, sign):
+    """so many tiles that one workgroup sums up all rows: every product one after
+    the other, of both signs or of one, where all roundings go one way"""
+    rng = np.random.default_rng(14)
+    rows, inputs, outputs = 6000, 4127, 2101
+    x, d = activations(rng, rows, inputs), rng.standard_normal((rows, outputs))
+    if not sign:
+        x, d = np.abs(x), np.abs(d)
+    w = Weights(gpu, Rows(d, kind), x)
+    assert w.nb == 0
+    w.call()
+    some = rng.choice(outputs, 40, replace=False)
+    some[:2] = 0, outputs - 1
+    dx = w.delta.x[:, some]
+    want, size = dx.T @ w.k.values, np.abs(dx).T @ np.abs(w.k.values)
+    off = np.abs(w.read()[some].astype(np.float64) - want)
+    assert (off <= 2 * (rows + 16) * U * size).all(), (off / size).max() / U
