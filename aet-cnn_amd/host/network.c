@@ -279,6 +279,7 @@ static int conv_backward(an_network *net, an_layer *l, an_state st)
     ach_stream_t s = net->stream;
     const size_t nout = (size_t)l->batch * l->outputs;
     if (l->batch_normalize) {
+        if (l->x == net->x_shared && !l->x_kept) return ACH_EUNSUPPORTED; /* x is another layer's by now */
         int act = ACH_LINEAR;
         if ((l->activation == ACH_LEAKY || l->activation == ACH_RELU) && !l->x_kept &&
             !output_masked_unreverted(net, l))
@@ -845,6 +846,14 @@ static size_t layer_ws(const an_layer *l, int batch)
     return ws;
 }
 
+/* whether an_backward runs a layer's backward                              */
+static int backward_reaches(const an_network *net, const an_layer *l)
+{
+    for (int i = l->index; i < net->n; ++i)
+        if (net->layers[i]->stopbackward) return 0;
+    return !l->onlyforward;
+}
+
 /* lay out every device tensor; b->dry only measures */
 static void layout(an_network *net, bump *b)
 {
@@ -882,7 +891,8 @@ static void layout(an_network *net, bump *b)
         if (l->type == AN_CONVOLUTIONAL && l->batch_normalize) {
             if (net->checkpoints) {
                 l->x = net->x_shared;
-                l->x_kept = take(b, ach_checkpoint_bytes(l->batch, l->outputs));
+                if (backward_reaches(net, l))
+                    l->x_kept = take(b, ach_checkpoint_bytes(l->batch, l->outputs));
             } else {
                 l->x = (float *)take(b, sizeof(float) * bo);
             }

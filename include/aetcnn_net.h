@@ -182,8 +182,10 @@ int an_set_subdivisions(an_network *net, int subdivisions);
  * memory, the tensor itself lying in one buffer that these layers share.  The
  * forward pass and the activations' gradients are the same bit for bit;
  * what the batch-norm backward makes of the rounded values differs by their
- * rounding, at most a 127th of the largest of 32 neighbours each.  No
- * counterpart in the reference.  Before an_finalize (ACH_EINVAL after).    */
+ * rounding, at most a 127th of the largest of 32 neighbours each.  Layers that
+ * an_backward does not reach (stopbackward, onlyforward) keep nothing, and their
+ * an_layer_backward is refused (ACH_EUNSUPPORTED).  No counterpart in the
+ * reference.  Before an_finalize (ACH_EINVAL after).                       */
 int an_set_checkpoints(an_network *net, int on);
 /* The per-layer cfg options the reference's CPU path acts on (NLayer.h:
  * 115-125, read by NetworkFactory.createLayer / createNetwork,
