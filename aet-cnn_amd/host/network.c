@@ -868,14 +868,19 @@ static void layout(an_network *net, bump *b)
     net->zero_region = b->dry ? NULL : (float *)(b->base + zstart);
     net->zero_floats = (b->off - zstart) / sizeof(float);
     /* 2. per-layer tensors (flat parameters are carved by an_finalize) */
-    size_t shared = 0;
+    /* the batch-norm layers' x: each its own, or a shared one and what is kept
+     * of each, if that is less (one layer's alone is more)                  */
+    size_t plain = 0, shared = 0, kept = 0;
     for (int i = 0; i < net->n; ++i) {
         const an_layer *l = net->layers[i];
-        if (net->checkpoints && l->type == AN_CONVOLUTIONAL && l->batch_normalize &&
-            B * l->outputs > shared)
-            shared = B * l->outputs;
+        if (l->type != AN_CONVOLUTIONAL || !l->batch_normalize) continue;
+        const size_t x = al(sizeof(float) * B * l->outputs);
+        plain += x;
+        if (x > shared) shared = x;
+        if (backward_reaches(net, l)) kept += al(ach_checkpoint_bytes(l->batch, l->outputs));
     }
-    if (shared) net->x_shared = (float *)take(b, sizeof(float) * shared);
+    const int keep = net->checkpoints && shared + kept < plain;
+    if (keep) net->x_shared = (float *)take(b, shared);
     for (int i = 0; i < net->n; ++i) {
         an_layer *l = net->layers[i];
         const size_t bo = B * l->outputs;
@@ -889,7 +894,7 @@ static void layout(an_network *net, bump *b)
         l->output = (float *)take(b, sizeof(float) * bo);
         if (!l->zero_delta) l->delta = (float *)take(b, sizeof(float) * bo);
         if (l->type == AN_CONVOLUTIONAL && l->batch_normalize) {
-            if (net->checkpoints) {
+            if (keep) {
                 l->x = net->x_shared;
                 if (backward_reaches(net, l))
                     l->x_kept = take(b, ach_checkpoint_bytes(l->batch, l->outputs));

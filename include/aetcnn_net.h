@@ -179,10 +179,12 @@ float an_current_rate(an_network *net);
 int an_set_subdivisions(an_network *net, int subdivisions);
 /* Batch-norm layers keep their pre-norm tensor, which only their backward
  * reads, in 8 bits instead of 32 (on = 1; ach_checkpoint_pack): 0.26 of its
- * memory, the tensor itself lying in one buffer that these layers share.  The
- * forward pass and the activations' gradients are the same bit for bit;
- * what the batch-norm backward makes of the rounded values differs by their
- * rounding, at most a 127th of the largest of 32 neighbours each.  Layers that
+ * memory, the tensor itself lying in one buffer that these layers share.  Where
+ * both together would take more than the tensors in 32 bits, as with a single
+ * layer, these stay as they are without it.  The forward pass and the
+ * activations' gradients are the same bit for bit; what the batch-norm backward
+ * makes of the rounded values differs by their rounding, at most a 127th of the
+ * largest of 32 neighbours each.  Layers that
  * an_backward does not reach (stopbackward, onlyforward) keep nothing, and their
  * an_layer_backward is refused (ACH_EUNSUPPORTED).  No counterpart in the
  * reference.  Before an_finalize (ACH_EINVAL after).                       */

@@ -57,3 +57,36 @@ def test_layers_without_a_backward_keep_nothing(gpu, options, reached):
     net.train(x, t)  # the refusal changed nothing
     plain.close()
     net.close()
+
+
+@pytest.mark.parametrize("widths", [(16,), (64, 8), (8, 64, 8), (16, 16, 16)])
+def test_never_more_memory(gpu, widths):
+    """a shared buffer beside one large layer's codes would be more than its
+    tensor: it stays in 32 bits, and training as it is"""
+    def small(on):
+        aetcnn.net_lib().an_rand_seed(5)
+        net = aetcnn.Network(B, 12, 10, 3)
+        net.checkpoints(on)
+        net.hyper(0.01, 0.9, 1e-4)
+        for w in widths:
+            net.conv(w, 3, 1, 1, LEAKY, 1)
+        net.connected(10, LINEAR, 0)
+        net.softmax()
+        net.finalize()
+        return net
+    plain, net = small(False), small(True)
+    sizes = [w * 120 for w in widths]
+    kept = sum(kept_bytes(n) for n in sizes) + max(sizes) * 4 * B < sum(sizes) * 4 * B
+    assert (net.device_bytes() < plain.device_bytes()) == kept and net.device_bytes() <= plain.device_bytes()
+    for i in range(len(widths)):
+        assert (net.buffer(i, 17) is not None) == kept and (net.buffer(i, 12) is None) == kept
+    for k in range(2):
+        x, t = batch(40 + k, B, size=12 * 10 * 3)
+        assert kept or plain.train(x, t) == net.train(x, t)
+    if not kept:
+        for i in range(net.n_layers()):
+            for which in (2, 4, 6):
+                u = plain.buffer(i, which)
+                assert u is None or np.array_equal(u, net.buffer(i, which))
+    plain.close()
+    net.close()
