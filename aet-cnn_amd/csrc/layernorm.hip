@@ -925,11 +925,12 @@ int ach_layernorm_bwd(const ach_layernorm_desc *desc, const void *delta, int64_t
     if (!aligned(scale_updates, 4) || !aligned(bias_updates, 4)) return ACH_EINVAL;
     if (dx == delta && dx_stride != delta_stride) return ACH_EINVAL;
     const Plan p = bwd_plan(d);
-    if (p.bytes && (!ws || ws_bytes < p.bytes || !aligned(ws, 16))) return ACH_EWORKSPACE;
+    const bool updating = scale_updates || bias_updates, joined = updating && p.spans != 1;
+    const size_t bytes = updating ? p.bytes : p.partial;  // (without updates no sums over rows)
+    if (bytes && (!ws || ws_bytes < bytes || !aligned(ws, 16))) return ACH_EWORKSPACE;
     if ((int64_t)d.rows * p.parts > MOST_GROUPS || (int64_t)p.tiles * p.spans > MOST_GROUPS)
         return ACH_EINVAL;
     hipStream_t st = as_stream(s);
-    const bool updating = scale_updates || bias_updates, joined = updating && p.spans != 1;
     float *const partial = joined ? (float *)((char *)ws + p.partial) : nullptr;
     const int vec = 16 / (int)size;
     if (d.rows) {

@@ -553,7 +553,8 @@ int ach_layernorm_fwd(const ach_layernorm_desc *d, const void *x, const float *s
  * with accumulate 0 (rows 0 then gives zeros).  delta and dx have rows
  * delta_stride and dx_stride apart (0: features); dx may be delta itself with
  * the same stride.  dx, scale_updates and bias_updates may be NULL, not all
- * three; scales NULL: 1.                                                   */
+ * three; scales NULL: 1.  For dx alone, rows of up to 16384 values need no
+ * workspace (ws NULL).                                                     */
 size_t ach_layernorm_bwd_workspace(const ach_layernorm_desc *d);
 int ach_layernorm_bwd(const ach_layernorm_desc *d, const void *delta, int64_t delta_stride,
                       const void *x, const void *checkpoint, const float *stats,
