@@ -17,10 +17,10 @@
 // tiles share out the rows in slices, whose sums a second launch adds up in order.
 //
 // Bound by the matrix units on many rows: 8192 x 8192 -> 4096 bf16 503 us, 1090
-// TFLOP/s (a matrix product of the library at 8192^3 in bf16: 1250); fp32 1326 us,
+// TFLOP/s (a matrix product of the library at 8192^3 in bf16: 1250); fp32 1340 us,
 // three passes of 415; 16384 x 4096 -> 1024 bf16 151 us, of which 14 are the four
 // slices' sums.  On few rows by the writing of dw, which two workgroups a compute unit
-// overlap in part with a tile's start and its stages: 128 x 9216 -> 4096 fp32 45 us for
+// overlap in part with a tile's start and its stages: 128 x 9216 -> 4096 fp32 47 us for
 // 154 MB, fp16 37, bf16 31.  What it took on 16384 x 4096 -> 1024 bf16: one stage ahead
 // 399 us, two 233; offsets in the loads' windows instead of 64-bit addresses and clamps
 // (100 vector instructions for 8 of the matrix) 189; waves of 128 x 64 162; the
@@ -147,7 +147,8 @@ template <int PITCH> __device__ __forceinline__ v8bf fragment(const short *p)
 // next row, or zeros behind the last one (WHOLE).  The range check is by dwords, so
 // 16-bit values, which would lose the last one of an odd number, are loaded whole
 // chunks inside a row instead, early and then shifted (EARLY), or one by one
-// (SINGLE, under 8 outputs).
+// (SINGLE, under 8 outputs; its 16 loads a stage take addresses that in fp16 tiles of 128 x
+// 128 lie in part in memory, six of them read back in the loop: 1000 x 3000 -> 6 11.5 us).
 enum { WHOLE, EARLY, SINGLE };
 
 // The sums of a lane's outputs o .. o + 3, o + 8 .. in fp32, for inputs i and i + 32.
@@ -186,6 +187,7 @@ template <int TYPE, int WO, int WI, int MO> struct Tile {
     static constexpr size_t LDS = 2 * sizeof(Stage) > OUT ? 2 * sizeof(Stage) : OUT;
 };
 
+// (fp32 tiles of 128 x 256 keep three values for after the loop in memory.)
 template <int TYPE, int WO, int WI, int MO, int HOW>
 __global__ void __launch_bounds__(64 * WO * WI, 2)
 k_fc_wgrad(const typename Elem<TYPE>::T *delta, Fc a)
@@ -453,11 +455,15 @@ Plan fc_plan(const ach_fc_desc &d)
     p.to = tiles_of(d.outputs, p.o);
     p.ti = tiles_of(d.inputs, p.i);
     const int64_t tiles = (int64_t)p.ti * p.to;
-    // Up to 256 workgroups (long bf16 deltas, two a compute unit: 512), each of four
-    // stages or more; as many as cost least, a stage 0.85 us and the sums of the slices
-    // 3 us and their writing and reading: 300 x 2000 -> 1500 fp32 19 us in one, 23 in
-    // two, 27 in three; 600 rows 28, 27, 32; 2000 x 4096 -> 1000 bf16 42, 38 in two, 41
-    // in three; 1531 x 1003 -> 777 fp16 49, 21 in six to nine.
+    // Up to 256 workgroups, each of four stages or more; as many as cost least, a stage
+    // 0.85 us and the sums of the slices 3 us and their writing and reading: 300 x 2000 ->
+    // 1500 fp32 19 us in one, 23 in two, 27 in three; 600 rows 28, 27, 32; 2000 x 4096 ->
+    // 1000 bf16 42, 38 in two, 41 in three; 1531 x 1003 -> 777 fp16 49, 21 in six to nine.
+    // Long bf16 deltas, from 256 stages of a slice on, two a compute unit: 512.  4096 ->
+    // 1024 of 16384 rows 147 us, with up to 256 154; 12000 rows 114 and 117, 8192 86 and
+    // 85, 6000 70 and 68 (2048 -> 2048 the same within a us).  Where 256 is not a multiple
+    // of the tiles it gains more, and sooner: 9000 -> 500, 142 tiles, of 16384 rows 217 and
+    // 373, 8192 118 and 190, 6000, which the rule leaves in 142 workgroups, 93 and 141.
     const size_t bytes = (size_t)d.outputs * d.inputs * sizeof(float);
     const int one_round = tiles < 256 ? (int)(256 / tiles) : 1;
     int each = whole_turns(stages), slices = one_round;

@@ -192,7 +192,9 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G)
 k_norm_fwd(const typename Elem<TYPE>::T *x, typename Elem<TYPE>::T *y, Fwd a)
 {
     constexpr int VEC = Row<TYPE>::VEC, NT = G < 256 ? 256 : G, AT_ONCE = NT / G;
-    constexpr bool HOLD = I <= 2, AHEAD = G < 1024 || !KEEP;  // (registers)
+    // (registers: 1024 threads have 128 each; with a checkpoint of 16-bit rows an address of
+    // two lies in memory and is read back for each row)
+    constexpr bool HOLD = I <= 2, AHEAD = G < 1024 || !KEEP;
     using T = typename Elem<TYPE>::T;
     __shared__ double sh[2][2 * NT / 64];
     const int t = threadIdx.x % G, step = (int)gridDim.x * AT_ONCE;
@@ -421,7 +423,8 @@ __device__ __forceinline__ float2 stats_of(const Bwd &a, int r)
 }
 
 // A workgroup of 1024 threads has 128 registers each: with four chunks a thread and
-// four ahead, the sums of the parameters' gradients lie in LDS.
+// four ahead, the sums of the parameters' gradients lie in LDS (and, from a checkpoint, one
+// value for after the rows in memory).
 template <int G, int I> constexpr int bwd_lds()
 {
     return G == 1024 && I == 4 ? 2 * 1024 * I * (int)sizeof(float4) : 0;
@@ -791,11 +794,11 @@ Plan bwd_plan(const ach_layernorm_desc &d)
     const int chunks = chunks_of(d);
     if (!for_bwd_kind(chunks, bwd_chunks(d.type), [&](auto k) {
             const int at_once = k.NT / k.G, all = (d.rows + at_once - 1) / at_once;
-            // at least so many that no chain of sums is longer than 256 rows
-            // two a compute unit, of large ones that fill its registers one (300 x 8000 fp16 14 us,
-            // with two 17, four chunks of each of 256 threads 18), and of those of 512 threads
-            // that share it also where the partial sums are a large part of the work (700 x
-            // 3000 fp32 12 and 13, 10000 rows 91 and 71)
+            // Two a compute unit.  One of those whose registers fill it (1024 and 768 threads, 512
+            // with 16-bit rows: 300 x 8000 fp16 14 us, two 17, four chunks of each of 256 threads
+            // 18), and one of 512 threads with fp32 rows, which would share it, where the partial
+            // sums are a large part of the work (700 x 3000 12 and 13, 10000 rows 91 and 71).
+            // More, where a chain of sums would be longer than 256 rows.
             const bool one = k.NT > 512 || (k.NT == 512 && (d.type != ACH_F32 || d.rows <= 1024));
             p.grid = min(all, max(one ? 256 : 512, (all + 255) / 256));
             // of 1024 threads no more than take equally many turns (1027 x 13001 with 206
