@@ -1625,7 +1625,7 @@ void *an_layer_buffer(an_network *net, int li, int which, size_t *count)
     case 9: p = l->rolling_variance; n = (size_t)l->n; break;
     case 10: p = l->mean; n = (size_t)l->n; break;
     case 11: p = l->variance; n = (size_t)l->n; break;
-    case 12: p = l->x_kept ? NULL : l->x; n = bo; break;
+    case 12: p = l->x == net->x_shared ? NULL : l->x; n = bo; break;
     case 14: p = l->indexes; n = bo; break;
     case 15: p = l->loss; n = bo; break;
     case 16: p = l->stats; n = 2 * (size_t)l->batch; break;

@@ -476,8 +476,8 @@ uint64_t an_seen(const an_network *net);
 int an_iteration(const an_network *net);
 /* device buffer of a layer: which = 0 output, 1 delta, 2 weights,
  * 3 weight_updates, 4 biases, 5 bias_updates, 6 scales, 7 scale_updates,
- * 8 rolling_mean, 9 rolling_variance, 10 mean, 11 variance, 12 x (pre-BN),
- * (NULL with an_set_checkpoints), 14 indexes (int32), 15 loss, 16 stats of a
+ * 8 rolling_mean, 9 rolling_variance, 10 mean, 11 variance, 12 x (pre-BN;
+ * NULL where layers share it), 14 indexes (int32), 15 loss, 16 stats of a
  * layer norm, 17 x's checkpoint (bytes); *count = elements (0 if absent)    */
 void *an_layer_buffer(an_network *net, int layer, int which, size_t *count);
 /* bytes of device memory that an_finalize took for the layers               */

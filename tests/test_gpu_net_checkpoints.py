@@ -38,6 +38,7 @@ def kept_bytes(n):
 def test_layers_without_a_backward_keep_nothing(gpu, options, reached):
     everything, net = build(True), build(True, options)
     assert [i for i in range(3) if net.buffer(i, 17) is not None] == reached
+    assert all(net.buffer(i, 12) is None for i in range(3))  # one buffer of all of them
     less = sum(kept_bytes(n) for i, n in enumerate(SIZES) if i not in reached)
     assert abs(everything.device_bytes() - net.device_bytes() - less) <= 3 * 256
     everything.close()
